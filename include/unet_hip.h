@@ -570,6 +570,60 @@ int uh_cldice_backward(int planes, int H, int W, const float* y_true, const floa
  * (sum t*p, sum t, sum p, sum skel_p*t, sum skel_p, sum skel_t*p, sum skel_t) */
 int uh_cldice_read_terms(const float* workspace, int planes, int H, int W, float* out17, uh_stream s);
 
+/* ---- class logits: log probabilities of labels, distillation from a teacher's top logits ----------------------------
+ * A row is one prediction over `classes` classes.  Row r = o*inner + i (o < outer, i < inner) has its logit of class c at
+ * element o*so + i*si + c*sc of the tensor: [N][C] rows have inner = 1, class maps [B][C][H][W] have inner = H*W.  At most
+ * 2^31 - 1 rows and UH_CLASSES_MAX classes.  Per-row tensors (labels, log_prob, weight, ...) are dense, in the order of r;
+ * tensors with k entries per row (alternatives, slots) are dense [outer][k][inner].  Every call reads all it needs while it
+ * runs on `stream`; nothing is kept. */
+enum { UH_F32 = 0, UH_BF16 = 1, UH_F16 = 2 };
+enum { UH_CLASSES_MAX = 1 << 20, UH_TOP_MAX = 64, UH_SLOTS_MAX = 256 };
+typedef struct {
+  long long outer, inner, so, si, sc;
+  int classes, dtype;
+} uh_class_view;
+/* a teacher's slots: values (UH_F32 / UH_BF16 / UH_F16) and class indices of 4 or 8 bytes; index < 0 = free slot */
+typedef struct {
+  const void *value, *index;
+  int slots, value_dtype, index_bytes;
+} uh_slots;
+
+/* z = (x - max x)/temperature, s = sum e^z:  log_prob = z[label] - ln s (fp32; only with labels, of 4 or 8 bytes),
+ * entropy = ln s - (sum e^z z)/s, and the `top` largest logits > -inf (equal ones: lowest class first) as
+ * top_log_prob = z - ln s with top_index their classes; places left over hold -inf and -1.
+ * label == ignore_index: log_prob = entropy = 0, no alternatives.  A label outside [0, classes): log_prob = NaN.
+ * A row with a NaN or +inf: NaN everywhere, indices -1.  A row of -inf: log_prob = -inf, entropy = 0, no alternatives.
+ * stats (may be NULL): [rows][2] fp32 for the backward call.  workspace: uh_label_log_probs_workspace() bytes. */
+size_t uh_label_log_probs_workspace(const uh_class_view* view, int top);
+int uh_label_log_probs(const uh_class_view* view, const void* logits, const void* labels, int label_bytes,
+                       long long ignore_index, int top, float temperature, float* log_prob, float* entropy,
+                       float* top_log_prob, int* top_index, float* stats, void* workspace, size_t workspace_bytes,
+                       uh_stream s);
+/* dlogits_j = [g (delta(j,label) - p_j) - h p_j (ln p_j + entropy)] / temperature, in the logits' type, laid out by
+ * out_view; g = g_log_prob, h = g_entropy (fp32 per row, either may be NULL).  Ignored rows and rows of -inf get zeros. */
+int uh_label_log_probs_bwd(const uh_class_view* view, const uh_class_view* out_view, const void* logits,
+                           const void* labels, int label_bytes, long long ignore_index, float temperature,
+                           const float* stats, const float* entropy, const float* g_log_prob, const float* g_entropy,
+                           void* dlogits, uh_stream s);
+
+/* t = softmax over a row's slots of value/T, p = softmax over its classes of x/T:
+ *   loss = scale * sum_rows w T^2 sum_k t_k (ln t_k - ln p[i_k])                (w = weight[r], 1 without weights)
+ *   dlogits_j = g * scale * w T (p_j - sum_{k: i_k = j} t_k)                    (g: gout[0], or grad_scale in the step)
+ * Rows with w = 0 or without a filled slot count as 0 and get zero gradients, whatever they hold.  An index >= classes or a
+ * NaN among a row's slots makes that row's loss and gradient NaN.  The loss is summed in a fixed order.
+ * uh_topk_distill_step gives loss and gradient in one call; stats ([rows][2], may be NULL) carries the rows' statistics
+ * from uh_topk_distill to uh_topk_distill_bwd.  workspace: uh_topk_distill_workspace() bytes, 16-byte aligned. */
+size_t uh_topk_distill_workspace(const uh_class_view* view);
+int uh_topk_distill(const uh_class_view* view, const void* logits, const uh_slots* slots, const float* weight,
+                    float temperature, double scale, float* loss, float* stats, void* workspace, size_t workspace_bytes,
+                    uh_stream s);
+int uh_topk_distill_bwd(const uh_class_view* view, const uh_class_view* out_view, const void* logits,
+                        const uh_slots* slots, const float* weight, float temperature, double scale, const float* gout,
+                        const float* stats, void* dlogits, uh_stream s);
+int uh_topk_distill_step(const uh_class_view* view, const uh_class_view* out_view, const void* logits,
+                         const uh_slots* slots, const float* weight, float temperature, double scale, float grad_scale,
+                         float* loss, void* dlogits, void* workspace, size_t workspace_bytes, uh_stream s);
+
 #ifdef __cplusplus
 }
 #endif

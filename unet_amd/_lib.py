@@ -48,6 +48,18 @@ class ReduceDesc(ctypes.Structure):
 REDUCE_MAX = 24         # UH_REDUCE_MAX
 REDUCE_COLSUM, REDUCE_WGRAD = 0, 1
 
+class ClassView(ctypes.Structure):
+    """uh_class_view: how the class logits of a call lie in memory"""
+    _fields_ = [("outer", L), ("inner", L), ("so", L), ("si", L), ("sc", L), ("classes", I), ("dtype", I)]
+
+
+class Slots(ctypes.Structure):
+    """uh_slots: a teacher's top logits and their classes"""
+    _fields_ = [("value", P), ("index", P), ("slots", I), ("value_dtype", I), ("index_bytes", I)]
+
+
+CLASSES_MAX, TOP_MAX, SLOTS_MAX = 1 << 20, 64, 256      # UH_CLASSES_MAX, UH_TOP_MAX, UH_SLOTS_MAX
+
 # name -> (restype, argtypes); mirrors include/unet_hip.h one to one
 SIGNATURES = {
     "uh_last_error": (ctypes.c_char_p, []),
@@ -164,6 +176,13 @@ SIGNATURES = {
     "uh_cldice_forward_pred": (I, [I, I, I, P, P, F, F, P, P, P]),
     "uh_cldice_backward": (I, [I, I, I, P, P, P, P, P, P]),
     "uh_cldice_read_terms": (I, [P, I, I, I, P, P]),
+    "uh_label_log_probs_workspace": (Z, [P, I]),
+    "uh_label_log_probs": (I, [P, P, P, I, L, I, F, P, P, P, P, P, P, Z, P]),
+    "uh_label_log_probs_bwd": (I, [P, P, P, P, I, L, F, P, P, P, P, P, P]),
+    "uh_topk_distill_workspace": (Z, [P]),
+    "uh_topk_distill": (I, [P, P, P, P, F, D, P, P, P, Z, P]),
+    "uh_topk_distill_bwd": (I, [P, P, P, P, P, F, D, P, P, P, P]),
+    "uh_topk_distill_step": (I, [P, P, P, P, P, F, D, F, P, P, P, Z, P]),
 }
 
 EPI_RAW_STATS, EPI_AFFINE_RELU, EPI_MASKED, EPI_CONVT, EPI_MASKED_BNBWD = 0, 1, 2, 3, 4

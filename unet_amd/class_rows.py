@@ -1,0 +1,115 @@
+"""Where the logits of a call over classes lie: the `uh_class_view` of a tensor and a class dimension, and the checks that
+`label_log_probs` and `topk_distill` share."""
+import ctypes
+
+import torch
+
+from . import _lib
+
+DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # UH_F32, UH_BF16, UH_F16
+INT_BYTES = {torch.int32: 4, torch.int64: 8}
+
+
+def _merge(sizes, strides):
+    """(elements, stride) of the dimensions seen as one, or None if no single stride walks them"""
+    n, step = 1, 1
+    for size, stride in zip(reversed(sizes), reversed(strides)):
+        if size == 1:
+            continue
+        if n == 1:
+            step = stride
+        elif stride != n * step:
+            return None
+        n *= size
+    return n, step
+
+
+class Rows:
+    """The logits of one call as rows of classes: `x` (the tensor, or a dense copy where no two strides describe it), its
+    view for the kernels, the shape of what belongs to a row, and the shape of k entries per row."""
+    __slots__ = ("x", "view", "rows", "classes", "row_shape", "dim", "device", "switch", "stream")
+
+    def __init__(self, logits, dim, what):
+        if not torch.is_tensor(logits) or logits.dtype not in DTYPE_CODE:
+            raise ValueError(f"{what}: logits must be a fp32, bf16 or fp16 tensor")
+        nd = logits.dim()
+        if nd < 1 or not -nd <= dim < nd:
+            raise ValueError(f"{what}: no class dimension {dim} in logits of shape {tuple(logits.shape)}")
+        self.dim = dim = dim % nd
+        shape = logits.shape
+        self.classes = shape[dim]
+        if not 0 < self.classes <= _lib.CLASSES_MAX:
+            raise ValueError(f"{what}: {self.classes} classes (1 to {_lib.CLASSES_MAX})")
+        self.row_shape = shape[:dim] + shape[dim + 1:]
+        self.rows = logits.numel() // self.classes
+        if self.rows > 0x7fffffff:
+            raise ValueError(f"{what}: {self.rows} rows (at most 2^31 - 1)")
+        self.x = logits.detach()
+        self.view = self._view(self.x) if self.rows else None
+        if self.rows and self.view is None:
+            self.x = self.x.contiguous()
+            self.view = self._view(self.x)
+        self.device = logits.device
+
+    def bind(self, what):
+        """after the checks of the arguments: the stream of the launches (the tensors' device's current one)"""
+        if self.device.type != "cuda":
+            raise RuntimeError(f"unet_amd.{what} runs on the HIP kernels only: tensors must be on a ROCm device")
+        # a launch goes to the current device: make the tensors' own the current one around it if it is another
+        self.switch = self.device.index != torch.cuda.current_device()
+        self.stream = torch.cuda.current_stream(self.device).cuda_stream
+        return self
+
+    def _view(self, t):
+        dim, shape, strides = self.dim, t.shape, t.stride()
+        outer = _merge(shape[:dim], strides[:dim])
+        inner = _merge(shape[dim + 1:], strides[dim + 1:])
+        if outer is None or inner is None:
+            return None
+        return _lib.ClassView(outer[0], inner[0], outer[1], inner[1], strides[dim] if shape[dim] > 1 else 1, shape[dim],
+                              DTYPE_CODE[t.dtype])
+
+    def new_grad(self):
+        """an empty gradient tensor (the logits' strides where those are dense) and its view"""
+        g = torch.empty_like(self.x)
+        view = self._view(g)
+        if view is None:
+            g = torch.empty_like(self.x, memory_format=torch.contiguous_format)
+            view = self._view(g)
+        return g, view
+
+    def entries(self, k):
+        """shape of a tensor with k entries per row in the place of the classes"""
+        return self.row_shape[:self.dim] + (k,) + self.row_shape[self.dim:]
+
+    def per_row(self, t, what, dtypes):
+        """a tensor with one value per row, dense in the rows' order"""
+        if not torch.is_tensor(t) or t.shape != self.row_shape:
+            raise ValueError(f"{what}: expected shape {tuple(self.row_shape)}, got "
+                             f"{tuple(t.shape) if torch.is_tensor(t) else type(t).__name__}")
+        return self.same_device(t, what, dtypes)
+
+    def same_device(self, t, what, dtypes):
+        if t.dtype not in dtypes:
+            raise ValueError(f"{what}: dtype {t.dtype} (expected one of {', '.join(str(d) for d in dtypes)})")
+        if t.device != self.device:
+            raise ValueError(f"{what} is on {t.device}, the logits are on {self.device}")
+        t = t.detach()
+        return t if t.is_contiguous() else t.contiguous()
+
+    def call(self, name, *args):
+        if self.switch:
+            with torch.cuda.device(self.device):
+                _lib.call(name, *args, self.stream)
+        else:
+            _lib.call(name, *args, self.stream)
+
+
+def checked_temperature(temperature, what):
+    t = float(temperature)
+    if not 1e-6 <= t <= 1e6:
+        raise ValueError(f"{what}: temperature {temperature} (1e-6 to 1e6)")
+    return t
+
+
+byref = ctypes.byref

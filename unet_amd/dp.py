@@ -21,6 +21,7 @@ import torch.distributed as dist
 import torch.nn as nn
 
 from . import _lib
+from .distill import TopKDistillLoss
 from .engine import UNetRun, side_stream_for
 from .unet import _Features, FEATURE_LAYERS
 
@@ -375,6 +376,8 @@ class DataParallelTrainer:
         # d(mean over ranks of loss)/dlogits: the 1/world of gradient averaging is folded into the seed
         if self._fused_bce and masks.shape == logits.shape:
             loss, dlogits = bce_with_logits(logits.detach(), masks, 1.0 / self.world)
+        elif isinstance(self.criterion, TopKDistillLoss):      # masks: a teacher's targets
+            loss, dlogits = self.criterion.value_and_grad(logits.detach(), masks, 1.0 / self.world)
         else:
             loss = self.criterion(logits, masks)
             (dlogits,) = torch.autograd.grad(loss / self.world, logits)
@@ -466,7 +469,8 @@ class LUNeXtTrainer:
     (cl_dice.cldice_with_logits).  Inside an initialised process group (unless standalone) the flat gradient is
     all-reduced once per step (14 MB: one collective) and 1/world is folded into the loss gradient.
 
-    criterion: "cl_dice", "bce" or a callable (logits, masks) -> loss, differentiated by autograd at the logits."""
+    criterion: "cl_dice", "bce", a TopKDistillLoss (train_step's masks are then a teacher's targets) or a callable
+    (logits, masks) -> loss, differentiated by autograd at the logits."""
 
     def __init__(self, model, lr=1e-3, criterion="bce", process_group=None, standalone=False):
         from .lunext import flat_param_order
@@ -491,6 +495,8 @@ class LUNeXtTrainer:
             return cldice_with_logits(masks, logits, grad_scale=scale, prepared=prepared)
         if c == "bce" and masks.shape == logits.shape:
             return bce_with_logits(logits, masks, scale)
+        if isinstance(c, TopKDistillLoss):                     # masks: a teacher's targets
+            return c.value_and_grad(logits, masks, scale)
         fn = nn.BCEWithLogitsLoss() if c == "bce" else c
         lg = logits.detach().requires_grad_(True)
         loss = fn(lg, masks)
