@@ -5,99 +5,505 @@
 //     dx_j = [ g (delta(j, label) - p_j) - h p_j (ln p_j + H) ] / T        (g, h: gradients of log_prob and H)
 #include "class_rows.h"
 
-// ---- one workgroup per row, any strides -------------------------------------------------------------------------------
+struct LpArgs {
+  RowView v;
+  long long rows;
+  const void* labels;
+  long long ignore;
+  int label_bytes, top;
+  float temperature, c2;
+  float *log_prob, *entropy, *top_lp;
+  int* top_idx;
+  float* stats;
+
+  __device__ __forceinline__ long long label(long long r) const { return labels ? load_int(labels, label_bytes, r) : -1; }
+  __device__ __forceinline__ bool ignored(long long l) const { return labels && l == ignore; }
+  // by one thread: a row that is not judged; its alternatives are written with write_top(.., 0, ..)
+  __device__ __forceinline__ void write_ignored(long long r) const {
+    log_prob[r] = 0.f;
+    entropy[r] = 0.f;
+    if (stats) { stats[2 * r] = 0.f; stats[2 * r + 1] = 0.f; }
+  }
+  // by one thread: values of a row; x_label: its label's logit where the label is a class.  Returns ln s.
+  __device__ __forceinline__ float write_row(long long r, long long l, float x_label, const RowStat& s) const {
+    const float ln_s = RowRef(s.m, c2).ln_s(s.m, s.s);
+    // ln s = log(s) - d and t share d (the rounding of M), so that the entropy takes log(s) itself
+    entropy[r] = s.s == 0.f ? 0.f : logf(s.s) - (s.t / s.s) * UH_LN2;
+    if (labels)
+      log_prob[r] = l < 0 || l >= v.C ? NAN : s.s == 0.f ? -INFINITY : scaled(x_label, s.m, temperature) - ln_s;
+    if (stats) { stats[2 * r] = s.m; stats[2 * r + 1] = s.s; }
+    return ln_s;
+  }
+  __device__ __forceinline__ bool is_class(long long l) const { return l >= 0 && l < v.C; }
+  // one alternative; cls < 0: the place is left over; undefined rows have s = NaN
+  __device__ __forceinline__ void write_top(long long r, int k, float value, int cls, float m, float ln_s, float s) const {
+    const bool undefined = !(s >= 0.f);
+    const long long e = v.entry(r, k, top);
+    top_lp[e] = undefined ? NAN : cls >= 0 ? scaled(value, m, temperature) - ln_s : -INFINITY;
+    top_idx[e] = undefined ? -1 : cls;
+  }
+};
+
+// ---- rows whose classes lie side by side: G lanes a row, the row in registers -------------------------------------------------
+// LIST > 0 (G = 16): up to LIST alternatives from the lanes' own falling lists; TOP (G >= 64): any number.
+template <typename T, int G, int NV, int LIST, bool TOP>
+__global__ __launch_bounds__(G > 64 ? G : 64) void lp_group_kernel(LpArgs a, const T* __restrict__ x) {
+  constexpr int RPB = G > 64 ? 1 : 64 / G;
+  constexpr int E = RowRegs<T, G, NV>::E;
+  __shared__ typename Red<G>::Buf red;
+  const int lane = threadIdx.x % G;
+  const int C = a.v.C;
+  const long long blocks = (a.rows + RPB - 1) / RPB;
+  for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const long long r = b * RPB + threadIdx.x / G;
+    const bool there = r < a.rows;
+    const long long l = there ? a.label(r) : 0;
+    const bool off = !there || a.ignored(l);
+    if (off) {
+      if (there) {
+        if (lane == 0) a.write_ignored(r);
+        for (int k = lane; k < a.top; k += G) a.write_top(r, k, 0.f, -1, 0.f, 0.f, 0.f);
+      }
+      if (RPB == 1) continue;                              // the whole workgroup's row
+    }
+    RowRegs<T, G, NV> reg;
+    const T* row = x + (there ? a.v.base(r) : 0);
+    if (!off) reg.load(row, C, lane);
+    const float lm = off ? -INFINITY : reg.lane_max(C);
+    RowStat s;
+    s.m = Red<G>::max_(lm, red);
+    if (s.m == -INFINITY) s.m = 0.f;
+    reg.fresh();
+    reg.template lane_sums<true>(RowRef(s.m, a.c2), C, s.s, s.t);
+    Red<G>::sum2(s.s, s.t, red);
+    float ln_s = 0.f;
+    if (!off) {
+      if (lane == 0) ln_s = a.write_row(r, l, a.is_class(l) ? ld(row + l) : 0.f, s);
+      else if (LIST > 0 || TOP) ln_s = RowRef(s.m, a.c2).ln_s(s.m, s.s);
+    }
+    if constexpr (LIST > 0) {
+      typedef SmallKey<T> SK;
+      typename SK::K list[LIST] = {};
+      reg.fresh();
+      if (!off) {
+#pragma unroll
+        for (int q = 0; q < NV; ++q)
+          if (q * G * E < C) {
+            const int e = RowRegs<T, G, NV>::first(q, lane, C);
+#pragma unroll
+            for (int j = 0; j < E; ++j) list_insert(list, SK::make(reg.get(q, j), e + j));
+          }
+      }
+      for (int k = 0; k < a.top; ++k) {
+        const typename SK::K best = group_max<G>(list[0]);
+        if (list[0] == best && best != 0) {
+          a.write_top(r, k, SK::val(best), SK::cls(best), s.m, ln_s, s.s);
+#pragma unroll
+          for (int i = 0; i + 1 < LIST; ++i) list[i] = list[i + 1];
+          list[LIST - 1] = 0;
+        } else if (best == 0 && lane == 0 && !off) {
+          a.write_top(r, k, 0.f, -1, s.m, ln_s, s.s);
+        }
+      }
+    }
+    if constexpr (TOP) {
+      __shared__ TopBuf<G> tb;
+      group_top<T, G, NV>(reg, row, C, lane, 0, a.top, lm, tb, red, [&](int k, uint64_t key) {
+        a.write_top(r, k, key_value(key), key ? key_class(key) : -1, s.m, ln_s, s.s);
+      });
+    }
+  }
+}
+
+// ---- long rows, or few of them: a workgroup takes one part of a row, a wave joins a row's parts ---------------------------------
+// part_stat[row][part] = (m, s, t); part_top[row][part][top]: rank keys, falling, 0 behind the last
+template <typename T, int NV, bool TOP>
+__global__ __launch_bounds__(256) void lp_part_kernel(LpArgs a, const T* __restrict__ x, int parts, int part_len,
+                                                      RowStat* __restrict__ part_stat, uint64_t* __restrict__ part_top) {
+  __shared__ Red<256>::Buf red;
+  const long long r = blockIdx.x;
+  const int part = blockIdx.y, c0 = part * part_len, lane = threadIdx.x;
+  if (a.ignored(a.label(r))) return;                       // the joining wave does not look at the parts of such a row
+  const int n = min(part_len, a.v.C - c0);
+  RowRegs<T, 256, NV> reg;
+  const T* row = x + a.v.base(r) + c0;
+  reg.load(row, n, lane);
+  const float lm = reg.lane_max(n);
+  RowStat s;
+  s.m = Red<256>::max_(lm, red);
+  if (s.m == -INFINITY) s.m = 0.f;
+  reg.fresh();
+  reg.template lane_sums<true>(RowRef(s.m, a.c2), n, s.s, s.t);
+  Red<256>::sum2(s.s, s.t, red);
+  if (lane == 0) part_stat[r * parts + part] = s;
+  if constexpr (TOP) {
+    __shared__ TopBuf<256> tb;
+    uint64_t* out = part_top + (r * parts + part) * a.top;
+    group_top<T, 256, NV>(reg, row, n, lane, c0, a.top, lm, tb, red, [&](int k, uint64_t key) { out[k] = key; });
+  }
+}
+
 template <typename T>
-__global__ __launch_bounds__(256) void label_probs_any_kernel(RowView v, long long rows, const T* __restrict__ x,
-                                                              const void* __restrict__ labels, int label_bytes,
-                                                              long long ignore, int top, float temperature, float c2,
-                                                              float* __restrict__ log_prob, float* __restrict__ entropy,
-                                                              float* __restrict__ top_lp, int* __restrict__ top_idx,
-                                                              float* __restrict__ stats) {
-  __shared__ float fbuf[4];
-  __shared__ uint64_t kbuf[4];
-  for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
-    const long long label = labels ? load_int(labels, label_bytes, r) : 0;
-    const bool ignored = labels && label == ignore;
-    if (ignored) {
-      if (threadIdx.x == 0) {
-        log_prob[r] = 0.f;
-        entropy[r] = 0.f;
-        if (stats) { stats[2 * r] = 0.f; stats[2 * r + 1] = INFINITY; }
-      }
-      for (int k = threadIdx.x; k < top; k += 256) {
-        top_lp[v.entry(r, k, top)] = -INFINITY;
-        top_idx[v.entry(r, k, top)] = -1;
-      }
+__global__ __launch_bounds__(64) void lp_join_kernel(LpArgs a, const T* __restrict__ x, int parts, const RowStat* __restrict__ part_stat,
+                                                     const uint64_t* __restrict__ part_top) {
+  extern __shared__ uint64_t keys[];                       // parts * top of them
+  __shared__ int count;
+  const long long r = blockIdx.x;
+  const int lane = threadIdx.x;
+  const long long l = a.label(r);
+  if (a.ignored(l)) {
+    if (lane == 0) a.write_ignored(r);
+    for (int k = lane; k < a.top; k += 64) a.write_top(r, k, 0.f, -1, 0.f, 0.f, 0.f);
+    return;
+  }
+  RowStat s = lane < parts ? part_stat[r * parts + lane] : RowStat{0.f, 0.f, 0.f};
+  for (int o = 32; o > 0; o >>= 1) {
+    const RowStat u{__shfl_xor(s.m, o, 64), __shfl_xor(s.s, o, 64), __shfl_xor(s.t, o, 64)};
+    s = lane & o ? join(u, s, a.c2) : join(s, u, a.c2);    // the same order of the two in both lanes
+  }
+  const float ln_s = RowRef(s.m, a.c2).ln_s(s.m, s.s);
+  if (lane == 0) a.write_row(r, l, a.is_class(l) ? ld(x + a.v.base(r) + l) : 0.f, s);
+  if (a.top == 0) return;
+  // the best of the parts' last places bounds the row's last place from below
+  const uint64_t* mine = part_top + (r * parts + lane) * a.top;
+  const uint64_t cut = group_max<64>(lane < parts ? mine[a.top - 1] : (uint64_t)0);
+  if (lane == 0) count = 0;
+  __syncthreads();
+  if (lane < parts)
+    for (int k = 0; k < a.top; ++k) {
+      const uint64_t key = mine[k];
+      if (key < cut || key == 0) break;
+      keys[atomicAdd(&count, 1)] = key;
+    }
+  __syncthreads();
+  wave_select(keys, count, a.top, [&](int k, uint64_t key) {
+    a.write_top(r, k, key_value(key), key ? key_class(key) : -1, s.m, ln_s, s.s);
+  });
+}
+
+// ---- one thread per row ----------------------------------------------------------------------------------------------------------
+// up to 64 classes in registers (CREG), side by side through LDS (STAGED) or apart; LIST alternatives a sweep
+template <typename T, int CREG, bool STAGED, int LIST>
+__global__ __launch_bounds__(64) void lp_thread_kernel(LpArgs a, const T* __restrict__ x, bool wide) {
+  extern __shared__ __align__(16) char lds[];
+  T* tile = reinterpret_cast<T*>(lds);
+  const int lane = threadIdx.x, C = a.v.C;
+  const long long blocks = (a.rows + 63) / 64;
+  for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const long long r = b * 64 + lane;
+    const bool there = r < a.rows;
+    const T* row;
+    if (STAGED) {
+      const int here = (int)min(64ll, a.rows - b * 64);
+      __syncthreads();
+      copy_to_lds(tile, x + b * 64 * a.v.so, (int)((here - 1) * a.v.so) + C);
+      __syncthreads();
+      row = tile + lane * (int)a.v.so;
+    } else {
+      row = x + (there ? a.v.base(r) : 0);
+    }
+    if (!there) continue;
+    const long long l = a.label(r);
+    if (a.ignored(l)) {
+      a.write_ignored(r);
+      for (int k = 0; k < a.top; ++k) a.write_top(r, k, 0.f, -1, 0.f, 0.f, 0.f);
       continue;
     }
-    const T* row = x + v.base(r);
-    const RowStat st = block_row_stat(row, v.C, v.sc, c2, fbuf);
-    const float ln_s = logf(st.s), m = st.m;
-    const bool undefined = !(st.s >= 0.f);
-    if (threadIdx.x == 0) {
-      entropy[r] = st.s == 0.f ? 0.f : ln_s - (st.t / st.s) * UH_LN2;
-      if (labels)
-        log_prob[r] = label < 0 || label >= v.C ? NAN
-                      : st.s == 0.f             ? -INFINITY
-                                                : scaled(ld(row + label * v.sc), m, temperature) - ln_s;
-      if (stats) { stats[2 * r] = m; stats[2 * r + 1] = stat_l2(st.s); }
-    }
-    uint64_t last = ~0ull;
-    for (int k = 0; k < top; ++k) {
-      uint64_t best = 0;
-      if (last && !undefined)
-        for (int c = threadIdx.x; c < v.C; c += 256) {
-          const uint64_t key = rank_key(ld(row + c * v.sc), c);
-          if (key < last && key > best) best = key;
+    float v[CREG];
+    load_classes<T, CREG, STAGED>(v, row, a.v.sc, C, wide);
+    const RowStat s = thread_row_stat<CREG, true>(v, C, a.c2);
+    const float ln_s = a.write_row(r, l, a.is_class(l) ? ld(row + (STAGED ? l : l * a.v.sc)) : 0.f, s);
+    if constexpr (LIST > 0) {
+      typedef SmallKey<T> SK;
+      typename SK::K last = ~(typename SK::K)0;
+      for (int k0 = 0; k0 < a.top; k0 += LIST) {
+        typename SK::K list[LIST] = {};
+        if constexpr (STAGED || CREG == 64) {              // from LDS or the caches again: 64 unrolled steps cost 256 registers
+          for (int c = 0; c < C; ++c) {
+            const typename SK::K key = SK::make((float)row[STAGED ? c : c * a.v.sc], c);
+            list_insert(list, key < last ? key : 0);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < CREG; ++c)
+            if (c < C) {
+              const typename SK::K key = SK::make(v[c], c);
+              list_insert(list, key < last ? key : 0);
+            }
         }
-      best = block_max(best, kbuf);
-      if (threadIdx.x == 0) {
-        top_lp[v.entry(r, k, top)] = undefined ? NAN : best ? scaled(key_value(best), m, temperature) - ln_s : -INFINITY;
-        top_idx[v.entry(r, k, top)] = best ? key_class(best) : -1;
+#pragma unroll
+        for (int i = 0; i < LIST; ++i)
+          if (k0 + i < a.top) a.write_top(r, k0 + i, SK::val(list[i]), list[i] ? SK::cls(list[i]) : -1, s.m, ln_s, s.s);
+        last = list[LIST - 1];
       }
+    }
+  }
+}
+
+// more classes, lying apart: the thread walks its row, once for the statistics and once for every LIST alternatives
+template <typename T, int LIST>
+__global__ __launch_bounds__(64) void lp_walk_kernel(LpArgs a, const T* __restrict__ x) {
+  const long long r = (long long)blockIdx.x * 64 + threadIdx.x;
+  if (r >= a.rows) return;
+  const int C = a.v.C;
+  const T* row = x + a.v.base(r);
+  const long long l = a.label(r);
+  if (a.ignored(l)) {
+    a.write_ignored(r);
+    for (int k = 0; k < a.top; ++k) a.write_top(r, k, 0.f, -1, 0.f, 0.f, 0.f);
+    return;
+  }
+  const RowStat s = walk_row_stat(row, a.v.sc, C, a.c2);
+  const float ln_s = a.write_row(r, l, a.is_class(l) ? ld(row + l * a.v.sc) : 0.f, s);
+  if constexpr (LIST > 0) {
+    uint64_t last = ~0ull;
+    for (int k0 = 0; k0 < a.top; k0 += LIST) {
+      uint64_t list[LIST] = {};
+      for (int c0 = 0; c0 < C; c0 += 8) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c0 + j < C ? ld(row + (c0 + j) * a.v.sc) : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint64_t key = rank_key(v[j], c0 + j);
+          if (key > list[LIST - 1] && key < last) list_insert(list, key);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < LIST; ++i)
+        if (k0 + i < a.top) a.write_top(r, k0 + i, key_value(list[i]), list[i] ? key_class(list[i]) : -1, s.m, ln_s, s.s);
+      last = list[LIST - 1];
+    }
+  }
+}
+
+// ---- one workgroup per row, any strides ----------------------------------------------------------------------------------------
+template <typename T> __global__ __launch_bounds__(256) void lp_any_kernel(LpArgs a, const T* __restrict__ x) {
+  __shared__ Red<256>::Buf red;
+  const int lane = threadIdx.x, C = a.v.C;
+  for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const long long l = a.label(r);
+    if (a.ignored(l)) {
+      if (lane == 0) a.write_ignored(r);
+      for (int k = lane; k < a.top; k += 256) a.write_top(r, k, 0.f, -1, 0.f, 0.f, 0.f);
+      continue;
+    }
+    const T* row = x + a.v.base(r);
+    const RowStat s = strided_row_stat<T, 256>(row, C, a.v.sc, a.c2, lane, red);
+    float ln_s = 0.f;
+    if (lane == 0) ln_s = a.write_row(r, l, a.is_class(l) ? ld(row + l * a.v.sc) : 0.f, s);
+    uint64_t last = ~0ull;
+    for (int k = 0; k < a.top; ++k) {
+      uint64_t best = 0;
+      for (int c = lane; c < C; c += 256) {
+        const uint64_t key = rank_key(ld(row + c * a.v.sc), c);
+        if (key < last && key > best) best = key;
+      }
+      best = Red<256>::maxkey(best, red);
+      if (lane == 0) a.write_top(r, k, key_value(best), best ? key_class(best) : -1, s.m, ln_s, s.s);
       last = best;
     }
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void label_probs_bwd_any_kernel(RowView v, RowView vo, long long rows,
-                                                                  const T* __restrict__ x, const void* __restrict__ labels,
-                                                                  int label_bytes, long long ignore, float inv_t, float c2,
-                                                                  const float* __restrict__ stats,
-                                                                  const float* __restrict__ entropy,
-                                                                  const float* __restrict__ g_lp,
-                                                                  const float* __restrict__ g_ent, T* __restrict__ dx) {
-  for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
-    const long long label = labels ? load_int(labels, label_bytes, r) : -1;
-    const T* row = x + v.base(r);
-    T* out = dx + vo.base(r);
-    if (labels && label == ignore) {
-      for (int c = threadIdx.x; c < v.C; c += 256) st(out + c * vo.sc, 0.f);
+// ---- gradient ---------------------------------------------------------------------------------------------------------------------
+struct LpBwd {
+  RowView v, vo;
+  long long rows;
+  const void* labels;
+  long long ignore;
+  int label_bytes;
+  float inv_t, c2;
+  const float *stats, *entropy, *g_lp, *g_ent;
+};
+// dx = e (b z + a) with e = 2^z, z = c x - M: the row's 1/s and ln s are folded into a and b
+struct LpCoef {
+  float a, b, own, m;
+  int label;              // -1: none
+  bool off;
+  __device__ __forceinline__ LpCoef(const LpBwd& k, long long r) {
+    const long long l = k.labels ? load_int(k.labels, k.label_bytes, r) : -1;
+    off = k.labels && l == k.ignore;
+    m = k.stats[2 * r];
+    const float s = k.stats[2 * r + 1];
+    const float g = k.g_lp ? k.g_lp[r] : 0.f, h = k.g_ent ? k.g_ent[r] : 0.f;
+    const float l2 = log2f(s), inv = 1.f / s;
+    const bool bad = k.g_lp && (l < 0 || l >= k.v.C);
+    b = -h * UH_LN2 * k.inv_t;
+    a = bad ? NAN : (-(g + h * k.entropy[r]) * k.inv_t - b * l2) * inv;
+    b *= inv;
+    own = g * k.inv_t;
+    label = l >= 0 && l < k.v.C && k.g_lp ? (int)l : -1;
+    if (s == 0.f || off) a = b = own = 0.f, label = -1;
+  }
+  __device__ __forceinline__ float of(const RowRef& ref, float x) const {
+    const float z = ref.z(x);
+    return ex2(z) * fmaf(b, fmaxf(z, UH_ZMIN), a);
+  }
+};
+
+template <typename T, int G, int NV>
+__global__ __launch_bounds__(G > 64 ? G : 64) void lp_bwd_group_kernel(LpBwd k, const T* __restrict__ x, T* __restrict__ dx, int part_len) {
+  constexpr int RPB = G > 64 ? 1 : 64 / G;
+  const int lane = threadIdx.x % G, c0 = blockIdx.y * part_len;
+  const int n = min(part_len, k.v.C - c0);
+  const long long blocks = (k.rows + RPB - 1) / RPB;
+  for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const long long r = b * RPB + threadIdx.x / G;
+    if (r >= k.rows) continue;
+    const LpCoef q(k, r);
+    T* out = dx + k.vo.base(r) + c0;
+    RowRegs<T, G, NV> reg;
+    if (q.off) {
+      reg.map_store(out, n, lane, [](float) { return 0.f; });
       continue;
     }
-    const float m = stats[2 * r], l2 = stats[2 * r + 1];
-    const float g = g_lp ? g_lp[r] : 0.f, h = g_ent ? g_ent[r] : 0.f;
-    float a = -(g + h * entropy[r]) * inv_t;
-    const float b = -h * UH_LN2 * inv_t;
-    const float own = l2 == INFINITY ? 0.f : g * inv_t;
-    if (g_lp && (label < 0 || label >= v.C)) a = NAN;
-    for (int c = threadIdx.x; c < v.C; c += 256) {
-      const float l = (ld(row + c * v.sc) - m) * c2 - l2;
-      float d = ex2(l) * fmaf(b, fmaxf(l, UH_ZMIN), a);
-      if (c == label) d += own;
-      st(out + c * vo.sc, d);
-    }
+    const T* row = x + k.v.base(r) + c0;
+    reg.load(row, n, lane);
+    const RowRef ref(q.m, k.c2);
+    reg.map_store(out, n, lane, [&](float v) { return q.of(ref, v); });
+    // the label's class once more, by the lane that has just written it
+    const int at = q.label - c0;
+    if (at >= 0 && at < n && (at / RowRegs<T, G, NV>::E) % G == lane) st(out + at, q.of(ref, ld(row + at)) + q.own);
   }
 }
 
-// ---- host ---------------------------------------------------------------------------------------------------------------
-static unsigned row_grid(long long rows) { return (unsigned)(rows < (1 << 20) ? rows : (1 << 20)); }
+// up to 64 classes, rows side by side in both tensors
+template <typename T> __global__ __launch_bounds__(64) void lp_bwd_thread_kernel(LpBwd k, const T* __restrict__ x, T* __restrict__ dx, bool wide) {
+  extern __shared__ __align__(16) char lds[];
+  constexpr int E = 16 / sizeof(T);
+  const int lane = threadIdx.x, C = k.v.C, so = (int)k.v.so;
+  T* tile = reinterpret_cast<T*>(lds);
+  T* res = tile + (64 * so + E - 1) / E * E;
+  const long long blocks = (k.rows + 63) / 64;
+  for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const long long r = b * 64 + lane;
+    const int here = (int)min(64ll, k.rows - b * 64);
+    __syncthreads();
+    copy_to_lds(tile, x + b * 64 * so, (here - 1) * so + C);
+    __syncthreads();
+    if (lane < here) {
+      const LpCoef q(k, r);
+      const RowRef ref(q.m, k.c2);
+      const T* row = tile + lane * so;
+      T* out = res + lane * C;
+      if (q.off) {
+        for (int c = 0; c < C; ++c) out[c] = (T)0.f;
+      } else if (wide) {                                   // C and so multiples of 16 bytes
+        for (int c = 0; c < C; c += E) {
+          T v[E];
+          *reinterpret_cast<U4*>(v) = *reinterpret_cast<const U4*>(row + c);
+#pragma unroll
+          for (int j = 0; j < E; ++j) v[j] = (T)(q.of(ref, (float)v[j]) + (c + j == q.label ? q.own : 0.f));
+          *reinterpret_cast<U4*>(out + c) = *reinterpret_cast<const U4*>(v);
+        }
+      } else {
+        for (int c = 0; c < C; ++c) out[c] = (T)(q.of(ref, (float)row[c]) + (c == q.label ? q.own : 0.f));
+      }
+    }
+    __syncthreads();
+    copy_from_lds(dx + b * 64 * C, res, here * C);
+  }
+}
+
+// classes that lie apart: one thread per row
+template <typename T> __global__ __launch_bounds__(64) void lp_bwd_walk_kernel(LpBwd k, const T* __restrict__ x, T* __restrict__ dx) {
+  const long long r = (long long)blockIdx.x * 64 + threadIdx.x;
+  if (r >= k.rows) return;
+  const LpCoef q(k, r);
+  const RowRef ref(q.m, k.c2);
+  const T* row = x + k.v.base(r);
+  T* out = dx + k.vo.base(r);
+  const int C = k.v.C;
+  for (int c0 = 0; c0 < C; c0 += 8) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c0 + j < C && !q.off ? ld(row + (c0 + j) * k.v.sc) : 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c0 + j < C) st(out + (c0 + j) * k.vo.sc, q.off ? 0.f : q.of(ref, v[j]) + (c0 + j == q.label ? q.own : 0.f));
+  }
+}
+
+// one workgroup per row, any strides
+template <typename T> __global__ __launch_bounds__(256) void lp_bwd_any_kernel(LpBwd k, const T* __restrict__ x, T* __restrict__ dx) {
+  for (long long r = blockIdx.x; r < k.rows; r += gridDim.x) {
+    const LpCoef q(k, r);
+    const RowRef ref(q.m, k.c2);
+    const T* row = x + k.v.base(r);
+    T* out = dx + k.vo.base(r);
+    for (int c = threadIdx.x; c < k.v.C; c += 256)
+      st(out + c * k.vo.sc, q.off ? 0.f : q.of(ref, ld(row + c * k.v.sc)) + (c == q.label ? q.own : 0.f));
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------------------
+// how the rows of a forward call are cut (one part: they are not)
+static RowCut lp_cut(const RowView& v, long long rows, int dtype) {
+  return uh_class_path(v, nullptr, rows) == PATH_GROUP ? uh_row_cut(rows, v.C, dtype) : RowCut{1, v.C};
+}
 
 extern "C" size_t uh_label_log_probs_workspace(const uh_class_view* view, int top) {
-  (void)view;
-  (void)top;
-  return 0;
+  if (uh_check_view(view, "label_log_probs_workspace") != UH_OK || top < 0 || top > UH_TOP_MAX) return 0;
+  const long long rows = view->outer * view->inner;
+  const int parts = lp_cut(uh_row_view(view), rows, view->dtype).parts;
+  if (parts == 1) return 0;
+  return (size_t)rows * parts * (16 + 8 * (size_t)top);         // a part's statistics (12 of 16) and its keys
+}
+
+template <typename T> static void lp_launch(const LpArgs& a, const T* x, int dtype, void* ws, hipStream_t s) {
+  constexpr int E = 16 / sizeof(T);
+  const int C = a.v.C;
+  const long long rows = a.rows;
+  const ClassPath path = uh_class_path(a.v, nullptr, rows);
+  const dim3 waves(uh_grid((rows + 63) / 64, UH_GRID_WAVES));
+  if (path == PATH_STAGED || path == PATH_APART) {
+    const bool staged = path == PATH_STAGED, wide = staged && (a.v.so * sizeof(T)) % 16 == 0;
+    const size_t lds = staged ? (size_t)64 * a.v.so * sizeof(T) : 0;
+#define UH_GO3(R, ST, LI) hipLaunchKernelGGL((lp_thread_kernel<T, R, ST, LI>), waves, dim3(64), lds, s, a, x, wide)
+#define UH_GO2(R, ST) do { if (a.top == 0) UH_GO3(R, ST, 0); else if (a.top <= 4) UH_GO3(R, ST, 4); else UH_GO3(R, ST, 8); } while (0)
+#define UH_GO(ST) do { if (C <= 8) UH_GO2(8, ST); else if (C <= 16) UH_GO2(16, ST); else if (C <= 32) UH_GO2(32, ST); else UH_GO2(64, ST); } while (0)
+    if (staged) UH_GO(true); else UH_GO(false);
+#undef UH_GO
+#undef UH_GO2
+#undef UH_GO3
+  } else if (path == PATH_WALK) {
+    const dim3 grid((unsigned)((rows + 63) / 64));
+    if (a.top == 0) hipLaunchKernelGGL((lp_walk_kernel<T, 0>), grid, dim3(64), 0, s, a, x);
+    else if (a.top <= 4) hipLaunchKernelGGL((lp_walk_kernel<T, 4>), grid, dim3(64), 0, s, a, x);
+    else hipLaunchKernelGGL((lp_walk_kernel<T, 8>), grid, dim3(64), 0, s, a, x);
+  } else if (path == PATH_ANY) {
+    hipLaunchKernelGGL((lp_any_kernel<T>), dim3(uh_grid(rows, UH_GRID_WAVES)), dim3(256), 0, s, a, x);
+  } else if (const auto [parts, len] = lp_cut(a.v, rows, dtype); parts > 1) {
+    RowStat* ps = (RowStat*)ws;
+    uint64_t* pt = (uint64_t*)((char*)ws + (size_t)rows * parts * 16);
+    const dim3 grid((unsigned)rows, (unsigned)parts);
+#define UH_GO(NV)                                                                                            \
+  do {                                                                                                       \
+    if (a.top) hipLaunchKernelGGL((lp_part_kernel<T, NV, true>), grid, dim3(256), 0, s, a, x, parts, len, ps, pt); \
+    else hipLaunchKernelGGL((lp_part_kernel<T, NV, false>), grid, dim3(256), 0, s, a, x, parts, len, ps, pt);      \
+  } while (0)
+    if (len <= 256 * E) UH_GO(1); else if (len <= 256 * 4 * E) UH_GO(4); else if (len <= 256 * 8 * E) UH_GO(8); else UH_GO(16);
+#undef UH_GO
+    hipLaunchKernelGGL((lp_join_kernel<T>), dim3((unsigned)rows), dim3(64), (size_t)parts * a.top * 8, s, a, x, parts, ps, pt);
+  } else {
+    const dim3 blocks(uh_grid(rows, UH_GRID_WAVES)), quads(uh_grid((rows + 3) / 4, UH_GRID_WAVES));
+#define UH_GO(G, NV)                                                                                            \
+  do {                                                                                                          \
+    if (a.top) hipLaunchKernelGGL((lp_group_kernel<T, G, NV, 0, true>), blocks, dim3(G), 0, s, a, x);           \
+    else hipLaunchKernelGGL((lp_group_kernel<T, G, NV, 0, false>), blocks, dim3(G), 0, s, a, x);                \
+  } while (0)
+    if (C <= 16 * 4 * E && a.top <= 8) {
+      if (a.top == 0) hipLaunchKernelGGL((lp_group_kernel<T, 16, 4, 0, false>), quads, dim3(64), 0, s, a, x);
+      else if (a.top <= 4) hipLaunchKernelGGL((lp_group_kernel<T, 16, 4, 4, false>), quads, dim3(64), 0, s, a, x);
+      else hipLaunchKernelGGL((lp_group_kernel<T, 16, 4, 8, false>), quads, dim3(64), 0, s, a, x);
+    } else if (C <= 64 * 4 * E) UH_GO(64, 4);
+    else if (C <= 64 * 8 * E) UH_GO(64, 8);
+    else if (C <= 256 * 4 * E) UH_GO(256, 4);
+    else if (C <= 256 * 8 * E) UH_GO(256, 8);
+    else UH_GO(256, 16);
+#undef UH_GO
+  }
 }
 
 extern "C" int uh_label_log_probs(const uh_class_view* view, const void* logits, const void* labels, int label_bytes,
@@ -114,20 +520,42 @@ extern "C" int uh_label_log_probs(const uh_class_view* view, const void* logits,
   UH_REQUIRE(top == 0 || (top_log_prob && top_index), "label_log_probs: null pointer");
   UH_REQUIRE(temperature > 0.f && temperature < INFINITY, "label_log_probs: temperature %g", temperature);
   const size_t need = uh_label_log_probs_workspace(view, top);
-  UH_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "label_log_probs: workspace of %zu bytes, %zu needed",
-             workspace_bytes, need);
-  const RowView v = uh_row_view(view);
-  const long long rows = v.outer * v.inner;
-  const float c2 = (float)(1.4426950408889634 / (double)temperature);
-#define UH_GO(T)                                                                                                        \
-  hipLaunchKernelGGL(label_probs_any_kernel<T>, dim3(row_grid(rows)), dim3(256), 0, (hipStream_t)s, v, rows,            \
-                     (const T*)logits, labels, label_bytes, ignore_index, top, temperature, c2, log_prob, entropy,      \
-                     top_log_prob, top_index, stats)
-  if (view->dtype == UH_F32) UH_GO(float);
-  else if (view->dtype == UH_BF16) UH_GO(bf16);
-  else UH_GO(f16);
-#undef UH_GO
+  UH_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+             "label_log_probs: workspace of %zu bytes, %zu needed on 16 bytes", workspace_bytes, need);
+  LpArgs a;
+  a.v = uh_row_view(view);
+  a.rows = view->outer * view->inner;
+  a.labels = labels, a.label_bytes = label_bytes, a.ignore = ignore_index;
+  a.top = top, a.temperature = temperature, a.c2 = (float)(1.4426950408889634 / (double)temperature);
+  a.log_prob = log_prob, a.entropy = entropy, a.top_lp = top_log_prob, a.top_idx = top_index, a.stats = stats;
+  if (view->dtype == UH_F32) lp_launch<float>(a, (const float*)logits, view->dtype, workspace, (hipStream_t)s);
+  else if (view->dtype == UH_BF16) lp_launch<bf16>(a, (const bf16*)logits, view->dtype, workspace, (hipStream_t)s);
+  else lp_launch<f16>(a, (const f16*)logits, view->dtype, workspace, (hipStream_t)s);
   return uh_check_launch("label_log_probs");
+}
+
+template <typename T> static void lp_bwd_launch(const LpBwd& k, const T* x, T* dx, hipStream_t s) {
+  constexpr int E = 16 / sizeof(T);
+  const int C = k.v.C;
+  const long long rows = k.rows;
+  const ClassPath path = uh_class_path(k.v, &k.vo, rows);
+  if (path == PATH_STAGED) {
+    const bool wide = (k.v.so * sizeof(T)) % 16 == 0 && (C * sizeof(T)) % 16 == 0;
+    const size_t lds = ((64 * k.v.so + E - 1) / E * E + 64 * C) * sizeof(T);
+    hipLaunchKernelGGL((lp_bwd_thread_kernel<T>), dim3(uh_grid((rows + 63) / 64, UH_GRID_WAVES)), dim3(64), lds, s, k, x, dx, wide);
+  } else if (path == PATH_APART || path == PATH_WALK) {
+    hipLaunchKernelGGL((lp_bwd_walk_kernel<T>), dim3((unsigned)((rows + 63) / 64)), dim3(64), 0, s, k, x, dx);
+  } else if (path == PATH_ANY) {
+    hipLaunchKernelGGL((lp_bwd_any_kernel<T>), dim3(uh_grid(rows, UH_GRID_WAVES)), dim3(256), 0, s, k, x, dx);
+  } else if (C <= 16 * 4 * E) {
+    hipLaunchKernelGGL((lp_bwd_group_kernel<T, 16, 4>), dim3(uh_grid((rows + 3) / 4, UH_GRID_WAVES)), dim3(64), 0, s, k, x, dx, C);
+  } else if (C <= 64 * 4 * E) {
+    hipLaunchKernelGGL((lp_bwd_group_kernel<T, 64, 4>), dim3(uh_grid(rows, UH_GRID_WAVES)), dim3(64), 0, s, k, x, dx, C);
+  } else {
+    const RowCut cut = uh_cut_parts(C, (C + 256 * 4 * E - 1) / (256 * 4 * E));
+    hipLaunchKernelGGL((lp_bwd_group_kernel<T, 256, 4>), dim3(uh_grid(rows, UH_GRID_WAVES), (unsigned)cut.parts), dim3(256), 0, s, k,
+                       x, dx, cut.len);
+  }
 }
 
 extern "C" int uh_label_log_probs_bwd(const uh_class_view* view, const uh_class_view* out_view, const void* logits,
@@ -144,16 +572,14 @@ extern "C" int uh_label_log_probs_bwd(const uh_class_view* view, const uh_class_
   UH_REQUIRE(!labels || label_bytes == 4 || label_bytes == 8, "label_log_probs_bwd: labels of %d bytes", label_bytes);
   UH_REQUIRE(labels || !g_log_prob, "label_log_probs_bwd: a gradient of log_prob without labels");
   UH_REQUIRE(temperature > 0.f && temperature < INFINITY, "label_log_probs_bwd: temperature %g", temperature);
-  const RowView v = uh_row_view(view), vo = uh_row_view(out_view);
-  const long long rows = v.outer * v.inner;
-  const float c2 = (float)(1.4426950408889634 / (double)temperature), inv_t = 1.f / temperature;
-#define UH_GO(T)                                                                                                        \
-  hipLaunchKernelGGL(label_probs_bwd_any_kernel<T>, dim3(row_grid(rows)), dim3(256), 0, (hipStream_t)s, v, vo, rows,    \
-                     (const T*)logits, labels, label_bytes, ignore_index, inv_t, c2, stats, entropy, g_log_prob,        \
-                     g_entropy, (T*)dlogits)
-  if (view->dtype == UH_F32) UH_GO(float);
-  else if (view->dtype == UH_BF16) UH_GO(bf16);
-  else UH_GO(f16);
-#undef UH_GO
+  LpBwd k;
+  k.v = uh_row_view(view), k.vo = uh_row_view(out_view);
+  k.rows = view->outer * view->inner;
+  k.labels = labels, k.label_bytes = label_bytes, k.ignore = ignore_index;
+  k.inv_t = 1.f / temperature, k.c2 = (float)(1.4426950408889634 / (double)temperature);
+  k.stats = stats, k.entropy = entropy, k.g_lp = g_log_prob, k.g_ent = g_entropy;
+  if (view->dtype == UH_F32) lp_bwd_launch<float>(k, (const float*)logits, (float*)dlogits, (hipStream_t)s);
+  else if (view->dtype == UH_BF16) lp_bwd_launch<bf16>(k, (const bf16*)logits, (bf16*)dlogits, (hipStream_t)s);
+  else lp_bwd_launch<f16>(k, (const f16*)logits, (f16*)dlogits, (hipStream_t)s);
   return uh_check_launch("label_log_probs_bwd");
 }

@@ -4,11 +4,17 @@
 // element o*so + i*si + c*sc: [N][C] rows have inner = 1 and sc = 1, class maps [B][C][H][W] have inner = H*W, si = 1
 // and sc = H*W.  What belongs to a row with k entries (top alternatives, a teacher's slots) lies at [o][k][i].
 //
-// With m = max x, c2 = log2(e) / T:  s = sum 2^((x - m) c2), L2 = log2 s, p = 2^((x - m) c2 - L2).  Statistics are fp32
-// whatever the logits' type; the difference x - m is taken before the product, so that logits of the size of the
-// type's lowest value (masks) neither overflow nor cancel.
-//   row without a finite logit: m = 0, L2 = +inf, hence p = 0 everywhere;
-//   row with a NaN or +inf:     L2 = NaN, hence p = NaN everywhere.
+// Statistics of a row, fp32 whatever the logits' type: m = max x, and with c = log2(e) / T, M = c m rounded to fp32
+//     s = sum 2^(c x - M),   t = sum 2^(c x - M) (c x - M)          one fused multiply-add and one exponential each
+// The rounding of M is no error: it is a common factor of s that ln s = log(s) - (c m - M) ln 2 takes out again.
+//   |m| >= 2^100 (masks of the type's lowest value throughout, or fp32 logits of that size): c = 2^-20 instead, for which
+//     M is exact; neighbouring numbers of that size are 2^57 apart after it, so that p is 1/n for the n largest, as it is
+//     with the true c, and nothing overflows;
+//   a row without a finite logit: m = 0, s = 0, and p = 0 everywhere;  a row with a NaN or +inf: s = NaN.
+//
+// Which kernel takes a row (class_path below): rows whose classes lie side by side are read by a group of lanes, 16 bytes
+// a load, and stay in registers between the maximum, the sums and the gradient; up to 64 classes, or classes that lie apart
+// (maps), a row is one thread's; anything else is one workgroup's, element by element.
 #pragma once
 #include "common.h"
 #include <math.h>
@@ -16,22 +22,30 @@
 typedef _Float16 f16;
 
 struct RowView {
-  long long outer, inner, so, si, sc;
+  long long inner, so, si, sc;    // inner = 1 where one step walks all rows, whatever the tensor's shape
+  long long einner;               // the view's own inner: what has k entries per row is laid out by it
   int C;
   __device__ __forceinline__ long long base(long long r) const {
     if (inner == 1) return r * so;
-    const long long o = r / inner;
-    return o * so + (r - o * inner) * si;
+    const unsigned o = (unsigned)r / (unsigned)inner;             // rows are counted in 31 bits
+    return o * so + ((unsigned)r - o * (unsigned)inner) * si;
   }
   // element of entry k of row r in a dense [outer][K][inner] table
   __device__ __forceinline__ long long entry(long long r, int k, int K) const {
-    if (inner == 1) return r * K + k;
-    const long long o = r / inner;
-    return (o * K + k) * inner + (r - o * inner);
+    if (einner == 1) return r * K + k;
+    const unsigned o = (unsigned)r / (unsigned)einner;
+    return ((long long)o * K + k) * einner + ((unsigned)r - o * (unsigned)einner);
   }
 };
 
-static inline RowView uh_row_view(const uh_class_view* v) { return RowView{v->outer, v->inner, v->so, v->si, v->sc, v->classes}; }
+static inline RowView uh_row_view(const uh_class_view* v) {
+  RowView w{v->inner, v->so, v->si, v->sc, v->inner, v->classes};
+  if (w.inner > 1 && (v->outer == 1 || w.so == w.inner * w.si)) {
+    w.so = w.si;
+    w.inner = 1;
+  }
+  return w;
+}
 
 // what every entry point checks of a view; rows are counted in 31 bits so that a launch can cover them
 static inline int uh_check_view(const uh_class_view* v, const char* who) {
@@ -45,16 +59,22 @@ static inline int uh_check_view(const uh_class_view* v, const char* who) {
   return UH_OK;
 }
 
+// ---- values -------------------------------------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ float ld(const T* p) { return (float)*p; }
-__device__ __forceinline__ void st(float* p, float v) { *p = v; }
-__device__ __forceinline__ void st(bf16* p, float v) { *p = (bf16)v; }
-__device__ __forceinline__ void st(f16* p, float v) { *p = (f16)v; }      // overflow gives inf, which a GradScaler looks for
+template <typename T> __device__ __forceinline__ void st(T* p, float v) { *p = (T)v; }   // fp16: overflow gives inf, which a GradScaler looks for
 
 static constexpr float UH_LN2 = 0.693147180559945309f;
-static constexpr float UH_LOG2E = 1.44269504088896341f;
-static constexpr float UH_ZMIN = -200.f;      // 2^-200 is 0 in fp32: below it a term of the entropy sum is 0
+static constexpr float UH_ZMIN = -200.f;      // 2^-200 is 0 in fp32: below it a term of t is 0
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+struct RowRef {           // the point and the scale a row's exponents are taken in
+  float c, M;
+  __device__ __forceinline__ RowRef(float m, float c2) : c(fabsf(m) >= 0x1p100f ? 0x1p-20f : c2), M(m * c) {}
+  __device__ __forceinline__ float z(float x) const { return fmaf(x, c, -M); }
+  __device__ __forceinline__ float ln_s(float m, float s) const { return logf(s) - fmaf(m, c, -M) * UH_LN2; }
+};
+struct RowStat { float m, s, t; };
 
 // (x - m) / T of a reported value; x - m may overflow where its quotient does not (a class masked with the type's lowest
 // value, T > 1)
@@ -63,8 +83,24 @@ __device__ __forceinline__ float scaled(float x, float m, float temperature) {
   return d == -INFINITY ? x / temperature - m / temperature : d / temperature;
 }
 
-// order[x] as unsigned: larger logits first, -0 = +0; the low half orders equal logits by class, lowest first.
-// 0 stands for "none": masked classes (-inf) are never alternatives.
+// joins the statistics of two parts of a row; a part without a finite logit (s = 0) has no say in m
+__device__ __forceinline__ RowStat join(const RowStat& a, const RowStat& b, float c2) {
+  const float ma = a.s == 0.f ? -INFINITY : a.m, mb = b.s == 0.f ? -INFINITY : b.m;
+  float m = fmaxf(ma, mb);
+  if (m == -INFINITY) m = 0.f;
+  const RowRef ref(m, c2), ra(a.m, c2), rb(b.m, c2);
+  const float da = a.s == 0.f ? 0.f : ra.c == ref.c ? ra.M - ref.M : (a.m - m) * c2;
+  const float db = b.s == 0.f ? 0.f : rb.c == ref.c ? rb.M - ref.M : (b.m - m) * c2;
+  const float ea = ex2(da), eb = ex2(db);
+  RowStat o;
+  o.m = m;
+  o.s = a.s * ea + b.s * eb;
+  o.t = ea * fmaf(a.s, fmaxf(da, UH_ZMIN), a.t) + eb * fmaf(b.s, fmaxf(db, UH_ZMIN), b.t);
+  return o;
+}
+
+// rank keys: larger logits first, -0 = +0, equal logits by class, lowest first.  0 stands for "none": classes masked with
+// -inf are never alternatives.
 __device__ __forceinline__ uint32_t order32(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
@@ -76,63 +112,539 @@ __device__ __forceinline__ uint64_t rank_key(float x, int c) {
 __device__ __forceinline__ int key_class(uint64_t k) { return (int)~(uint32_t)k; }
 __device__ __forceinline__ float key_value(uint64_t k) { return unorder32((uint32_t)(k >> 32)); }
 
+// ---- reductions -----------------------------------------------------------------------------------------------------------
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+// max of three in one instruction; NaNs lose against numbers, as in fmaxf
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
+}
+// over groups of 16 or 64 lanes, result in all of them: rotations inside rows of 16 lanes (0x120 + n), then across rows
 template <int G> __device__ __forceinline__ float group_max(float v) {
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  v = fmaxf(v, dpp<0x128>(v));
+  v = fmaxf(v, dpp<0x124>(v));
+  v = fmaxf(v, dpp<0x122>(v));
+  v = fmaxf(v, dpp<0x121>(v));
+  if (G > 16) {
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    v = fmaxf(v, __shfl_xor(v, 32, 64));
+  }
   return v;
 }
 template <int G> __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  v += dpp<0x128>(v);
+  v += dpp<0x124>(v);
+  v += dpp<0x122>(v);
+  v += dpp<0x121>(v);
+  if (G > 16) {
+    v += __shfl_xor(v, 16, 64);
+    v += __shfl_xor(v, 32, 64);
+  }
   return v;
 }
 template <int G> __device__ __forceinline__ uint64_t group_max(uint64_t v) {
 #pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) {
+  for (int o = (G > 64 ? 64 : G) / 2; o > 0; o >>= 1) {
     const uint64_t w = ((uint64_t)__shfl_xor((uint32_t)(v >> 32), o, 64) << 32) | __shfl_xor((uint32_t)v, o, 64);
     v = v > w ? v : w;
   }
   return v;
 }
-
-// over a workgroup of 256 threads; `buf` has 4 entries and may be reused after the call
-template <typename V> __device__ __forceinline__ V block_max(V v, V* buf) {
-  v = group_max<64>(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = buf[0];
+template <int G> __device__ __forceinline__ uint32_t group_max(uint32_t v) {
 #pragma unroll
-  for (int w = 1; w < 4; ++w) v = v > buf[w] ? v : buf[w];
+  for (int o = G / 2; o > 0; o >>= 1) {
+    const uint32_t w = __shfl_xor(v, o, 64);
+    v = v > w ? v : w;
+  }
   return v;
 }
-__device__ __forceinline__ float block_sum(float v, float* buf) {
-  v = group_sum<64>(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return (buf[0] + buf[1]) + (buf[2] + buf[3]);
-}
+
+// LDS of the reductions over a workgroup of NW waves; nothing for groups inside a wave
+template <int NW> struct RedBuf {
+  float m[NW], s[NW], t[NW];
+  uint64_t k[NW];
+};
+template <> struct RedBuf<0> {};
+
+// over all G lanes of a group (G > 64: the whole workgroup, which must call together)
+template <int G> struct Red {
+  static constexpr int NW = G > 64 ? G / 64 : 0;
+  typedef RedBuf<NW> Buf;
+  __device__ static __forceinline__ float max_(float v, Buf& b) {
+    v = group_max<(G > 64 ? 64 : G)>(v);
+    if constexpr (NW > 0) {
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) b.m[threadIdx.x >> 6] = v;
+      __syncthreads();
+      v = b.m[0];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) v = fmaxf(v, b.m[w]);
+    }
+    return v;
+  }
+  __device__ static __forceinline__ float sum_(float v, Buf& b) {
+    v = group_sum<(G > 64 ? 64 : G)>(v);
+    if constexpr (NW > 0) {
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) b.s[threadIdx.x >> 6] = v;
+      __syncthreads();
+      v = b.s[0];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) v += b.s[w];
+    }
+    return v;
+  }
+  __device__ static __forceinline__ void sum2(float& v, float& u, Buf& b) {
+    v = group_sum<(G > 64 ? 64 : G)>(v);
+    u = group_sum<(G > 64 ? 64 : G)>(u);
+    if constexpr (NW > 0) {
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) { b.s[threadIdx.x >> 6] = v; b.t[threadIdx.x >> 6] = u; }
+      __syncthreads();
+      v = b.s[0], u = b.t[0];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) { v += b.s[w]; u += b.t[w]; }
+    }
+  }
+  __device__ static __forceinline__ uint64_t maxkey(uint64_t v, Buf& b) {
+    v = group_max<(G > 64 ? 64 : G)>(v);
+    if constexpr (NW > 0) {
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) b.k[threadIdx.x >> 6] = v;
+      __syncthreads();
+      v = b.k[0];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) v = v > b.k[w] ? v : b.k[w];
+    }
+    return v;
+  }
+};
 
 __device__ __forceinline__ long long load_int(const void* p, int bytes, long long i) {
   return bytes == 8 ? ((const long long*)p)[i] : (long long)((const int*)p)[i];
 }
 
-// statistics of one row by a workgroup of 256 threads: m, s and t = sum e z2 (for the entropy)
-struct RowStat { float m, s, t; };
-template <typename T> __device__ RowStat block_row_stat(const T* __restrict__ x, int C, long long sc, float c2, float* buf) {
+// ---- a row in the registers of a group of lanes ------------------------------------------------------------------------------
+// 16 bytes wherever an element may lie: rows of odd sizes start anywhere (the hardware takes element-aligned vectors)
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Loose16 { uint32_t w[4]; };
+
+template <typename T, int G, int NV> struct RowRegs {
+  static constexpr int E = 16 / sizeof(T);
+  static constexpr int CAP = G * NV * E;
+  uint32_t w[NV][4];
+
+  __device__ __forceinline__ static uint32_t neg_inf() {
+    return sizeof(T) == 4 ? 0xff800000u : std_is_half() ? 0xfc00fc00u : 0xff80ff80u;
+  }
+  __device__ __forceinline__ static constexpr bool std_is_half() { return __is_same(T, f16); }
+
+  // vector v = r*G + lane holds elements first(v) .. first(v) + E - 1; the last one of a row that is no multiple of E is
+  // read so that it ends with the row, with -inf in the places that its left neighbour holds too.  n >= E.
+  __device__ __forceinline__ static int first(int r, int lane, int n) {
+    const int e = (r * G + lane) * E;
+    return e + E <= n ? e : n - E;
+  }
+  __device__ __forceinline__ void load(const T* __restrict__ p, int n, int lane) {
+#pragma unroll
+    for (int r = 0; r < NV; ++r)
+      if (r * G * E < n) {
+        const int e = (r * G + lane) * E;
+        if (e < n) {
+          const Loose16<T> u = *reinterpret_cast<const Loose16<T>*>(p + first(r, lane, n));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[r][i] = u.w[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[r][i] = neg_inf();
+        }
+      }
+    // the ragged vector
+    if (n % E) {
+      const int dup = E - n % E;                                   // places that the left neighbour holds
+#pragma unroll
+      for (int r = 0; r < NV; ++r)
+        if (r * G * E < n && (r + 1) * G * E > n - E) {
+          const int e = (r * G + lane) * E;
+          if (e < n && e + E > n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if constexpr (sizeof(T) == 4) {
+                if (i < dup) w[r][i] = neg_inf();
+              } else {
+                if (2 * i < dup) w[r][i] = (w[r][i] & 0xffff0000u) | (neg_inf() & 0xffffu);
+                if (2 * i + 1 < dup) w[r][i] = (w[r][i] & 0xffffu) | (neg_inf() & 0xffff0000u);
+              }
+            }
+          }
+        }
+    }
+  }
+  // Between two sweeps: without it the compiler unpacks 16-bit logits once and keeps them in twice the registers (256 and
+  // spills where 64 hold the row).
+  __device__ __forceinline__ void fresh() {
+#pragma unroll
+    for (int r = 0; r < NV; ++r) asm volatile("" : "+v"(w[r][0]), "+v"(w[r][1]), "+v"(w[r][2]), "+v"(w[r][3]));
+  }
+  __device__ __forceinline__ float get(int r, int j) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[r][j]);
+    else if constexpr (std_is_half()) {
+      typedef __attribute__((ext_vector_type(2))) _Float16 h2;
+      const h2 v = __builtin_bit_cast(h2, w[r][j >> 1]);
+      return (float)v[j & 1];
+    } else
+      return __uint_as_float(j & 1 ? w[r][j >> 1] & 0xffff0000u : w[r][j >> 1] << 16);
+  }
+  __device__ __forceinline__ float lane_max(int n) const {
+    float m = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < NV; ++r)
+      if (r * G * E < n) {
+#pragma unroll
+        for (int j = 0; j < E; j += 2) m = max3(m, get(r, j), get(r, j + 1));
+        __builtin_amdgcn_sched_barrier(0);                  // one vector at a time: unpacked ones would pile up
+      }
+    return m;
+  }
+  // s and (ENT) t of a lane's elements
+  template <bool ENT> __device__ __forceinline__ void lane_sums(const RowRef& ref, int n, float& s, float& t) const {
+    float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f;
+#pragma unroll
+    for (int r = 0; r < NV; ++r)
+      if (r * G * E < n) {
+#pragma unroll
+        for (int j = 0; j < E; j += 2) {
+          const float z0 = ref.z(get(r, j)), z1 = ref.z(get(r, j + 1));
+          const float e0 = ex2(z0), e1 = ex2(z1);
+          s0 += e0, s1 += e1;
+          if (ENT) t0 = fmaf(e0, fmaxf(z0, UH_ZMIN), t0), t1 = fmaf(e1, fmaxf(z1, UH_ZMIN), t1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    s = s0 + s1, t = t0 + t1;
+  }
+  // f(x) of every element to out[0 .. n)
+  template <typename F> __device__ __forceinline__ void map_store(T* __restrict__ out, int n, int lane, F f) const {
+#pragma unroll
+    for (int r = 0; r < NV; ++r)
+      if (r * G * E < n) {
+        const int e = (r * G + lane) * E;
+        if (e + E <= n) {
+          Loose16<T> u;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) u.w[i] = __float_as_uint(f(get(r, i)));
+            else {
+              typedef __attribute__((ext_vector_type(2))) T T2;
+              const T2 v = {(T)f(get(r, 2 * i)), (T)f(get(r, 2 * i + 1))};
+              u.w[i] = __builtin_bit_cast(uint32_t, v);
+            }
+          }
+          *reinterpret_cast<Loose16<T>*>(out + e) = u;
+        } else if (e < n) {
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (n - E + j >= e) out[n - E + j] = (T)f(get(r, j));
+        }
+      }
+  }
+};
+
+// statistics of one row by G lanes of a workgroup (any strides, element by element)
+template <typename T, int G> __device__ RowStat strided_row_stat(const T* __restrict__ x, int C, long long sc, float c2, int lane,
+                                                                 typename Red<G>::Buf& buf) {
   float m = -INFINITY;
-  for (int c = threadIdx.x; c < C; c += 256) m = fmaxf(m, ld(x + c * sc));
-  m = block_max(m, buf);
+  for (int c = lane; c < C; c += G) m = fmaxf(m, ld(x + c * sc));
+  m = Red<G>::max_(m, buf);
   if (m == -INFINITY) m = 0.f;
+  const RowRef ref(m, c2);
   float s = 0.f, t = 0.f;
-  for (int c = threadIdx.x; c < C; c += 256) {
-    const float z = (ld(x + c * sc) - m) * c2, e = ex2(z);
+  for (int c = lane; c < C; c += G) {
+    const float z = ref.z(ld(x + c * sc)), e = ex2(z);
     s += e;
     t = fmaf(e, fmaxf(z, UH_ZMIN), t);
   }
-  s = block_sum(s, buf);
-  t = block_sum(t, buf);
+  Red<G>::sum2(s, t, buf);
   return RowStat{m, s, t};
 }
-__device__ __forceinline__ float stat_l2(float s) { return s == 0.f ? INFINITY : log2f(s); }
+
+// ---- the largest of a row ---------------------------------------------------------------------------------------------------
+// Keys of rows of up to 64 classes held by a lane: 16-bit logits and their class fit 32 bits.
+template <typename T> struct SmallKey {
+  typedef uint32_t K;
+  __device__ __forceinline__ static K make(float x, int c) {
+    uint32_t b;
+    if constexpr (__is_same(T, f16)) b = __builtin_bit_cast(uint16_t, (f16)(x + 0.f));
+    else b = __float_as_uint(x + 0.f) >> 16;
+    b = b & 0x8000u ? b ^ 0xffffu : b | 0x8000u;
+    return x > -INFINITY ? (b << 16) | (0xffffu - (uint32_t)c) : 0u;
+  }
+  __device__ __forceinline__ static int cls(K k) { return 0xffff - (int)(k & 0xffffu); }
+  __device__ __forceinline__ static float val(K k) {
+    uint32_t b = k >> 16;
+    b = b & 0x8000u ? b & 0x7fffu : b ^ 0xffffu;
+    if constexpr (__is_same(T, f16)) return (float)__builtin_bit_cast(f16, (uint16_t)b);
+    else return __uint_as_float(b << 16);
+  }
+};
+template <> struct SmallKey<float> {
+  typedef uint64_t K;
+  __device__ __forceinline__ static K make(float x, int c) { return rank_key(x, c); }
+  __device__ __forceinline__ static int cls(K k) { return key_class(k); }
+  __device__ __forceinline__ static float val(K k) { return key_value(k); }
+};
+// keeps the N largest keys of a lane, falling
+template <typename K, int N> __device__ __forceinline__ void list_insert(K (&l)[N], K k) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const K hi = l[i] > k ? l[i] : k;
+    k = l[i] > k ? k : l[i];
+    l[i] = hi;
+  }
+}
+
+__device__ __forceinline__ int ballot_count(bool p) { return __popcll(__ballot(p)); }
+
+// a lower bound of the k-th largest of a wave's NK keys a lane, with at least k keys at or above it; 0 if there are fewer
+template <int NK> __device__ __forceinline__ uint32_t wave_kth(const uint32_t (&key)[NK], int k) {
+  uint32_t low = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t test = low | (1u << bit);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < NK; ++i) n += ballot_count(key[i] >= test);
+    if (n >= k) {
+      low = test;
+      if (n == k) break;
+    }
+  }
+  return low;
+}
+
+// one wave: emit(rank, key) of the k largest of n different keys in LDS, emit(rank, 0) for the places left over.  More than
+// 128 keys are first cut down to the k by a search over the bits of the k-th largest.
+template <typename F> __device__ __forceinline__ void wave_select(uint64_t* list, int n, int k, F emit) {
+  const int lane = threadIdx.x & 63;
+  if (n > 128 && n > k) {
+    uint64_t low = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const uint64_t test = low | (1ull << bit);
+      int c = 0;
+      for (int i = 0; i < n; i += 64) c += ballot_count(i + lane < n && list[i + lane] >= test);
+      if (c >= k) {
+        low = test;
+        if (c == k) break;
+      }
+    }
+    // the k keys move to the front: a step reads its 64 places before it writes, and writes no further than it has read
+    int at = 0;
+    for (int i = 0; i < n; i += 64) {
+      const uint64_t mine = i + lane < n ? list[i + lane] : 0;
+      const bool in = mine >= low && mine != 0;
+      const uint64_t who = __ballot(in);
+      __builtin_amdgcn_wave_barrier();
+      if (in) list[at + __popcll(who & ((1ull << lane) - 1))] = mine;
+      __builtin_amdgcn_wave_barrier();
+      at += __popcll(who);
+    }
+    n = at;
+  }
+  for (int i = lane; i < n; i += 64) {
+    const uint64_t mine = list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += list[j] > mine;
+    if (rank < k) emit(rank, mine);
+  }
+  for (int i = n + lane; i < k; i += 64) emit(i, 0ull);
+}
+
+// The k largest of a row in registers.  The k-th largest of the lanes' own maxima bounds the k-th largest element from
+// below (each of k lanes holds one at least as large): the few elements at or above it go to a list in LDS, which one wave
+// ranks.  Rows whose many equal values overflow the list take the largest k times over instead.  All G lanes call; the
+// list may be used again after the next barrier of the workgroup.
+template <int G> struct TopBuf {
+  static constexpr int CAP = G > 64 ? 2048 : 512;
+  uint64_t list[CAP];
+  float lane_max[G > 64 ? G : 1];
+  uint32_t low;
+  int count;
+};
+template <typename T, int G, int NV, typename F>
+__device__ __forceinline__ void group_top(RowRegs<T, G, NV>& x, const T* __restrict__ row, int n, int lane, int c0, int k, float lane_max, TopBuf<G>& b,
+                                          typename Red<G>::Buf& red, F emit) {
+  constexpr int E = RowRegs<T, G, NV>::E;
+  const uint32_t mine = lane_max > -INFINITY ? order32(lane_max) : 0u;
+  __syncthreads();
+  if (lane == 0) b.count = 0;
+  uint32_t low;
+  if constexpr (G == 64) {
+    const uint32_t key[1] = {mine};
+    low = wave_kth<1>(key, k);
+  } else {
+    b.lane_max[lane] = lane_max;
+    __syncthreads();
+    if (lane < 64) {
+      uint32_t key[G / 64];
+#pragma unroll
+      for (int i = 0; i < G / 64; ++i) {
+        const float v = b.lane_max[lane + 64 * i];
+        key[i] = v > -INFINITY ? order32(v) : 0u;
+      }
+      const uint32_t l = wave_kth<G / 64>(key, k);
+      if (lane == 0) b.low = l;
+    }
+    __syncthreads();
+    low = b.low;
+  }
+  __syncthreads();
+  // lanes that hold one look for it again; its few hits are read once more from memory (a register cannot be indexed)
+  const float cut = low ? unorder32(low) : -3.402823466e38f;
+  x.fresh();
+  if (mine != 0 && mine >= low) {
+#pragma unroll
+    for (int r = 0; r < NV; ++r)
+      if (r * G * E < n) {
+        uint32_t hits = 0;
+#pragma unroll
+        for (int j = 0; j < E; ++j) hits |= x.get(r, j) >= cut ? 1u << j : 0u;
+        const int e = RowRegs<T, G, NV>::first(r, lane, n);
+        while (hits) {
+          const int c = e + __ffs(hits) - 1;
+          hits &= hits - 1;
+          const int at = atomicAdd(&b.count, 1);
+          if (at < TopBuf<G>::CAP) b.list[at] = rank_key(ld(row + c), c0 + c);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  }
+  __syncthreads();
+  const int found = b.count;
+  if (found <= TopBuf<G>::CAP) {
+    if (lane < 64) wave_select(b.list, found, k, emit);
+    return;
+  }
+  uint64_t last = ~0ull;
+  for (int i = 0; i < k; ++i) {
+    uint64_t best = 0;
+    for (int c = lane; c < n; c += G) {
+      const uint64_t key = rank_key(ld(row + c), c0 + c);
+      if (key < last && key > best) best = key;
+    }
+    best = Red<G>::maxkey(best, red);
+    if (lane == 0) emit(i, best);
+    last = best;
+  }
+}
+
+// ---- one thread per row: up to 64 classes ---------------------------------------------------------------------------------------
+// A workgroup is one wave and takes 64 rows.  Rows side by side in memory (STAGED) come through LDS, so that the wave's loads
+// are whole lines; classes that lie apart (maps) are loaded by the row's thread itself: neighbouring threads, neighbouring rows.
+template <typename T> __device__ __forceinline__ void copy_to_lds(T* __restrict__ dst, const T* __restrict__ src, int n) {
+  constexpr int E = 16 / sizeof(T);
+  const int lane = threadIdx.x;
+  int i = lane * E;
+  for (; i + E <= n; i += 64 * E)
+    *reinterpret_cast<U4*>(dst + i) = __builtin_bit_cast(U4, *reinterpret_cast<const Loose16<T>*>(src + i));
+  for (int e = n / E * E + lane; e < n; e += 64) dst[e] = src[e];
+}
+template <typename T> __device__ __forceinline__ void copy_from_lds(T* __restrict__ dst, const T* __restrict__ src, int n) {
+  constexpr int E = 16 / sizeof(T);
+  const int lane = threadIdx.x;
+  for (int i = lane * E; i + E <= n; i += 64 * E)
+    *reinterpret_cast<Loose16<T>*>(dst + i) = __builtin_bit_cast(Loose16<T>, *reinterpret_cast<const U4*>(src + i));
+  for (int e = n / E * E + lane; e < n; e += 64) dst[e] = src[e];
+}
+// a row of C <= CREG classes to registers, -inf behind its end
+template <typename T, int CREG, bool STAGED>
+__device__ __forceinline__ void load_classes(float (&x)[CREG], const T* __restrict__ p, long long sc, int C, bool wide) {
+  constexpr int E = 16 / sizeof(T);
+  if (STAGED && wide) {                                    // rows start on 16 bytes and are at least that far apart
+#pragma unroll
+    for (int c = 0; c < CREG; c += E)
+      if (c < C) {
+        T v[E];
+        *reinterpret_cast<U4*>(v) = *reinterpret_cast<const U4*>(p + c);
+#pragma unroll
+        for (int j = 0; j < E; ++j) x[c + j] = c + j < C ? (float)v[j] : -INFINITY;
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j) x[c + j] = -INFINITY;
+      }
+    return;
+  }
+#pragma unroll
+  for (int c = 0; c < CREG; ++c) x[c] = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < CREG; ++c)
+    if (c < C) x[c] = STAGED ? (float)p[c] : (float)p[c * sc];
+}
+template <int CREG, bool ENT> __device__ __forceinline__ RowStat thread_row_stat(const float (&x)[CREG], int C, float c2) {
+  float m = x[0];
+#pragma unroll
+  for (int c = 1; c < CREG; c += 2)
+    if (c < C) m = max3(m, x[c], c + 1 < CREG ? x[c + 1] : x[c]);
+  if (m == -INFINITY) m = 0.f;
+  const RowRef ref(m, c2);
+  float s = 0.f, t = 0.f;
+#pragma unroll
+  for (int c = 0; c < CREG; ++c)
+    if (c < C) {
+      const float z = ref.z(x[c]), e = ex2(z);
+      s += e;
+      if (ENT) t = fmaf(e, fmaxf(z, UH_ZMIN), t);
+    }
+  return RowStat{m, s, t};
+}
+// the same of a row of any length that one thread walks, eight classes at a time
+template <typename T> __device__ __forceinline__ RowStat walk_row_stat(const T* __restrict__ p, long long sc, int C, float c2) {
+  RowStat a{0.f, 0.f, 0.f};
+  for (int c0 = 0; c0 < C; c0 += 8) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = c0 + j < C ? ld(p + (c0 + j) * sc) : -INFINITY;
+    a = join(a, thread_row_stat<8, true>(x, 8, c2), c2);
+  }
+  return a;
+}
+
+// ---- which kernel takes a call ---------------------------------------------------------------------------------------------
+static inline int uh_elem_bytes(int dtype) { return dtype == UH_F32 ? 4 : 2; }
+static inline unsigned uh_grid(long long blocks, long long most) { return (unsigned)(blocks < most ? blocks : most); }
+enum { UH_GRID_WAVES = 256 * 32 };               // workgroups that loop over rows: 32 a CU
+
+// Rows of at most 64 classes are a thread's: a group of 16 lanes, four loads each, would leave most lanes empty (12 classes of
+// 16 bits: 2 of 16 at work).  STAGED needs one step from row to row, no more than 64 classes and a half further (LDS, and bytes
+// read between the rows), and a dense gradient.
+enum ClassPath { PATH_GROUP, PATH_STAGED, PATH_APART, PATH_WALK, PATH_ANY };
+static inline ClassPath uh_class_path(const RowView& v, const RowView* vo, long long rows) {
+  if (v.C <= 64) {
+    const bool staged = v.sc == 1 && v.inner == 1 && v.so >= v.C && v.so <= 96 &&
+                        (!vo || (vo->sc == 1 && vo->inner == 1 && vo->so == v.C));
+    return staged ? PATH_STAGED : PATH_APART;
+  }
+  if (v.sc == 1 && (!vo || vo->sc == 1)) return PATH_GROUP;
+  return rows >= 256 ? PATH_WALK : PATH_ANY;
+}
+
+// A row is cut when it is longer than the 64 KB a workgroup of 256 holds in registers, or when there are too few rows to give
+// every CU two workgroups; a part is then at least 2048 classes (8 a lane).  At most 64 parts: a wave joins them, one a lane.
+// Parts are multiples of 64 classes, the last one what is left (at least one class; its loads may reach back into the part
+// before it).
+struct RowCut { int parts, len; };
+static inline RowCut uh_cut_parts(int C, long long parts) {
+  const int len = (int)(((C + parts - 1) / parts + 63) / 64 * 64);
+  return RowCut{(C + len - 1) / len, len};
+}
+static inline RowCut uh_row_cut(long long rows, int C, int dtype) {
+  const int most = 65536 / uh_elem_bytes(dtype);
+  long long parts = (C + most - 1) / most;
+  if (rows * parts < 512) {
+    long long want = (512 + rows - 1) / rows;
+    if (want > C / 2048) want = C / 2048;
+    if (want > 64) want = 64;
+    if (want > parts) parts = want;
+  }
+  return uh_cut_parts(C, parts);
+}

@@ -5,110 +5,473 @@
 //     dx_j = g scale w_row T (p_j - sum_{k: i_k = j} t_k)
 // A slot with a negative index is free (t_k = 0).  Rows with w = 0 or without a filled slot count as 0 and get no
 // gradient, whatever they hold.  A class index past C or a NaN among a row's slots makes that row's loss and gradient NaN.
+//
+// Sums over rows: every workgroup adds the rows it takes in 64 bits, one kernel adds the workgroups' sums, all in an order
+// that the sizes alone decide.
 #include "class_rows.h"
 
-// teacher's slot k of a row: its value (-inf for a free slot) and class
-__device__ __forceinline__ float slot_value(const void* v, int dtype, long long i) {
-  return dtype == UH_F32 ? ((const float*)v)[i] : dtype == UH_BF16 ? (float)((const bf16*)v)[i] : (float)((const f16*)v)[i];
-}
+struct DsArgs {
+  RowView v, vo;
+  long long rows;
+  const void *value, *index;
+  int K, value_dtype, index_bytes;
+  const float* weight;
+  float temperature, c2;
+  float grad_scale;               // scale * grad_scale, or scale where gout is given
+  const float* gout;
+  float* stats;                   // [rows][2]: m, s
+  double* partial;
 
-struct Slots {
-  const void* value;
-  const void* index;
-  int K, dtype, index_bytes;
+  __device__ __forceinline__ float weight_of(long long r) const { return weight ? weight[r] : 1.f; }
+  __device__ __forceinline__ float value_of(long long e) const {
+    return value_dtype == UH_F32    ? ((const float*)value)[e]
+           : value_dtype == UH_BF16 ? (float)((const bf16*)value)[e]
+                                    : (float)((const f16*)value)[e];
+  }
+  // slot k of a row: its class (-1: free, C: past the last one) and value (-inf where free, but a NaN stays one)
+  __device__ __forceinline__ void slot(long long r, int k, float& val, int& cls) const {
+    const long long e = v.entry(r, k, K);
+    val = value_of(e);
+    const long long i = load_int(index, index_bytes, e);
+    cls = i < 0 ? -1 : i >= v.C ? v.C : (int)i;
+    if (cls < 0 && val == val) val = -INFINITY;
+  }
+  __device__ __forceinline__ float coef(float w) const { return (gout ? gout[0] * grad_scale : grad_scale) * w * temperature; }
 };
 
-// ---- one workgroup per row, any strides -------------------------------------------------------------------------------
-// mode 0: loss only, 1: gradient only (statistics given), 2: both
-template <typename T, int MODE>
-__global__ __launch_bounds__(256) void distill_any_kernel(RowView v, RowView vo, long long rows, const T* __restrict__ x, Slots sl,
-                                                          const float* __restrict__ weight, float temperature, float c2,
-                                                          float grad_scale, const float* __restrict__ gout,
-                                                          float* __restrict__ stats, float* __restrict__ row_loss,
-                                                          T* __restrict__ dx) {
-  __shared__ float fbuf[4];
-  __shared__ float t_of[UH_SLOTS_MAX];
-  __shared__ int i_of[UH_SLOTS_MAX];
-  const int tid = threadIdx.x;
-  for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
-    const float w = weight ? weight[r] : 1.f;
-    const T* row = x + v.base(r);
-    __syncthreads();                                   // the slots of the row before are read no more
-    // the teacher's softmax: one slot per thread (K <= 256)
+// ln t_k - ln p of a slot, weighted by t_k: e is 2^(..) of the slot against the teacher's maximum vm, sv their sum
+__device__ __forceinline__ float slot_term(float t, float val, float vm, float ln_sv, float x, float m, float ln_s, float temperature) {
+  return t > 0.f ? t * ((scaled(val, vm, temperature) - ln_sv) - (scaled(x, m, temperature) - ln_s)) : t == t ? 0.f : NAN;
+}
+
+// ---- a row by G lanes: the slots in LDS ----------------------------------------------------------------------------------------
+// The teacher's softmax of a row's slots into t_of / c_of [K].  Returns the sum of t (1, 0 without a filled slot, NaN).
+struct Teacher { float vm, ln_sv, sum; };
+template <int G> __device__ __forceinline__ Teacher group_teacher(const DsArgs& a, long long r, int lane, bool off, float* t_of, int* c_of,
+                                                                  typename Red<G>::Buf& red) {
+  float vm = -INFINITY, bad = 0.f;
+  for (int k = lane; k < a.K; k += G) {
     float val = -INFINITY;
-    int idx = -1;
-    if (tid < sl.K && w != 0.f) {
-      const long long e = v.entry(r, tid, sl.K);
-      val = slot_value(sl.value, sl.dtype, e);
-      const long long i = load_int(sl.index, sl.index_bytes, e);
-      idx = i < 0 ? -1 : i >= v.C ? v.C : (int)i;
-      if (idx < 0 && val == val) val = -INFINITY;
+    int cls = -1;
+    if (!off) a.slot(r, k, val, cls);
+    t_of[k] = val, c_of[k] = cls;
+    vm = fmaxf(vm, val);
+    if (val != val || cls >= a.v.C) bad = 1.f;
+  }
+  vm = Red<G>::max_(vm, red);
+  const float m = vm == -INFINITY ? 0.f : vm;
+  const RowRef ref(m, a.c2);
+  float sv = 0.f;
+  for (int k = lane; k < a.K; k += G) sv += ex2(ref.z(t_of[k]));
+  Red<G>::sum2(sv, bad, red);
+  const float inv = bad != 0.f ? NAN : sv == 0.f ? 0.f : 1.f / sv;
+  for (int k = lane; k < a.K; k += G) {
+    const float val = t_of[k];
+    t_of[k] = ex2(ref.z(val)) * inv;
+  }
+  return Teacher{m, ref.ln_s(m, sv), bad != 0.f || !(sv >= 0.f) ? NAN : sv == 0.f ? 0.f : 1.f};
+}
+// sum_k t_k (ln t_k - ln p[i_k]); the lanes read the slots' values again (t has taken their place)
+template <typename T, int G> __device__ __forceinline__ float group_kl(const DsArgs& a, long long r, const T* __restrict__ row, int lane,
+                                                                       const Teacher& q, const RowStat& s, const float* t_of, const int* c_of,
+                                                                       typename Red<G>::Buf& red) {
+  const float ln_s = s.s == 0.f ? 0.f : RowRef(s.m, a.c2).ln_s(s.m, s.s);      // no class left: ln p = -inf
+  float part = 0.f;
+  if (!(q.sum == q.sum)) part = NAN;
+  else if (q.sum != 0.f)
+    for (int k = lane; k < a.K; k += G) {
+      const float t = t_of[k];
+      if (t != 0.f) part += slot_term(t, a.value_of(a.v.entry(r, k, a.K)), q.vm, q.ln_sv, ld(row + c_of[k] * a.v.sc), s.m, ln_s, a.temperature);
     }
-    const float vm = block_max(val, fbuf);
-    const float bad = block_sum((val != val || idx >= v.C) ? 1.f : 0.f, fbuf);
-    const bool empty = vm == -INFINITY && bad == 0.f;
-    const float ev = val == -INFINITY ? 0.f : ex2((val - vm) * c2);
-    const float sv = block_sum(ev, fbuf);
-    const float t = bad != 0.f ? NAN : empty ? 0.f : ev / sv;
-    if (tid < sl.K) { t_of[tid] = t; i_of[tid] = idx; }
-    __syncthreads();
-    float m, l2;
-    if (empty) {
-      m = 0.f, l2 = INFINITY;
-    } else if (MODE == 1) {
-      m = stats[2 * r], l2 = stats[2 * r + 1];
+  return Red<G>::sum_(part, red);
+}
+// classes the teacher names, written again after the dense part: p minus what all slots of that class hold
+template <typename T, int G> __device__ __forceinline__ void group_fix(const DsArgs& a, const T* __restrict__ row, T* __restrict__ out, int lane,
+                                                                       int c0, int n, float sum_t, float coef, const RowRef& ref, float inv_s,
+                                                                       const float* t_of, const int* c_of) {
+  for (int k = lane; k < a.K; k += G) {
+    const int c = c_of[k] - c0;
+    if (c < 0 || c >= n || c_of[k] >= a.v.C) continue;
+    float mine = 0.f;
+    for (int j = 0; j < a.K; ++j) mine += c_of[j] == c_of[k] ? t_of[j] : 0.f;
+    st(out + c * a.vo.sc, coef * (sum_t * (ex2(ref.z(ld(row + c * a.v.sc))) * inv_s) - mine));
+  }
+}
+
+// loss (LOSS) and gradient (GRAD) of rows whose classes lie side by side, the row in registers
+template <typename T, int G, int NV, bool GRAD>
+__global__ __launch_bounds__(G > 64 ? G : 64) void ds_group_kernel(DsArgs a, const T* __restrict__ x, T* __restrict__ dx) {
+  constexpr int RPB = G > 64 ? 1 : 64 / G;
+  extern __shared__ __align__(16) char lds[];
+  __shared__ typename Red<G>::Buf red;
+  const int lane = threadIdx.x % G, sub = threadIdx.x / G, C = a.v.C;
+  float* t_of = reinterpret_cast<float*>(lds) + sub * a.K;
+  int* c_of = reinterpret_cast<int*>(lds) + (RPB + sub) * a.K;
+  const long long blocks = (a.rows + RPB - 1) / RPB;
+  double total = 0.0;
+  for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const long long r = b * RPB + sub;
+    const bool there = r < a.rows;
+    const float w = there ? a.weight_of(r) : 0.f;
+    const bool off = w == 0.f;
+    const T* row = x + (there ? a.v.base(r) : 0);
+    RowRegs<T, G, NV> reg;
+    if (off && RPB == 1) {
+      if (GRAD) reg.map_store(dx + a.vo.base(r), C, lane, [](float) { return 0.f; });
+      if (a.stats && lane == 0) { a.stats[2 * r] = 0.f; a.stats[2 * r + 1] = 0.f; }
+      continue;
+    }
+    if (!off) reg.load(row, C, lane);
+    if (RPB == 1) __syncthreads();                         // the slots of the row before are read no more
+    const Teacher q = group_teacher<G>(a, r, lane, off, t_of, c_of, red);
+    RowStat s;
+    s.m = Red<G>::max_(off ? -INFINITY : reg.lane_max(C), red);
+    if (s.m == -INFINITY) s.m = 0.f;
+    const RowRef ref(s.m, a.c2);
+    reg.fresh();
+    reg.template lane_sums<false>(ref, C, s.s, s.t);
+    s.s = Red<G>::sum_(s.s, red);
+    const float kl = group_kl<T, G>(a, r, row, lane, q, s, t_of, c_of, red);
+    if (lane == 0 && !off) {
+      if (q.sum != 0.f) total += (double)w * a.temperature * a.temperature * kl;
+      if (a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
+    }
+    if constexpr (GRAD) {
+      if (there) {
+        T* out = dx + a.vo.base(r);
+        const float inv_s = s.s == 0.f ? 0.f : 1.f / s.s, co = a.coef(w), dense = co * q.sum * inv_s;
+        reg.fresh();
+        if (off || q.sum == 0.f) reg.map_store(out, C, lane, [](float) { return 0.f; });
+        else {
+          reg.map_store(out, C, lane, [&](float v) { return dense * ex2(ref.z(v)); });
+          if (G > 64) __syncthreads();                     // another wave may have written the class
+          group_fix<T, G>(a, row, out, lane, 0, C, q.sum, co, ref, inv_s, t_of, c_of);
+        }
+      }
+    }
+  }
+  if (RPB > 1) {
+    total += __shfl_xor(total, 16, 64);
+    total += __shfl_xor(total, 32, 64);
+  }
+  if (threadIdx.x == 0) a.partial[blockIdx.x] = total;
+}
+
+// gradient alone, statistics given; a workgroup takes one part of a row
+template <typename T, int G, int NV>
+__global__ __launch_bounds__(G > 64 ? G : 64) void ds_bwd_group_kernel(DsArgs a, const T* __restrict__ x, T* __restrict__ dx, int part_len) {
+  constexpr int RPB = G > 64 ? 1 : 64 / G;
+  extern __shared__ __align__(16) char lds[];
+  __shared__ typename Red<G>::Buf red;
+  const int lane = threadIdx.x % G, sub = threadIdx.x / G, c0 = blockIdx.y * part_len;
+  const int n = min(part_len, a.v.C - c0);
+  float* t_of = reinterpret_cast<float*>(lds) + sub * a.K;
+  int* c_of = reinterpret_cast<int*>(lds) + (RPB + sub) * a.K;
+  const long long blocks = (a.rows + RPB - 1) / RPB;
+  for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const long long r = b * RPB + sub;
+    const bool there = r < a.rows;
+    const float w = there ? a.weight_of(r) : 0.f;
+    const bool off = w == 0.f;
+    RowRegs<T, G, NV> reg;
+    const T* row = x + (there ? a.v.base(r) : 0) + c0;
+    T* out = dx + (there ? a.vo.base(r) : 0) + c0;
+    if (off && RPB == 1) {
+      reg.map_store(out, n, lane, [](float) { return 0.f; });
+      continue;
+    }
+    if (!off) reg.load(row, n, lane);
+    if (RPB == 1) __syncthreads();
+    const Teacher q = group_teacher<G>(a, r, lane, off, t_of, c_of, red);
+    if (!there) continue;
+    if (off || q.sum == 0.f) {
+      reg.map_store(out, n, lane, [](float) { return 0.f; });
+      continue;
+    }
+    const float m = a.stats[2 * r], s = a.stats[2 * r + 1];
+    const RowRef ref(m, a.c2);
+    const float inv_s = s == 0.f ? 0.f : 1.f / s, co = a.coef(w), dense = co * q.sum * inv_s;
+    reg.map_store(out, n, lane, [&](float v) { return dense * ex2(ref.z(v)); });
+    if (G > 64) __syncthreads();                           // another wave may have written the class
+    group_fix<T, G>(a, row, out, lane, c0, n, q.sum, co, ref, inv_s, t_of, c_of);
+  }
+}
+
+// ---- long rows, or few of them: statistics by parts, joined by a wave that adds the row's loss ------------------------------------
+template <typename T, int NV>
+__global__ __launch_bounds__(256) void ds_part_kernel(DsArgs a, const T* __restrict__ x, int parts, int part_len, RowStat* __restrict__ part_stat) {
+  __shared__ Red<256>::Buf red;
+  const long long r = blockIdx.x;
+  const int part = blockIdx.y, c0 = part * part_len, lane = threadIdx.x;
+  if (a.weight_of(r) == 0.f) return;
+  const int n = min(part_len, a.v.C - c0);
+  RowRegs<T, 256, NV> reg;
+  reg.load(x + a.v.base(r) + c0, n, lane);
+  RowStat s;
+  s.m = Red<256>::max_(reg.lane_max(n), red);
+  if (s.m == -INFINITY) s.m = 0.f;
+  reg.fresh();
+  reg.template lane_sums<false>(RowRef(s.m, a.c2), n, s.s, s.t);
+  s.t = 0.f;
+  s.s = Red<256>::sum_(s.s, red);
+  if (lane == 0) part_stat[r * parts + part] = s;
+}
+template <typename T>
+__global__ __launch_bounds__(64) void ds_join_kernel(DsArgs a, const T* __restrict__ x, int parts, const RowStat* __restrict__ part_stat) {
+  extern __shared__ __align__(16) char lds[];
+  float* t_of = reinterpret_cast<float*>(lds);
+  int* c_of = reinterpret_cast<int*>(lds) + a.K;
+  Red<64>::Buf red;
+  const int lane = threadIdx.x;
+  double total = 0.0;
+  for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const float w = a.weight_of(r);
+    RowStat s{0.f, 0.f, 0.f};
+    if (w != 0.f) {
+      if (lane < parts) s = part_stat[r * parts + lane];
+      for (int o = 32; o > 0; o >>= 1) {
+        const RowStat u{__shfl_xor(s.m, o, 64), __shfl_xor(s.s, o, 64), 0.f};
+        s = lane & o ? join(u, s, a.c2) : join(s, u, a.c2);
+      }
+      const Teacher q = group_teacher<64>(a, r, lane, false, t_of, c_of, red);
+      const float kl = group_kl<T, 64>(a, r, x + a.v.base(r), lane, q, s, t_of, c_of, red);
+      if (q.sum != 0.f) total += (double)w * a.temperature * a.temperature * kl;
+    }
+    if (lane == 0 && a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
+  }
+  if (lane == 0) a.partial[blockIdx.x] = total;
+}
+
+// ---- one thread per row ----------------------------------------------------------------------------------------------------------
+// The teacher's softmax of a thread's own row; the slots are read once for the maximum, once for the sum and once for use.
+struct ThreadTeacher {
+  float vm, ln_sv, inv, sum;
+  RowRef ref;
+  __device__ __forceinline__ ThreadTeacher(const DsArgs& a, long long r, float w) : ref(0.f, a.c2) {
+    vm = -INFINITY;
+    bool bad = false;
+    float sv = 0.f;
+    if (w != 0.f) {
+      for (int k = 0; k < a.K; ++k) {
+        float val;
+        int cls;
+        a.slot(r, k, val, cls);
+        bad |= val != val || cls >= a.v.C;
+        vm = fmaxf(vm, val);
+      }
+      if (vm == -INFINITY) vm = 0.f;
+      ref = RowRef(vm, a.c2);
+      for (int k = 0; k < a.K; ++k) {
+        float val;
+        int cls;
+        a.slot(r, k, val, cls);
+        sv += ex2(ref.z(val));
+      }
+    }
+    inv = bad ? NAN : sv == 0.f ? 0.f : 1.f / sv;
+    ln_sv = w != 0.f ? ref.ln_s(vm, sv) : 0.f;
+    sum = bad || !(sv >= 0.f) ? NAN : sv == 0.f ? 0.f : 1.f;
+  }
+  __device__ __forceinline__ float t(const DsArgs& a, long long r, int k, float& val, int& cls) const {
+    a.slot(r, k, val, cls);
+    return ex2(ref.z(val)) * inv;
+  }
+};
+template <typename T> __device__ __forceinline__ float thread_kl(const DsArgs& a, long long r, const T* row, long long sc, const ThreadTeacher& q,
+                                                                 const RowStat& s) {
+  if (!(q.sum == q.sum)) return NAN;
+  const float ln_s = s.s == 0.f ? 0.f : RowRef(s.m, a.c2).ln_s(s.m, s.s);      // no class left: ln p = -inf
+  float kl = 0.f;
+  for (int k = 0; k < a.K; ++k) {
+    float val;
+    int cls;
+    const float t = q.t(a, r, k, val, cls);
+    if (t != 0.f) kl += slot_term(t, val, q.vm, q.ln_sv, ld(row + cls * sc), s.m, ln_s, a.temperature);
+  }
+  return kl;
+}
+__device__ __forceinline__ double wave_total(double v) {
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// MODE 0: loss, 1: gradient with statistics given, 2: both.  Up to 64 classes; what the teacher holds of each class is added up
+// in LDS (tab), so that a class named twice costs nothing and every gradient is rounded once.
+template <typename T, int CREG, bool STAGED, int MODE>
+__global__ __launch_bounds__(64) void ds_thread_kernel(DsArgs a, const T* __restrict__ x, T* __restrict__ dx, bool wide) {
+  extern __shared__ __align__(16) char lds[];
+  constexpr int E = 16 / sizeof(T);
+  const int lane = threadIdx.x, C = a.v.C;
+  float* tab = reinterpret_cast<float*>(lds);                                     // [C][64]
+  T* tile = reinterpret_cast<T*>(lds + (MODE ? (size_t)C * 64 * 4 : 0));
+  T* res = tile + (64 * (int)a.v.so + E - 1) / E * E;                              // STAGED, MODE > 0: the gradient on its way out
+  const long long blocks = (a.rows + 63) / 64;
+  double total = 0.0;
+  for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const long long r = b * 64 + lane;
+    const int here = (int)min(64ll, a.rows - b * 64);
+    const T* row;
+    if (STAGED) {
+      __syncthreads();
+      copy_to_lds(tile, x + b * 64 * a.v.so, (here - 1) * (int)a.v.so + C);
+      __syncthreads();
+      row = tile + lane * (int)a.v.so;
     } else {
-      const RowStat s = block_row_stat(row, v.C, v.sc, c2, fbuf);
-      m = s.m, l2 = stat_l2(s.s);
+      row = x + (lane < here ? a.v.base(r) : 0);
+    }
+    const long long sc = STAGED ? 1 : a.v.sc;
+    if (lane < here) {
+      const float w = a.weight_of(r);
+      const ThreadTeacher q(a, r, w);
+      float v[CREG];
+      const bool on = w != 0.f && q.sum != 0.f;
+      RowStat s{0.f, 0.f, 0.f};
+      if (on) {
+        load_classes<T, CREG, STAGED>(v, row, sc, C, wide);
+        if (MODE == 1) s.m = a.stats[2 * r], s.s = a.stats[2 * r + 1];
+        else s = thread_row_stat<CREG, false>(v, C, a.c2);
+      }
+      if (MODE != 1) {
+        if (on) total += (double)w * a.temperature * a.temperature * thread_kl(a, r, row, sc, q, s);
+        if (a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
+      }
+      if constexpr (MODE != 0) {
+        T* out = STAGED ? res + lane * C : dx + a.vo.base(r);
+        const long long osc = STAGED ? 1 : a.vo.sc;
+        if (!on) {
+          for (int c = 0; c < C; ++c) st(out + c * osc, 0.f);
+        } else {
+          const RowRef ref(s.m, a.c2);
+          const float inv_s = s.s == 0.f ? 0.f : 1.f / s.s, co = a.coef(w), scale_p = q.sum * inv_s;
+          for (int c = 0; c < C; ++c) tab[c * 64 + lane] = 0.f;
+          for (int k = 0; k < a.K; ++k) {
+            float val;
+            int cls;
+            const float t = q.t(a, r, k, val, cls);
+            if (cls >= 0 && cls < C) tab[cls * 64 + lane] += t;
+          }
+#pragma unroll
+          for (int c = 0; c < CREG; ++c)
+            if (c < C) st(out + c * osc, co * (scale_p * ex2(ref.z(v[c])) - tab[c * 64 + lane]));
+        }
+      }
+    }
+    if (STAGED && MODE != 0) {
+      __syncthreads();
+      copy_from_lds(dx + b * 64 * C, res, here * C);
+    }
+  }
+  if (MODE != 1) {
+    total = wave_total(total);
+    if (lane == 0) a.partial[blockIdx.x] = total;
+  }
+}
+
+// more classes, lying apart: the thread walks its row
+template <typename T, int MODE> __global__ __launch_bounds__(64) void ds_walk_kernel(DsArgs a, const T* __restrict__ x, T* __restrict__ dx) {
+  const int C = a.v.C;
+  const long long sc = a.v.sc, osc = a.vo.sc, blocks = (a.rows + 63) / 64;
+  double total = 0.0;
+  for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const long long r = b * 64 + threadIdx.x;
+    if (r >= a.rows) continue;
+    const T* row = x + a.v.base(r);
+    const float w = a.weight_of(r);
+    const ThreadTeacher q(a, r, w);
+    const bool on = w != 0.f && q.sum != 0.f;
+    RowStat s{0.f, 0.f, 0.f};
+    if (on) {
+      if (MODE == 1) s.m = a.stats[2 * r], s.s = a.stats[2 * r + 1];
+      else s = walk_row_stat(row, sc, C, a.c2);
     }
     if (MODE != 1) {
-      float part = 0.f;
-      if (bad != 0.f) part = NAN;
-      else if (t > 0.f) part = t * ((scaled(val, vm, temperature) - logf(sv)) - (scaled(ld(row + idx * v.sc), m, temperature) - l2 * UH_LN2));
-      else if (t != t) part = NAN;
-      part = block_sum(part, fbuf);
-      if (tid == 0) {
-        row_loss[r] = empty ? 0.f : w * temperature * temperature * part;
-        if (stats) { stats[2 * r] = m; stats[2 * r + 1] = l2; }
-      }
+      if (on) total += (double)w * a.temperature * a.temperature * thread_kl(a, r, row, sc, q, s);
+      if (a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
     }
-    if (MODE != 0) {
-      T* out = dx + vo.base(r);
-      const float a = empty ? 0.f : (MODE == 1 ? gout[0] * grad_scale : grad_scale) * w * temperature;
-      if (empty) {
-        for (int c = tid; c < v.C; c += 256) st(out + c * vo.sc, 0.f);
-        continue;
+    if constexpr (MODE != 0) {
+      T* out = dx + a.vo.base(r);
+      const RowRef ref(s.m, a.c2);
+      const float inv_s = s.s == 0.f ? 0.f : 1.f / s.s, co = a.coef(w), dense = co * q.sum * inv_s;
+      for (int c0 = 0; c0 < C; c0 += 8) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c0 + j < C && on ? ld(row + (c0 + j) * sc) : 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c0 + j < C) st(out + (c0 + j) * osc, on ? dense * ex2(ref.z(v[j])) : 0.f);
       }
-      const float sum_t = bad != 0.f || !(sv >= 0.f) ? NAN : 1.f;
-      for (int c = tid; c < v.C; c += 256) st(out + c * vo.sc, a * sum_t * ex2((ld(row + c * v.sc) - m) * c2 - l2));
-      __syncthreads();                                 // the dense part is written before a slot's class is written again
-      if (tid < sl.K && idx >= 0 && idx < v.C) {
-        float mine = 0.f;
-        for (int k = 0; k < sl.K; ++k) mine += i_of[k] == idx ? t_of[k] : 0.f;
-        st(out + idx * vo.sc, a * (sum_t * ex2((ld(row + idx * v.sc) - m) * c2 - l2) - mine));
-      }
+      if (on)
+        for (int k = 0; k < a.K; ++k) {
+          float val, mine = 0.f;
+          int cls, other;
+          a.slot(r, k, val, cls);
+          if (cls < 0 || cls >= C) continue;
+          for (int j = 0; j < a.K; ++j) {
+            const float t = q.t(a, r, j, val, other);
+            mine += other == cls ? t : 0.f;
+          }
+          st(out + cls * osc, co * (q.sum * (ex2(ref.z(ld(row + cls * sc))) * inv_s) - mine));
+        }
     }
+  }
+  if (MODE != 1) {
+    total = wave_total(total);
+    if (threadIdx.x == 0) a.partial[blockIdx.x] = total;
   }
 }
 
-// loss = scale * sum of the rows' losses, in 64 bits and a fixed order
-__global__ __launch_bounds__(1024) void distill_finish_kernel(long long n, const float* __restrict__ row_loss, double scale,
-                                                              float* __restrict__ loss) {
-  __shared__ double buf[1024];
-  double a = 0.0;
-  for (long long i = threadIdx.x; i < n; i += 1024) a += (double)row_loss[i];
-  buf[threadIdx.x] = a;
-  __syncthreads();
-  for (int o = 512; o > 0; o >>= 1) {
-    if (threadIdx.x < o) buf[threadIdx.x] += buf[threadIdx.x + o];
+// ---- one workgroup per row, any strides ----------------------------------------------------------------------------------------
+template <typename T, int MODE> __global__ __launch_bounds__(256) void ds_any_kernel(DsArgs a, const T* __restrict__ x, T* __restrict__ dx) {
+  extern __shared__ __align__(16) char lds[];
+  float* t_of = reinterpret_cast<float*>(lds);
+  int* c_of = reinterpret_cast<int*>(lds) + a.K;
+  __shared__ Red<256>::Buf red;
+  const int lane = threadIdx.x, C = a.v.C;
+  double total = 0.0;
+  for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const float w = a.weight_of(r);
+    const T* row = x + a.v.base(r);
     __syncthreads();
+    const Teacher q = group_teacher<256>(a, r, lane, w == 0.f, t_of, c_of, red);
+    const bool on = q.sum != 0.f;
+    RowStat s{0.f, 0.f, 0.f};
+    if (on) {
+      if (MODE == 1) s.m = a.stats[2 * r], s.s = a.stats[2 * r + 1];
+      else s = strided_row_stat<T, 256>(row, C, a.v.sc, a.c2, lane, red);
+    }
+    if (MODE != 1) {
+      const float kl = group_kl<T, 256>(a, r, row, lane, q, s, t_of, c_of, red);
+      if (lane == 0) {
+        if (on) total += (double)w * a.temperature * a.temperature * kl;
+        if (a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
+      }
+    }
+    if constexpr (MODE != 0) {
+      T* out = dx + a.vo.base(r);
+      const RowRef ref(s.m, a.c2);
+      const float inv_s = s.s == 0.f ? 0.f : 1.f / s.s, co = a.coef(w), dense = co * q.sum * inv_s;
+      for (int c = lane; c < C; c += 256) st(out + c * a.vo.sc, on ? dense * ex2(ref.z(ld(row + c * a.v.sc))) : 0.f);
+      __syncthreads();
+      if (on) group_fix<T, 256>(a, row, out, lane, 0, C, q.sum, co, ref, inv_s, t_of, c_of);
+    }
   }
-  if (threadIdx.x == 0) loss[0] = (float)(buf[0] * scale);
+  if (MODE != 1 && lane == 0) a.partial[blockIdx.x] = total;
 }
 
-// ---- host ---------------------------------------------------------------------------------------------------------------
-static unsigned row_grid(long long rows) { return (unsigned)(rows < (1 << 20) ? rows : (1 << 20)); }
+__global__ __launch_bounds__(1024) void ds_finish_kernel(int n, const double* __restrict__ partial, double scale, float* __restrict__ loss) {
+  __shared__ double buf[16];
+  double v = 0.0;
+  for (int i = threadIdx.x; i < n; i += 1024) v += partial[i];
+  v = wave_total(v);
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) v += buf[w];
+    loss[0] = (float)(v * scale);
+  }
+}
 
+// ---- host ---------------------------------------------------------------------------------------------------------------------------
 static int distill_check(const char* who, const uh_class_view* v, const void* logits, const uh_slots* sl, float temperature) {
   const int ok = uh_check_view(v, who);
   if (ok != UH_OK) return ok;
@@ -129,26 +492,103 @@ static int same_rows(const char* who, const uh_class_view* v, const uh_class_vie
   return UH_OK;
 }
 
-template <int MODE>
-static void distill_launch(const uh_class_view* view, const uh_class_view* out_view, const void* logits, const uh_slots* s,
-                           const float* weight, float temperature, float grad_scale, const float* gout, float* stats,
-                           float* row_loss, void* dx, hipStream_t st) {
-  const RowView v = uh_row_view(view), vo = uh_row_view(out_view);
-  const long long rows = v.outer * v.inner;
-  const float c2 = (float)(1.4426950408889634 / (double)temperature);
-  const Slots sl{s->value, s->index, s->slots, s->value_dtype, s->index_bytes};
-#define UH_GO(T)                                                                                                       \
-  hipLaunchKernelGGL((distill_any_kernel<T, MODE>), dim3(row_grid(rows)), dim3(256), 0, st, v, vo, rows,               \
-                     (const T*)logits, sl, weight, temperature, c2, grad_scale, gout, stats, row_loss, (T*)dx)
-  if (view->dtype == UH_F32) UH_GO(float);
-  else if (view->dtype == UH_BF16) UH_GO(bf16);
-  else UH_GO(f16);
+static DsArgs ds_args(const uh_class_view* view, const uh_class_view* out, const uh_slots* s, const float* weight, float temperature) {
+  DsArgs a;
+  a.v = uh_row_view(view), a.vo = uh_row_view(out);
+  a.rows = view->outer * view->inner;
+  a.value = s->value, a.index = s->index, a.K = s->slots, a.value_dtype = s->value_dtype, a.index_bytes = s->index_bytes;
+  a.weight = weight, a.temperature = temperature, a.c2 = (float)(1.4426950408889634 / (double)temperature);
+  a.grad_scale = 0.f, a.gout = nullptr, a.stats = nullptr, a.partial = nullptr;
+  return a;
+}
+
+// Workspace of a call: the workgroups' sums, then (rows that are cut) the rows' statistics and those of their parts.
+struct DsPlan {
+  ClassPath path;
+  RowCut cut;
+  size_t stats_at, parts_at, bytes;
+};
+static DsPlan ds_plan(const RowView& v, const RowView* vo, long long rows, int dtype) {
+  DsPlan p;
+  p.path = uh_class_path(v, vo, rows);
+  p.cut = p.path == PATH_GROUP ? uh_row_cut(rows, v.C, dtype) : RowCut{1, v.C};
+  p.stats_at = UH_GRID_WAVES * sizeof(double);
+  p.parts_at = p.stats_at + (p.cut.parts > 1 ? ((size_t)rows * 8 + 15) / 16 * 16 : 0);
+  p.bytes = p.parts_at + (p.cut.parts > 1 ? (size_t)rows * p.cut.parts * sizeof(RowStat) : 0);
+  return p;
+}
+
+// MODE 0: loss, 1: gradient, 2: both; returns how many partial sums there are
+template <typename T, int MODE> static int ds_launch(const DsArgs& a, const T* x, T* dx, const DsPlan& p, char* ws, hipStream_t s) {
+  constexpr int E = 16 / sizeof(T);
+  const int C = a.v.C;
+  const long long rows = a.rows;
+  const unsigned waves = uh_grid((rows + 63) / 64, UH_GRID_WAVES), blocks = uh_grid(rows, UH_GRID_WAVES);
+  if (p.path == PATH_STAGED || p.path == PATH_APART) {
+    const bool staged = p.path == PATH_STAGED, wide = staged && (a.v.so * sizeof(T)) % 16 == 0;
+    const size_t lds = (MODE ? (size_t)C * 64 * 4 : 0) + (staged ? ((64 * a.v.so + E - 1) / E * E + (MODE ? 64 * C : 0)) * sizeof(T) : 0);
+#define UH_GO2(R, ST) hipLaunchKernelGGL((ds_thread_kernel<T, R, ST, MODE>), dim3(waves), dim3(64), lds, s, a, x, dx, wide)
+#define UH_GO(ST) do { if (C <= 8) UH_GO2(8, ST); else if (C <= 16) UH_GO2(16, ST); else if (C <= 32) UH_GO2(32, ST); else UH_GO2(64, ST); } while (0)
+    if (staged) UH_GO(true); else UH_GO(false);
 #undef UH_GO
+#undef UH_GO2
+    return (int)waves;
+  }
+  const size_t slots = (size_t)a.K * 8;
+  if (p.path == PATH_WALK) {
+    hipLaunchKernelGGL((ds_walk_kernel<T, MODE>), dim3(waves), dim3(64), 0, s, a, x, dx);
+    return (int)waves;
+  }
+  if (p.path == PATH_ANY) {
+    hipLaunchKernelGGL((ds_any_kernel<T, MODE>), dim3(blocks), dim3(256), slots, s, a, x, dx);
+    return (int)blocks;
+  }
+  if constexpr (MODE == 1) {
+    if (C <= 16 * 4 * E)
+      hipLaunchKernelGGL((ds_bwd_group_kernel<T, 16, 4>), dim3(uh_grid((rows + 3) / 4, UH_GRID_WAVES)), dim3(64), 4 * slots, s, a, x, dx, C);
+    else if (C <= 64 * 4 * E)
+      hipLaunchKernelGGL((ds_bwd_group_kernel<T, 64, 4>), dim3(blocks), dim3(64), slots, s, a, x, dx, C);
+    else {
+      const RowCut cut = uh_cut_parts(C, (C + 256 * 4 * E - 1) / (256 * 4 * E));
+      hipLaunchKernelGGL((ds_bwd_group_kernel<T, 256, 4>), dim3(blocks, (unsigned)cut.parts), dim3(256), slots, s, a, x, dx, cut.len);
+    }
+    return 0;
+  } else {
+    if (p.cut.parts > 1) {
+      RowStat* ps = (RowStat*)(ws + p.parts_at);
+      DsArgs j = a;
+      if (!j.stats) j.stats = (float*)(ws + p.stats_at);
+      const dim3 grid((unsigned)rows, (unsigned)p.cut.parts);
+#define UH_GO(NV) hipLaunchKernelGGL((ds_part_kernel<T, NV>), grid, dim3(256), 0, s, j, x, p.cut.parts, p.cut.len, ps)
+      if (p.cut.len <= 256 * E) UH_GO(1); else if (p.cut.len <= 256 * 4 * E) UH_GO(4); else if (p.cut.len <= 256 * 8 * E) UH_GO(8); else UH_GO(16);
+#undef UH_GO
+      hipLaunchKernelGGL((ds_join_kernel<T>), dim3(blocks), dim3(64), slots, s, j, x, p.cut.parts, ps);
+      if (MODE == 2) ds_launch<T, 1>(j, x, dx, p, ws, s);
+      return (int)blocks;
+    }
+#define UH_GO(G, NV, GR, R) hipLaunchKernelGGL((ds_group_kernel<T, G, NV, MODE == 2>), dim3(GR), dim3(G > 64 ? G : 64), R * slots, s, a, x, dx)
+    const unsigned quads = uh_grid((rows + 3) / 4, UH_GRID_WAVES);
+    if (C <= 16 * 4 * E) { UH_GO(16, 4, quads, 4); return (int)quads; }
+    if (C <= 64 * 4 * E) UH_GO(64, 4, blocks, 1);
+    else if (C <= 64 * 8 * E) UH_GO(64, 8, blocks, 1);
+    else if (C <= 256 * 4 * E) UH_GO(256, 4, blocks, 1);
+    else if (C <= 256 * 8 * E) UH_GO(256, 8, blocks, 1);
+    else UH_GO(256, 16, blocks, 1);
+#undef UH_GO
+    return (int)blocks;
+  }
+}
+
+template <int MODE> static int ds_dispatch(const DsArgs& a, int dtype, const void* x, void* dx, const DsPlan& p, void* ws, hipStream_t s) {
+  if (dtype == UH_F32) return ds_launch<float, MODE>(a, (const float*)x, (float*)dx, p, (char*)ws, s);
+  if (dtype == UH_BF16) return ds_launch<bf16, MODE>(a, (const bf16*)x, (bf16*)dx, p, (char*)ws, s);
+  return ds_launch<f16, MODE>(a, (const f16*)x, (f16*)dx, p, (char*)ws, s);
 }
 
 extern "C" size_t uh_topk_distill_workspace(const uh_class_view* view) {
   if (uh_check_view(view, "topk_distill_workspace") != UH_OK) return 0;
-  return (size_t)(view->outer * view->inner) * sizeof(float);
+  const RowView v = uh_row_view(view);
+  return ds_plan(v, nullptr, view->outer * view->inner, view->dtype).bytes;
 }
 
 extern "C" int uh_topk_distill(const uh_class_view* view, const void* logits, const uh_slots* slots, const float* weight,
@@ -156,11 +596,13 @@ extern "C" int uh_topk_distill(const uh_class_view* view, const void* logits, co
                                size_t workspace_bytes, uh_stream s) {
   const int ok = distill_check("topk_distill", view, logits, slots, temperature);
   if (ok != UH_OK) return ok;
-  UH_REQUIRE(loss && workspace && workspace_bytes >= uh_topk_distill_workspace(view), "topk_distill: null pointer or workspace of %zu bytes",
-             workspace_bytes);
-  distill_launch<0>(view, view, logits, slots, weight, temperature, 0.f, nullptr, stats, (float*)workspace, nullptr, (hipStream_t)s);
-  hipLaunchKernelGGL(distill_finish_kernel, dim3(1), dim3(1024), 0, (hipStream_t)s, view->outer * view->inner,
-                     (const float*)workspace, scale, loss);
+  UH_REQUIRE(loss && workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= uh_topk_distill_workspace(view),
+             "topk_distill: null pointer or workspace of %zu bytes", workspace_bytes);
+  DsArgs a = ds_args(view, view, slots, weight, temperature);
+  a.stats = stats, a.partial = (double*)workspace;
+  const DsPlan p = ds_plan(a.v, nullptr, a.rows, view->dtype);
+  const int n = ds_dispatch<0>(a, view->dtype, logits, nullptr, p, workspace, (hipStream_t)s);
+  hipLaunchKernelGGL(ds_finish_kernel, dim3(1), dim3(1024), 0, (hipStream_t)s, n, (const double*)workspace, scale, loss);
   return uh_check_launch("topk_distill");
 }
 
@@ -171,8 +613,10 @@ extern "C" int uh_topk_distill_bwd(const uh_class_view* view, const uh_class_vie
   if (ok == UH_OK) ok = same_rows("topk_distill_bwd", view, out_view);
   if (ok != UH_OK) return ok;
   UH_REQUIRE(gout && stats && dlogits, "topk_distill_bwd: null pointer");
-  distill_launch<1>(view, out_view, logits, slots, weight, temperature, (float)scale, gout, const_cast<float*>(stats), nullptr,
-                    dlogits, (hipStream_t)s);
+  DsArgs a = ds_args(view, out_view, slots, weight, temperature);
+  a.gout = gout, a.grad_scale = (float)scale, a.stats = const_cast<float*>(stats);
+  const DsPlan p = ds_plan(a.v, &a.vo, a.rows, view->dtype);
+  ds_dispatch<1>(a, view->dtype, logits, dlogits, p, nullptr, (hipStream_t)s);
   return uh_check_launch("topk_distill_bwd");
 }
 
@@ -183,11 +627,12 @@ extern "C" int uh_topk_distill_step(const uh_class_view* view, const uh_class_vi
   int ok = distill_check("topk_distill_step", view, logits, slots, temperature);
   if (ok == UH_OK) ok = same_rows("topk_distill_step", view, out_view);
   if (ok != UH_OK) return ok;
-  UH_REQUIRE(loss && dlogits && workspace && workspace_bytes >= uh_topk_distill_workspace(view),
+  UH_REQUIRE(loss && dlogits && workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= uh_topk_distill_workspace(view),
              "topk_distill_step: null pointer or workspace of %zu bytes", workspace_bytes);
-  distill_launch<2>(view, out_view, logits, slots, weight, temperature, (float)(scale * (double)grad_scale), nullptr, nullptr,
-                    (float*)workspace, dlogits, (hipStream_t)s);
-  hipLaunchKernelGGL(distill_finish_kernel, dim3(1), dim3(1024), 0, (hipStream_t)s, view->outer * view->inner,
-                     (const float*)workspace, scale, loss);
+  DsArgs a = ds_args(view, out_view, slots, weight, temperature);
+  a.grad_scale = (float)(scale * (double)grad_scale), a.partial = (double*)workspace;
+  const DsPlan p = ds_plan(a.v, &a.vo, a.rows, view->dtype);
+  const int n = ds_dispatch<2>(a, view->dtype, logits, dlogits, p, workspace, (hipStream_t)s);
+  hipLaunchKernelGGL(ds_finish_kernel, dim3(1), dim3(1024), 0, (hipStream_t)s, n, (const double*)workspace, scale, loss);
   return uh_check_launch("topk_distill_step");
 }
