@@ -51,10 +51,10 @@ __global__ __launch_bounds__(G > 64 ? G : 64) void lp_group_kernel(LpArgs a, con
   constexpr int RPB = G > 64 ? 1 : 64 / G;
   constexpr int E = RowRegs<T, G, NV>::E;
   __shared__ typename Red<G>::Buf red;
-  const int lane = threadIdx.x % G;
   const int C = a.v.C;
   const long long blocks = (a.rows + RPB - 1) / RPB;
   for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const int lane = renew(threadIdx.x % G);
     const long long r = b * RPB + threadIdx.x / G;
     const bool there = r < a.rows;
     const long long l = there ? a.label(r) : 0;
@@ -82,8 +82,7 @@ __global__ __launch_bounds__(G > 64 ? G : 64) void lp_group_kernel(LpArgs a, con
       else if (LIST > 0 || TOP) ln_s = RowRef(s.m, a.c2).ln_s(s.m, s.s);
     }
     if constexpr (LIST > 0) {
-      typedef SmallKey<T> SK;
-      typename SK::K list[LIST] = {};
+      TopList<LIST> list;
       reg.fresh();
       if (!off) {
 #pragma unroll
@@ -91,39 +90,48 @@ __global__ __launch_bounds__(G > 64 ? G : 64) void lp_group_kernel(LpArgs a, con
           if (q * G * E < C) {
             const int e = RowRegs<T, G, NV>::first(q, lane, C);
 #pragma unroll
-            for (int j = 0; j < E; ++j) list_insert(list, SK::make(reg.get(q, j), e + j));
+            for (int j = 0; j < E; ++j) list.insert(reg.get(q, j), e + j);
           }
       }
       for (int k = 0; k < a.top; ++k) {
-        const typename SK::K best = group_max<G>(list[0]);
-        if (list[0] == best && best != 0) {
-          a.write_top(r, k, SK::val(best), SK::cls(best), s.m, ln_s, s.s);
-#pragma unroll
-          for (int i = 0; i + 1 < LIST; ++i) list[i] = list[i + 1];
-          list[LIST - 1] = 0;
-        } else if (best == 0 && lane == 0 && !off) {
-          a.write_top(r, k, 0.f, -1, s.m, ln_s, s.s);
+        const uint64_t head = list.c[0] < 0 ? 0 : rank_key(list.v[0], list.c[0]);
+        const uint64_t best = group_max<G>(head);
+        if (best == 0 ? lane == 0 && !off : head == best) {
+          a.write_top(r, k, list.v[0], best ? list.c[0] : -1, s.m, ln_s, s.s);
+          list.pop();
         }
       }
     }
     if constexpr (TOP) {
       __shared__ TopBuf<G> tb;
-      group_top<T, G, NV>(reg, row, C, lane, 0, a.top, lm, tb, red, [&](int k, uint64_t key) {
+      uint32_t low;
+      const int found = group_candidates<T, G, NV>(reg, C, lane, 0, a.top, lm, tb, low);
+      const auto emit = [&](int k, uint64_t key) {
         a.write_top(r, k, key_value(key), key ? key_class(key) : -1, s.m, ln_s, s.s);
-      });
+      };
+      if (found <= TopBuf<G>::CAP) group_rank<G>(tb.list, found, lane, a.top, emit);
+      else group_rounds<T, G>(row, C, lane, 0, a.top, red, emit);
     }
   }
 }
 
 // ---- long rows, or few of them: a workgroup takes one part of a row, a wave joins a row's parts ---------------------------------
-// part_stat[row][part] = (m, s, t); part_top[row][part][top]: rank keys, falling, 0 behind the last
+// A part leaves its statistics and candidates for the alternatives in any order: all it found, or the `top` largest where
+// that is more than `keep`.  low: order32 of a value that at least `top` of the part's elements reach (0: there are fewer).
+struct LpPart {
+  float m, s, t;
+  uint32_t low;
+  int count, pad[3];
+};
+static inline int lp_keep(int top) { return top ? top + 32 : 0; }
+
 template <typename T, int NV, bool TOP>
-__global__ __launch_bounds__(256) void lp_part_kernel(LpArgs a, const T* __restrict__ x, int parts, int part_len,
-                                                      RowStat* __restrict__ part_stat, uint64_t* __restrict__ part_top) {
+__global__ __launch_bounds__(256) void lp_part_kernel(LpArgs a, const T* __restrict__ x, int parts, int part_len, int keep,
+                                                      LpPart* __restrict__ part, uint64_t* __restrict__ part_top) {
   __shared__ Red<256>::Buf red;
-  const long long r = blockIdx.x;
-  const int part = blockIdx.y, c0 = part * part_len, lane = threadIdx.x;
-  if (a.ignored(a.label(r))) return;                       // the joining wave does not look at the parts of such a row
+  const long long r = blockIdx.x, me = r * parts + blockIdx.y;
+  const int c0 = blockIdx.y * part_len, lane = threadIdx.x;
+  if (a.ignored(a.label(r))) return;                       // the join does not look at the parts of such a row
   const int n = min(part_len, a.v.C - c0);
   RowRegs<T, 256, NV> reg;
   const T* row = x + a.v.base(r) + c0;
@@ -135,48 +143,72 @@ __global__ __launch_bounds__(256) void lp_part_kernel(LpArgs a, const T* __restr
   reg.fresh();
   reg.template lane_sums<true>(RowRef(s.m, a.c2), n, s.s, s.t);
   Red<256>::sum2(s.s, s.t, red);
-  if (lane == 0) part_stat[r * parts + part] = s;
+  uint32_t low = 0;
+  int found = 0;
   if constexpr (TOP) {
     __shared__ TopBuf<256> tb;
-    uint64_t* out = part_top + (r * parts + part) * a.top;
-    group_top<T, 256, NV>(reg, row, n, lane, c0, a.top, lm, tb, red, [&](int k, uint64_t key) { out[k] = key; });
+    uint64_t* out = part_top + me * keep;
+    found = group_candidates<T, 256, NV>(reg, n, lane, c0, a.top, lm, tb, low);
+    if (found > TopBuf<256>::CAP) {
+      group_rounds<T, 256>(row, n, lane, c0, a.top, red, [&](int k, uint64_t key) { out[k] = key; });
+      found = a.top;                                       // those left over are 0: below any bound
+    } else {
+      if (found > keep) {
+        if (lane < 64) wave_cut(tb.list, found, a.top);
+        found = a.top;
+        __syncthreads();
+      }
+      for (int i = lane; i < found; i += 256) out[i] = tb.list[i];
+    }
+  }
+  if (lane == 0) {
+    LpPart& p = part[me];
+    p.m = s.m, p.s = s.s, p.t = s.t, p.low = low, p.count = found;
   }
 }
 
 template <typename T>
-__global__ __launch_bounds__(64) void lp_join_kernel(LpArgs a, const T* __restrict__ x, int parts, const RowStat* __restrict__ part_stat,
-                                                     const uint64_t* __restrict__ part_top) {
-  extern __shared__ uint64_t keys[];                       // parts * top of them
+__global__ __launch_bounds__(256) void lp_join_kernel(LpArgs a, const T* __restrict__ x, int parts, int keep, const LpPart* __restrict__ part,
+                                                      const uint64_t* __restrict__ part_top) {
+  extern __shared__ __align__(16) uint64_t keys[];         // parts * keep of them and two to spare
   __shared__ int count;
   const long long r = blockIdx.x;
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63;
   const long long l = a.label(r);
   if (a.ignored(l)) {
-    if (lane == 0) a.write_ignored(r);
-    for (int k = lane; k < a.top; k += 64) a.write_top(r, k, 0.f, -1, 0.f, 0.f, 0.f);
+    if (threadIdx.x == 0) a.write_ignored(r);
+    for (int k = threadIdx.x; k < a.top; k += 256) a.write_top(r, k, 0.f, -1, 0.f, 0.f, 0.f);
     return;
   }
-  RowStat s = lane < parts ? part_stat[r * parts + lane] : RowStat{0.f, 0.f, 0.f};
-  for (int o = 32; o > 0; o >>= 1) {
+  if (threadIdx.x == 0) count = 0;
+  __syncthreads();
+  // every wave joins the statistics for itself
+  const LpPart* p = part + r * parts + min(lane, parts - 1);
+  RowStat s{p->m, p->s, p->t};
+  uint32_t low = p->low;
+  const int mine = p->count;
+  if (lane >= parts) s.s = s.t = 0.f;                      // nobody's part
+  for (int o = 1; o < 64 && o < parts; o <<= 1) {
     const RowStat u{__shfl_xor(s.m, o, 64), __shfl_xor(s.s, o, 64), __shfl_xor(s.t, o, 64)};
     s = lane & o ? join(u, s, a.c2) : join(s, u, a.c2);    // the same order of the two in both lanes
+    low = max(low, (uint32_t)__shfl_xor(low, o, 64));
   }
+  s = RowStat{__shfl(s.m, 0, 64), __shfl(s.s, 0, 64), __shfl(s.t, 0, 64)};
+  low = __shfl(low, 0, 64);
   const float ln_s = RowRef(s.m, a.c2).ln_s(s.m, s.s);
-  if (lane == 0) a.write_row(r, l, a.is_class(l) ? ld(x + a.v.base(r) + l) : 0.f, s);
+  if (threadIdx.x == 0) a.write_row(r, l, a.is_class(l) ? ld(x + a.v.base(r) + l) : 0.f, s);
   if (a.top == 0) return;
-  // the best of the parts' last places bounds the row's last place from below
-  const uint64_t* mine = part_top + (r * parts + lane) * a.top;
-  const uint64_t cut = group_max<64>(lane < parts ? mine[a.top - 1] : (uint64_t)0);
-  if (lane == 0) count = 0;
-  __syncthreads();
-  if (lane < parts)
-    for (int k = 0; k < a.top; ++k) {
-      const uint64_t key = mine[k];
-      if (key < cut || key == 0) break;
-      keys[atomicAdd(&count, 1)] = key;
+  const uint64_t cut = max((uint64_t)low << 32, (uint64_t)1);
+  const uint64_t* from = part_top + r * parts * keep;
+  for (int q = threadIdx.x >> 6; q < parts; q += 4) {      // a wave a part
+    const int n = __shfl(mine, q, 64);
+    for (int i = lane; i < n; i += 64) {
+      const uint64_t key = from[q * keep + i];
+      if (key >= cut) keys[atomicAdd(&count, 1)] = key;
     }
+  }
   __syncthreads();
-  wave_select(keys, count, a.top, [&](int k, uint64_t key) {
+  group_rank<256>(keys, count, threadIdx.x, a.top, [&](int k, uint64_t key) {
     a.write_top(r, k, key_value(key), key ? key_class(key) : -1, s.m, ln_s, s.s);
   });
 }
@@ -203,38 +235,35 @@ __global__ __launch_bounds__(64) void lp_thread_kernel(LpArgs a, const T* __rest
       row = x + (there ? a.v.base(r) : 0);
     }
     if (!there) continue;
+    float v[CREG];
+    load_classes<T, CREG, STAGED>(v, row, a.v.sc, C, wide);                       // on its way while the label is
     const long long l = a.label(r);
     if (a.ignored(l)) {
       a.write_ignored(r);
       for (int k = 0; k < a.top; ++k) a.write_top(r, k, 0.f, -1, 0.f, 0.f, 0.f);
       continue;
     }
-    float v[CREG];
-    load_classes<T, CREG, STAGED>(v, row, a.v.sc, C, wide);
     const RowStat s = thread_row_stat<CREG, true>(v, C, a.c2);
     const float ln_s = a.write_row(r, l, a.is_class(l) ? ld(row + (STAGED ? l : l * a.v.sc)) : 0.f, s);
     if constexpr (LIST > 0) {
-      typedef SmallKey<T> SK;
-      typename SK::K last = ~(typename SK::K)0;
+      float lv = 0.f;
+      int lc = 0;
       for (int k0 = 0; k0 < a.top; k0 += LIST) {
-        typename SK::K list[LIST] = {};
+        TopList<LIST> list;
         if constexpr (STAGED || CREG == 64) {              // from LDS or the caches again: 64 unrolled steps cost 256 registers
           for (int c = 0; c < C; ++c) {
-            const typename SK::K key = SK::make((float)row[STAGED ? c : c * a.v.sc], c);
-            list_insert(list, key < last ? key : 0);
+            const float u = (float)row[STAGED ? c : c * a.v.sc];
+            list.insert(k0 ? behind(u, c, lv, lc) : u, c);
           }
         } else {
 #pragma unroll
           for (int c = 0; c < CREG; ++c)
-            if (c < C) {
-              const typename SK::K key = SK::make(v[c], c);
-              list_insert(list, key < last ? key : 0);
-            }
+            if (c < C) list.insert(k0 ? behind(v[c], c, lv, lc) : v[c], c);
         }
 #pragma unroll
         for (int i = 0; i < LIST; ++i)
-          if (k0 + i < a.top) a.write_top(r, k0 + i, SK::val(list[i]), list[i] ? SK::cls(list[i]) : -1, s.m, ln_s, s.s);
-        last = list[LIST - 1];
+          if (k0 + i < a.top) a.write_top(r, k0 + i, list.v[i], list.c[i], s.m, ln_s, s.s);
+        lv = list.v[LIST - 1], lc = list.c[LIST - 1];
       }
     }
   }
@@ -256,23 +285,24 @@ __global__ __launch_bounds__(64) void lp_walk_kernel(LpArgs a, const T* __restri
   const RowStat s = walk_row_stat(row, a.v.sc, C, a.c2);
   const float ln_s = a.write_row(r, l, a.is_class(l) ? ld(row + l * a.v.sc) : 0.f, s);
   if constexpr (LIST > 0) {
-    uint64_t last = ~0ull;
+    float lv = 0.f;
+    int lc = 0;
     for (int k0 = 0; k0 < a.top; k0 += LIST) {
-      uint64_t list[LIST] = {};
+      TopList<LIST> list;
       for (int c0 = 0; c0 < C; c0 += 8) {
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = c0 + j < C ? ld(row + (c0 + j) * a.v.sc) : -INFINITY;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const uint64_t key = rank_key(v[j], c0 + j);
-          if (key > list[LIST - 1] && key < last) list_insert(list, key);
+          const float u = k0 ? behind(v[j], c0 + j, lv, lc) : v[j];
+          if (u > list.v[LIST - 1]) list.insert(u, c0 + j);
         }
       }
 #pragma unroll
       for (int i = 0; i < LIST; ++i)
-        if (k0 + i < a.top) a.write_top(r, k0 + i, key_value(list[i]), list[i] ? key_class(list[i]) : -1, s.m, ln_s, s.s);
-      last = list[LIST - 1];
+        if (k0 + i < a.top) a.write_top(r, k0 + i, list.v[i], list.c[i], s.m, ln_s, s.s);
+      lv = list.v[LIST - 1], lc = list.c[LIST - 1];
     }
   }
 }
@@ -345,10 +375,11 @@ struct LpCoef {
 template <typename T, int G, int NV>
 __global__ __launch_bounds__(G > 64 ? G : 64) void lp_bwd_group_kernel(LpBwd k, const T* __restrict__ x, T* __restrict__ dx, int part_len) {
   constexpr int RPB = G > 64 ? 1 : 64 / G;
-  const int lane = threadIdx.x % G, c0 = blockIdx.y * part_len;
+  const int c0 = blockIdx.y * part_len;
   const int n = min(part_len, k.v.C - c0);
   const long long blocks = (k.rows + RPB - 1) / RPB;
   for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const int lane = renew(threadIdx.x % G);
     const long long r = b * RPB + threadIdx.x / G;
     if (r >= k.rows) continue;
     const LpCoef q(k, r);
@@ -448,7 +479,7 @@ extern "C" size_t uh_label_log_probs_workspace(const uh_class_view* view, int to
   const long long rows = view->outer * view->inner;
   const int parts = lp_cut(uh_row_view(view), rows, view->dtype).parts;
   if (parts == 1) return 0;
-  return (size_t)rows * parts * (16 + 8 * (size_t)top);         // a part's statistics (12 of 16) and its keys
+  return (size_t)rows * parts * (sizeof(LpPart) + 8 * (size_t)lp_keep(top));
 }
 
 template <typename T> static void lp_launch(const LpArgs& a, const T* x, int dtype, void* ws, hipStream_t s) {
@@ -461,8 +492,8 @@ template <typename T> static void lp_launch(const LpArgs& a, const T* x, int dty
     const bool staged = path == PATH_STAGED, wide = staged && (a.v.so * sizeof(T)) % 16 == 0;
     const size_t lds = staged ? (size_t)64 * a.v.so * sizeof(T) : 0;
 #define UH_GO3(R, ST, LI) hipLaunchKernelGGL((lp_thread_kernel<T, R, ST, LI>), waves, dim3(64), lds, s, a, x, wide)
-#define UH_GO2(R, ST) do { if (a.top == 0) UH_GO3(R, ST, 0); else if (a.top <= 4) UH_GO3(R, ST, 4); else UH_GO3(R, ST, 8); } while (0)
-#define UH_GO(ST) do { if (C <= 8) UH_GO2(8, ST); else if (C <= 16) UH_GO2(16, ST); else if (C <= 32) UH_GO2(32, ST); else UH_GO2(64, ST); } while (0)
+#define UH_GO2(R, ST) do { if (a.top == 0) UH_GO3(R, ST, 0); else if (a.top <= 2) UH_GO3(R, ST, 2); else if (a.top == 3) UH_GO3(R, ST, 3); else if (a.top <= 5) UH_GO3(R, ST, 5); else UH_GO3(R, ST, 8); } while (0)
+#define UH_GO(ST) do { if (C <= 16) UH_GO2(16, ST); else if (C <= 32) UH_GO2(32, ST); else UH_GO2(64, ST); } while (0)
     if (staged) UH_GO(true); else UH_GO(false);
 #undef UH_GO
 #undef UH_GO2
@@ -475,17 +506,18 @@ template <typename T> static void lp_launch(const LpArgs& a, const T* x, int dty
   } else if (path == PATH_ANY) {
     hipLaunchKernelGGL((lp_any_kernel<T>), dim3(uh_grid(rows, UH_GRID_WAVES)), dim3(256), 0, s, a, x);
   } else if (const auto [parts, len] = lp_cut(a.v, rows, dtype); parts > 1) {
-    RowStat* ps = (RowStat*)ws;
-    uint64_t* pt = (uint64_t*)((char*)ws + (size_t)rows * parts * 16);
+    const int keep = lp_keep(a.top);
+    LpPart* ps = (LpPart*)ws;
+    uint64_t* pt = (uint64_t*)(ps + (size_t)rows * parts);
     const dim3 grid((unsigned)rows, (unsigned)parts);
 #define UH_GO(NV)                                                                                            \
   do {                                                                                                       \
-    if (a.top) hipLaunchKernelGGL((lp_part_kernel<T, NV, true>), grid, dim3(256), 0, s, a, x, parts, len, ps, pt); \
-    else hipLaunchKernelGGL((lp_part_kernel<T, NV, false>), grid, dim3(256), 0, s, a, x, parts, len, ps, pt);      \
+    if (a.top) hipLaunchKernelGGL((lp_part_kernel<T, NV, true>), grid, dim3(256), 0, s, a, x, parts, len, keep, ps, pt); \
+    else hipLaunchKernelGGL((lp_part_kernel<T, NV, false>), grid, dim3(256), 0, s, a, x, parts, len, keep, ps, pt);      \
   } while (0)
     if (len <= 256 * E) UH_GO(1); else if (len <= 256 * 4 * E) UH_GO(4); else if (len <= 256 * 8 * E) UH_GO(8); else UH_GO(16);
 #undef UH_GO
-    hipLaunchKernelGGL((lp_join_kernel<T>), dim3((unsigned)rows), dim3(64), (size_t)parts * a.top * 8, s, a, x, parts, ps, pt);
+    hipLaunchKernelGGL((lp_join_kernel<T>), dim3((unsigned)rows), dim3(256), ((size_t)parts * keep + 2) * 8, s, a, x, parts, keep, ps, pt);
   } else {
     const dim3 blocks(uh_grid(rows, UH_GRID_WAVES)), quads(uh_grid((rows + 3) / 4, UH_GRID_WAVES));
 #define UH_GO(G, NV)                                                                                            \

@@ -291,11 +291,19 @@ template <typename T, int G, int NV> struct RowRegs {
   __device__ __forceinline__ float get(int r, int j) const {
     if constexpr (sizeof(T) == 4) return __uint_as_float(w[r][j]);
     else if constexpr (std_is_half()) {
-      typedef __attribute__((ext_vector_type(2))) _Float16 h2;
-      const h2 v = __builtin_bit_cast(h2, w[r][j >> 1]);
-      return (float)v[j & 1];
+      float v;                                             // the compiler would keep every upper half in a register of its own
+      if (j & 1) asm("v_cvt_f32_f16_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:WORD_1" : "=v"(v) : "v"(w[r][j >> 1]));
+      else asm("v_cvt_f32_f16 %0, %1" : "=v"(v) : "v"(w[r][j >> 1]));
+      return v;
     } else
       return __uint_as_float(j & 1 ? w[r][j >> 1] & 0xffff0000u : w[r][j >> 1] << 16);
+  }
+  // the same with an element that only the lane knows
+  __device__ __forceinline__ float pick(int r, int j) const {
+    const int i = sizeof(T) == 4 ? j : j >> 1;
+    const uint32_t lo = i & 1 ? w[r][1] : w[r][0], hi = i & 1 ? w[r][3] : w[r][2], u = i & 2 ? hi : lo;
+    if constexpr (sizeof(T) == 4) return __uint_as_float(u);
+    else return (float)__builtin_bit_cast(T, (uint16_t)(j & 1 ? u >> 16 : u));
   }
   __device__ __forceinline__ float lane_max(int n) const {
     float m = -INFINITY;
@@ -308,9 +316,8 @@ template <typename T, int G, int NV> struct RowRegs {
       }
     return m;
   }
-  // s and (ENT) t of a lane's elements
-  template <bool ENT> __device__ __forceinline__ void lane_sums(const RowRef& ref, int n, float& s, float& t) const {
-    float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f;
+  // s and (ENT) t of a lane's elements, even and odd ones apart
+  template <bool ENT> __device__ __forceinline__ void add_sums(const RowRef& ref, int n, float& s0, float& s1, float& t0, float& t1) const {
 #pragma unroll
     for (int r = 0; r < NV; ++r)
       if (r * G * E < n) {
@@ -323,6 +330,10 @@ template <typename T, int G, int NV> struct RowRegs {
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+  }
+  template <bool ENT> __device__ __forceinline__ void lane_sums(const RowRef& ref, int n, float& s, float& t) const {
+    float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f;
+    add_sums<ENT>(ref, n, s0, s1, t0, t1);
     s = s0 + s1, t = t0 + t1;
   }
   // f(x) of every element to out[0 .. n)
@@ -348,9 +359,17 @@ template <typename T, int G, int NV> struct RowRegs {
           for (int j = 0; j < E; ++j)
             if (n - E + j >= e) out[n - E + j] = (T)f(get(r, j));
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
   }
 };
+
+// Inside a loop over rows: keeps the compiler from carrying every vector's place in a row from turn to turn (two registers
+// a vector, which cost a third of the waves).
+__device__ __forceinline__ int renew(int lane) {
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
 
 // statistics of one row by G lanes of a workgroup (any strides, element by element)
 template <typename T, int G> __device__ RowStat strided_row_stat(const T* __restrict__ x, int C, long long sc, float c2, int lane,
@@ -371,39 +390,35 @@ template <typename T, int G> __device__ RowStat strided_row_stat(const T* __rest
 }
 
 // ---- the largest of a row ---------------------------------------------------------------------------------------------------
-// Keys of rows of up to 64 classes held by a lane: 16-bit logits and their class fit 32 bits.
-template <typename T> struct SmallKey {
-  typedef uint32_t K;
-  __device__ __forceinline__ static K make(float x, int c) {
-    uint32_t b;
-    if constexpr (__is_same(T, f16)) b = __builtin_bit_cast(uint16_t, (f16)(x + 0.f));
-    else b = __float_as_uint(x + 0.f) >> 16;
-    b = b & 0x8000u ? b ^ 0xffffu : b | 0x8000u;
-    return x > -INFINITY ? (b << 16) | (0xffffu - (uint32_t)c) : 0u;
-  }
-  __device__ __forceinline__ static int cls(K k) { return 0xffff - (int)(k & 0xffffu); }
-  __device__ __forceinline__ static float val(K k) {
-    uint32_t b = k >> 16;
-    b = b & 0x8000u ? b & 0x7fffu : b ^ 0xffffu;
-    if constexpr (__is_same(T, f16)) return (float)__builtin_bit_cast(f16, (uint16_t)b);
-    else return __uint_as_float(b << 16);
-  }
-};
-template <> struct SmallKey<float> {
-  typedef uint64_t K;
-  __device__ __forceinline__ static K make(float x, int c) { return rank_key(x, c); }
-  __device__ __forceinline__ static int cls(K k) { return key_class(k); }
-  __device__ __forceinline__ static float val(K k) { return key_value(k); }
-};
-// keeps the N largest keys of a lane, falling
-template <typename K, int N> __device__ __forceinline__ void list_insert(K (&l)[N], K k) {
+// A lane's N largest so far, falling, with their classes (-1: none).  Classes come in rising order, so that a strict
+// comparison keeps the lowest of equal ones; x = -inf and NaN never enter.  A value's new place takes the middle of its own,
+// its left neighbour's and x: one instruction for the value, a comparison and two selections for the class.
+template <int N> struct TopList {
+  float v[N];
+  int c[N];
+  __device__ __forceinline__ TopList() {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const K hi = l[i] > k ? l[i] : k;
-    k = l[i] > k ? k : l[i];
-    l[i] = hi;
+    for (int i = 0; i < N; ++i) v[i] = -INFINITY, c[i] = -1;
   }
-}
+  __device__ __forceinline__ void insert(float x, int cls) {
+#pragma unroll
+    for (int i = N - 1; i > 0; --i) {
+      const bool above = x > v[i - 1], here = x > v[i];
+      c[i] = above ? c[i - 1] : here ? cls : c[i];
+      v[i] = above ? v[i - 1] : here ? x : v[i];
+    }
+    const bool first = x > v[0];
+    c[0] = first ? cls : c[0];
+    v[0] = first ? x : v[0];
+  }
+  __device__ __forceinline__ void pop() {
+#pragma unroll
+    for (int i = 0; i + 1 < N; ++i) v[i] = v[i + 1], c[i] = c[i + 1];
+    v[N - 1] = -INFINITY, c[N - 1] = -1;
+  }
+};
+// x if it comes behind (v, c) in the order of the alternatives, else -inf
+__device__ __forceinline__ float behind(float x, int cls, float v, int c) { return x < v || (x == v && cls > c) ? x : -INFINITY; }
 
 __device__ __forceinline__ int ballot_count(bool p) { return __popcll(__ballot(p)); }
 
@@ -423,62 +438,77 @@ template <int NK> __device__ __forceinline__ uint32_t wave_kth(const uint32_t (&
   return low;
 }
 
-// one wave: emit(rank, key) of the k largest of n different keys in LDS, emit(rank, 0) for the places left over.  More than
-// 128 keys are first cut down to the k by a search over the bits of the k-th largest.
-template <typename F> __device__ __forceinline__ void wave_select(uint64_t* list, int n, int k, F emit) {
+// One wave cuts a list of n > k different keys in LDS down to its k largest, in any order: a search over the bits of the
+// k-th largest, then the keys move to the front (a step reads its 64 places before it writes, and no further than it has read).
+__device__ __forceinline__ void wave_cut(uint64_t* list, int n, int k) {
   const int lane = threadIdx.x & 63;
-  if (n > 128 && n > k) {
-    uint64_t low = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-      const uint64_t test = low | (1ull << bit);
-      int c = 0;
-      for (int i = 0; i < n; i += 64) c += ballot_count(i + lane < n && list[i + lane] >= test);
-      if (c >= k) {
-        low = test;
-        if (c == k) break;
-      }
+  uint64_t low = 0;
+  for (int bit = 63; bit >= 0; --bit) {
+    const uint64_t test = low | (1ull << bit);
+    int c = 0;
+    for (int i = 0; i < n; i += 64) c += ballot_count(i + lane < n && list[i + lane] >= test);
+    if (c >= k) {
+      low = test;
+      if (c == k) break;
     }
-    // the k keys move to the front: a step reads its 64 places before it writes, and writes no further than it has read
-    int at = 0;
-    for (int i = 0; i < n; i += 64) {
-      const uint64_t mine = i + lane < n ? list[i + lane] : 0;
-      const bool in = mine >= low && mine != 0;
-      const uint64_t who = __ballot(in);
-      __builtin_amdgcn_wave_barrier();
-      if (in) list[at + __popcll(who & ((1ull << lane) - 1))] = mine;
-      __builtin_amdgcn_wave_barrier();
-      at += __popcll(who);
+  }
+  int at = 0;
+  for (int i = 0; i < n; i += 64) {
+    const uint64_t mine = i + lane < n ? list[i + lane] : 0;
+    const uint64_t who = __ballot(mine >= low && mine != 0);
+    __builtin_amdgcn_wave_barrier();
+    if (mine >= low && mine != 0) list[at + __popcll(who & ((1ull << lane) - 1))] = mine;
+    __builtin_amdgcn_wave_barrier();
+    at += __popcll(who);
+  }
+}
+// G lanes: emit(rank, key) of the k largest of n different keys in LDS (16-byte aligned, one place to spare), emit(rank, 0) for
+// the places left over.  A key's rank is the number of larger ones: up to two keys a lane are compared with all; more than that
+// are cut down first.  Ends with the list still being read: the caller's next write to it needs a barrier before.
+template <int G, typename F> __device__ __forceinline__ void group_rank(uint64_t* list, int n, int lane, int k, F emit) {
+  if (n > 2 * G && n > k) {
+    if (lane < 64) wave_cut(list, n, k);
+    n = k;
+    __syncthreads();
+  }
+  if (lane == 0) list[n] = 0;                                // pairs of keys are read
+  __syncthreads();
+  typedef __attribute__((ext_vector_type(2))) unsigned long long Pair;
+  const Pair* pairs = reinterpret_cast<const Pair*>(list);
+  for (int i = lane; i < n; i += 2 * G) {
+    const bool two = i + G < n;
+    const uint64_t a = list[i], b = two ? list[i + G] : ~0ull;
+    int ra = 0, rb = 0;
+#pragma unroll 4
+    for (int j = 0; j < (n + 1) / 2; ++j) {
+      const Pair p = pairs[j];
+      ra += (p.x > a) + (p.y > a);
+      rb += (p.x > b) + (p.y > b);
     }
-    n = at;
+    if (ra < k) emit(ra, a);
+    if (two && rb < k) emit(rb, b);
   }
-  for (int i = lane; i < n; i += 64) {
-    const uint64_t mine = list[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += list[j] > mine;
-    if (rank < k) emit(rank, mine);
-  }
-  for (int i = n + lane; i < k; i += 64) emit(i, 0ull);
+  for (int i = n + lane; i < k; i += G) emit(i, 0ull);
 }
 
 // The k largest of a row in registers.  The k-th largest of the lanes' own maxima bounds the k-th largest element from
-// below (each of k lanes holds one at least as large): the few elements at or above it go to a list in LDS, which one wave
-// ranks.  Rows whose many equal values overflow the list take the largest k times over instead.  All G lanes call; the
-// list may be used again after the next barrier of the workgroup.
+// below (each of k lanes holds one at least as large): the few elements at or above it go to a list in LDS.
 template <int G> struct TopBuf {
   static constexpr int CAP = G > 64 ? 2048 : 512;
-  uint64_t list[CAP];
+  alignas(16) uint64_t list[CAP + 2];
   float lane_max[G > 64 ? G : 1];
   uint32_t low;
   int count;
 };
-template <typename T, int G, int NV, typename F>
-__device__ __forceinline__ void group_top(RowRegs<T, G, NV>& x, const T* __restrict__ row, int n, int lane, int c0, int k, float lane_max, TopBuf<G>& b,
-                                          typename Red<G>::Buf& red, F emit) {
+// Fills b.list and returns how many there are (more than CAP: the list is of no use); low: their bound's order32 (0: none).
+// All G lanes call; the list stays until the next call.
+template <typename T, int G, int NV>
+__device__ __forceinline__ int group_candidates(RowRegs<T, G, NV>& x, int n, int lane, int c0, int k,
+                                                float lane_max, TopBuf<G>& b, uint32_t& low) {
   constexpr int E = RowRegs<T, G, NV>::E;
   const uint32_t mine = lane_max > -INFINITY ? order32(lane_max) : 0u;
   __syncthreads();
   if (lane == 0) b.count = 0;
-  uint32_t low;
   if constexpr (G == 64) {
     const uint32_t key[1] = {mine};
     low = wave_kth<1>(key, k);
@@ -499,7 +529,7 @@ __device__ __forceinline__ void group_top(RowRegs<T, G, NV>& x, const T* __restr
     low = b.low;
   }
   __syncthreads();
-  // lanes that hold one look for it again; its few hits are read once more from memory (a register cannot be indexed)
+  // lanes that hold one look for it again, and pick their few hits out of the vector's registers
   const float cut = low ? unorder32(low) : -3.402823466e38f;
   x.fresh();
   if (mine != 0 && mine >= low) {
@@ -511,20 +541,20 @@ __device__ __forceinline__ void group_top(RowRegs<T, G, NV>& x, const T* __restr
         for (int j = 0; j < E; ++j) hits |= x.get(r, j) >= cut ? 1u << j : 0u;
         const int e = RowRegs<T, G, NV>::first(r, lane, n);
         while (hits) {
-          const int c = e + __ffs(hits) - 1;
+          const int j = __ffs(hits) - 1;
           hits &= hits - 1;
           const int at = atomicAdd(&b.count, 1);
-          if (at < TopBuf<G>::CAP) b.list[at] = rank_key(ld(row + c), c0 + c);
+          if (at < TopBuf<G>::CAP) b.list[at] = rank_key(x.pick(r, j), c0 + e + j);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
   }
   __syncthreads();
-  const int found = b.count;
-  if (found <= TopBuf<G>::CAP) {
-    if (lane < 64) wave_select(b.list, found, k, emit);
-    return;
-  }
+  return b.count;
+}
+// rows whose many equal values overflow the list: the largest k times over
+template <typename T, int G, typename F>
+__device__ __forceinline__ void group_rounds(const T* __restrict__ row, int n, int lane, int c0, int k, typename Red<G>::Buf& red, F emit) {
   uint64_t last = ~0ull;
   for (int i = 0; i < k; ++i) {
     uint64_t best = 0;
@@ -629,7 +659,7 @@ static inline ClassPath uh_class_path(const RowView& v, const RowView* vo, long 
 }
 
 // A row is cut when it is longer than the 64 KB a workgroup of 256 holds in registers, or when there are too few rows to give
-// every CU two workgroups; a part is then at least 2048 classes (8 a lane).  At most 64 parts: a wave joins them, one a lane.
+// every CU two workgroups; a part is then about 2048 classes (8 a lane) or more.  At most 64 parts: a wave joins them, one a lane.
 // Parts are multiples of 64 classes, the last one what is left (at least one class; its loads may reach back into the part
 // before it).
 struct RowCut { int parts, len; };
@@ -642,7 +672,7 @@ static inline RowCut uh_row_cut(long long rows, int C, int dtype) {
   long long parts = (C + most - 1) / most;
   if (rows * parts < 512) {
     long long want = (512 + rows - 1) / rows;
-    if (want > C / 2048) want = C / 2048;
+    if (want > (C + 2047) / 2048) want = (C + 2047) / 2048;
     if (want > 64) want = 64;
     if (want > parts) parts = want;
   }

@@ -9,6 +9,7 @@
 // Sums over rows: every workgroup adds the rows it takes in 64 bits, one kernel adds the workgroups' sums, all in an order
 // that the sizes alone decide.
 #include "class_rows.h"
+#include <stdlib.h>
 
 struct DsArgs {
   RowView v, vo;
@@ -44,7 +45,7 @@ __device__ __forceinline__ float slot_term(float t, float val, float vm, float l
   return t > 0.f ? t * ((scaled(val, vm, temperature) - ln_sv) - (scaled(x, m, temperature) - ln_s)) : t == t ? 0.f : NAN;
 }
 
-// ---- a row by G lanes: the slots in LDS ----------------------------------------------------------------------------------------
+// ---- a row by 16 lanes, or by any group with any strides: the slots in LDS -------------------------------------------------------
 // The teacher's softmax of a row's slots into t_of / c_of [K].  Returns the sum of t (1, 0 without a filled slot, NaN).
 struct Teacher { float vm, ln_sv, sum; };
 template <int G> __device__ __forceinline__ Teacher group_teacher(const DsArgs& a, long long r, int lane, bool off, float* t_of, int* c_of,
@@ -87,207 +88,407 @@ template <typename T, int G> __device__ __forceinline__ float group_kl(const DsA
 }
 // classes the teacher names, written again after the dense part: p minus what all slots of that class hold
 template <typename T, int G> __device__ __forceinline__ void group_fix(const DsArgs& a, const T* __restrict__ row, T* __restrict__ out, int lane,
-                                                                       int c0, int n, float sum_t, float coef, const RowRef& ref, float inv_s,
-                                                                       const float* t_of, const int* c_of) {
+                                                                       float sum_t, float coef, const RowRef& ref, float inv_s, const float* t_of,
+                                                                       const int* c_of) {
   for (int k = lane; k < a.K; k += G) {
-    const int c = c_of[k] - c0;
-    if (c < 0 || c >= n || c_of[k] >= a.v.C) continue;
+    const int c = c_of[k];
+    if (c < 0 || c >= a.v.C) continue;
     float mine = 0.f;
-    for (int j = 0; j < a.K; ++j) mine += c_of[j] == c_of[k] ? t_of[j] : 0.f;
+    for (int j = 0; j < a.K; ++j) mine += c_of[j] == c ? t_of[j] : 0.f;
     st(out + c * a.vo.sc, coef * (sum_t * (ex2(ref.z(ld(row + c * a.v.sc))) * inv_s) - mine));
   }
 }
 
-// loss (LOSS) and gradient (GRAD) of rows whose classes lie side by side, the row in registers
-template <typename T, int G, int NV, bool GRAD>
-__global__ __launch_bounds__(G > 64 ? G : 64) void ds_group_kernel(DsArgs a, const T* __restrict__ x, T* __restrict__ dx) {
-  constexpr int RPB = G > 64 ? 1 : 64 / G;
+// MODE 0: loss, 1: gradient with statistics given, 2: both.  Four rows of 16 lanes a wave.
+template <typename T, int NV, int MODE>
+__global__ __launch_bounds__(64) void ds_quad_kernel(DsArgs a, const T* __restrict__ x, T* __restrict__ dx) {
   extern __shared__ __align__(16) char lds[];
-  __shared__ typename Red<G>::Buf red;
-  const int lane = threadIdx.x % G, sub = threadIdx.x / G, C = a.v.C;
+  Red<16>::Buf red;
+  const int sub = threadIdx.x / 16, C = a.v.C;
   float* t_of = reinterpret_cast<float*>(lds) + sub * a.K;
-  int* c_of = reinterpret_cast<int*>(lds) + (RPB + sub) * a.K;
-  const long long blocks = (a.rows + RPB - 1) / RPB;
+  int* c_of = reinterpret_cast<int*>(lds) + (4 + sub) * a.K;
+  const long long blocks = (a.rows + 3) / 4;
   double total = 0.0;
   for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const long long r = b * RPB + sub;
+    const int lane = renew(threadIdx.x % 16);
+    const long long r = b * 4 + sub;
     const bool there = r < a.rows;
     const float w = there ? a.weight_of(r) : 0.f;
     const bool off = w == 0.f;
     const T* row = x + (there ? a.v.base(r) : 0);
-    RowRegs<T, G, NV> reg;
-    if (off && RPB == 1) {
-      if (GRAD) reg.map_store(dx + a.vo.base(r), C, lane, [](float) { return 0.f; });
-      if (a.stats && lane == 0) { a.stats[2 * r] = 0.f; a.stats[2 * r + 1] = 0.f; }
-      continue;
-    }
+    RowRegs<T, 16, NV> reg;
     if (!off) reg.load(row, C, lane);
-    if (RPB == 1) __syncthreads();                         // the slots of the row before are read no more
-    const Teacher q = group_teacher<G>(a, r, lane, off, t_of, c_of, red);
-    RowStat s;
-    s.m = Red<G>::max_(off ? -INFINITY : reg.lane_max(C), red);
-    if (s.m == -INFINITY) s.m = 0.f;
-    const RowRef ref(s.m, a.c2);
-    reg.fresh();
-    reg.template lane_sums<false>(ref, C, s.s, s.t);
-    s.s = Red<G>::sum_(s.s, red);
-    const float kl = group_kl<T, G>(a, r, row, lane, q, s, t_of, c_of, red);
-    if (lane == 0 && !off) {
-      if (q.sum != 0.f) total += (double)w * a.temperature * a.temperature * kl;
-      if (a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
+    const Teacher q = group_teacher<16>(a, r, lane, off, t_of, c_of, red);
+    RowStat s{0.f, 0.f, 0.f};
+    if constexpr (MODE == 1) {
+      if (!off) s.m = a.stats[2 * r], s.s = a.stats[2 * r + 1];
+    } else {
+      s.m = group_max<16>(off ? -INFINITY : reg.lane_max(C));
+      if (s.m == -INFINITY) s.m = 0.f;
+      reg.fresh();
+      reg.template lane_sums<false>(RowRef(s.m, a.c2), C, s.s, s.t);
+      s.s = group_sum<16>(s.s);
+      const float kl = group_kl<T, 16>(a, r, row, lane, q, s, t_of, c_of, red);
+      if (lane == 0 && there) {
+        if (!off && q.sum != 0.f) total += (double)w * a.temperature * a.temperature * kl;
+        if (a.stats) { a.stats[2 * r] = off ? 0.f : s.m; a.stats[2 * r + 1] = off ? 0.f : s.s; }
+      }
     }
-    if constexpr (GRAD) {
+    if constexpr (MODE != 0) {
       if (there) {
         T* out = dx + a.vo.base(r);
+        const RowRef ref(s.m, a.c2);
         const float inv_s = s.s == 0.f ? 0.f : 1.f / s.s, co = a.coef(w), dense = co * q.sum * inv_s;
         reg.fresh();
         if (off || q.sum == 0.f) reg.map_store(out, C, lane, [](float) { return 0.f; });
         else {
           reg.map_store(out, C, lane, [&](float v) { return dense * ex2(ref.z(v)); });
-          if (G > 64) __syncthreads();                     // another wave may have written the class
-          group_fix<T, G>(a, row, out, lane, 0, C, q.sum, co, ref, inv_s, t_of, c_of);
+          group_fix<T, 16>(a, row, out, lane, q.sum, co, ref, inv_s, t_of, c_of);
         }
       }
     }
   }
-  if (RPB > 1) {
+  if constexpr (MODE != 1) {
     total += __shfl_xor(total, 16, 64);
     total += __shfl_xor(total, 32, 64);
-  }
-  if (threadIdx.x == 0) a.partial[blockIdx.x] = total;
-}
-
-// gradient alone, statistics given; a workgroup takes one part of a row
-template <typename T, int G, int NV>
-__global__ __launch_bounds__(G > 64 ? G : 64) void ds_bwd_group_kernel(DsArgs a, const T* __restrict__ x, T* __restrict__ dx, int part_len) {
-  constexpr int RPB = G > 64 ? 1 : 64 / G;
-  extern __shared__ __align__(16) char lds[];
-  __shared__ typename Red<G>::Buf red;
-  const int lane = threadIdx.x % G, sub = threadIdx.x / G, c0 = blockIdx.y * part_len;
-  const int n = min(part_len, a.v.C - c0);
-  float* t_of = reinterpret_cast<float*>(lds) + sub * a.K;
-  int* c_of = reinterpret_cast<int*>(lds) + (RPB + sub) * a.K;
-  const long long blocks = (a.rows + RPB - 1) / RPB;
-  for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const long long r = b * RPB + sub;
-    const bool there = r < a.rows;
-    const float w = there ? a.weight_of(r) : 0.f;
-    const bool off = w == 0.f;
-    RowRegs<T, G, NV> reg;
-    const T* row = x + (there ? a.v.base(r) : 0) + c0;
-    T* out = dx + (there ? a.vo.base(r) : 0) + c0;
-    if (off && RPB == 1) {
-      reg.map_store(out, n, lane, [](float) { return 0.f; });
-      continue;
-    }
-    if (!off) reg.load(row, n, lane);
-    if (RPB == 1) __syncthreads();
-    const Teacher q = group_teacher<G>(a, r, lane, off, t_of, c_of, red);
-    if (!there) continue;
-    if (off || q.sum == 0.f) {
-      reg.map_store(out, n, lane, [](float) { return 0.f; });
-      continue;
-    }
-    const float m = a.stats[2 * r], s = a.stats[2 * r + 1];
-    const RowRef ref(m, a.c2);
-    const float inv_s = s == 0.f ? 0.f : 1.f / s, co = a.coef(w), dense = co * q.sum * inv_s;
-    reg.map_store(out, n, lane, [&](float v) { return dense * ex2(ref.z(v)); });
-    if (G > 64) __syncthreads();                           // another wave may have written the class
-    group_fix<T, G>(a, row, out, lane, c0, n, q.sum, co, ref, inv_s, t_of, c_of);
+    if (threadIdx.x == 0) a.partial[blockIdx.x] = total;
   }
 }
 
-// ---- long rows, or few of them: statistics by parts, joined by a wave that adds the row's loss ------------------------------------
-template <typename T, int NV>
-__global__ __launch_bounds__(256) void ds_part_kernel(DsArgs a, const T* __restrict__ x, int parts, int part_len, RowStat* __restrict__ part_stat) {
-  __shared__ Red<256>::Buf red;
-  const long long r = blockIdx.x;
-  const int part = blockIdx.y, c0 = part * part_len, lane = threadIdx.x;
-  if (a.weight_of(r) == 0.f) return;
-  const int n = min(part_len, a.v.C - c0);
-  RowRegs<T, 256, NV> reg;
-  reg.load(x + a.v.base(r) + c0, n, lane);
-  RowStat s;
-  s.m = Red<256>::max_(reg.lane_max(n), red);
-  if (s.m == -INFINITY) s.m = 0.f;
-  reg.fresh();
-  reg.template lane_sums<false>(RowRef(s.m, a.c2), n, s.s, s.t);
-  s.t = 0.f;
-  s.s = Red<256>::sum_(s.s, red);
-  if (lane == 0) part_stat[r * parts + part] = s;
-}
-template <typename T>
-__global__ __launch_bounds__(64) void ds_join_kernel(DsArgs a, const T* __restrict__ x, int parts, const RowStat* __restrict__ part_stat) {
+// ---- a row by one wave or by workgroups of 256: one wave holds the slots in its registers ------------------------------------------
+// slot 64 q + lane of the row.  They are asked for before the row itself, so that their softmax is done while the row is on
+// its way (a wave's loads come back in order).
+struct SlotWave {
+  float val[4], t[4], mine[4];          // mine: what all slots of the same class hold
+  int cls[4];
+  float vm, ln_sv, sum;
+
+  __device__ __forceinline__ void load(const DsArgs& a, long long r, int lane) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      val[q] = -INFINITY, cls[q] = -1;
+      if (q * 64 < a.K && q * 64 + lane < a.K) a.slot(r, q * 64 + lane, val[q], cls[q]);
+    }
+  }
+  // t_of, c_of: K + 3 places, 16-byte aligned
+  __device__ __forceinline__ void softmax(const DsArgs& a, int lane, float* t_of, int* c_of, bool classes) {
+    float best = -INFINITY, sv = 0.f, bad = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q * 64 < a.K) {
+        best = fmaxf(best, val[q]);
+        if (val[q] != val[q] || cls[q] >= a.v.C) bad = 1.f;
+      }
+    best = group_max<64>(best);
+    vm = best == -INFINITY ? 0.f : best;
+    const RowRef ref(vm, a.c2);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      t[q] = q * 64 < a.K ? ex2(ref.z(val[q])) : 0.f;
+      sv += t[q];
+    }
+    sv = group_sum<64>(sv);
+    const bool wrong = __any(bad != 0.f);
+    const float inv = wrong ? NAN : sv == 0.f ? 0.f : 1.f / sv;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) t[q] *= inv;
+    ln_sv = ref.ln_s(vm, sv);
+    sum = wrong || !(sv >= 0.f) ? NAN : sv == 0.f ? 0.f : 1.f;
+    if (!classes) return;
+    const int K4 = (a.K + 3) / 4;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q * 64 < a.K && q * 64 + lane < 4 * K4) {
+        t_of[q * 64 + lane] = t[q];
+        c_of[q * 64 + lane] = cls[q];
+      }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) mine[q] = 0.f;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+    for (int j = 0; j < K4; ++j) {
+      const int4 c4 = reinterpret_cast<const int4*>(c_of)[j];
+      const float4 t4 = reinterpret_cast<const float4*>(t_of)[j];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (q * 64 < a.K)
+          mine[q] += ((c4.x == cls[q] ? t4.x : 0.f) + (c4.y == cls[q] ? t4.y : 0.f)) + ((c4.z == cls[q] ? t4.z : 0.f) + (c4.w == cls[q] ? t4.w : 0.f));
+    }
+  }
+  // sum_k t_k (ln t_k - ln p[i_k]) in all lanes
+  template <typename T> __device__ __forceinline__ float kl(const DsArgs& a, const T* __restrict__ row, const RowStat& s) const {
+    const float ln_s = s.s == 0.f ? 0.f : RowRef(s.m, a.c2).ln_s(s.m, s.s);    // no class left: ln p = -inf
+    float part = 0.f;
+    if (!(sum == sum)) part = NAN;
+    else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (q * 64 < a.K && t[q] != 0.f) part += slot_term(t[q], val[q], vm, ln_sv, ld(row + cls[q]), s.m, ln_s, a.temperature);
+    }
+    return group_sum<64>(part);
+  }
+  // classes the teacher names between c0 and c0 + n, written again after the dense part
+  template <typename T> __device__ __forceinline__ void fix(const DsArgs& a, const T* __restrict__ row, T* __restrict__ out, int c0, int n,
+                                                            float coef, const RowRef& ref, float inv_s) const {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q * 64 < a.K) {
+        const int c = cls[q];
+        if (c >= c0 && c < c0 + n && c < a.v.C) st(out + c, coef * (sum * (ex2(ref.z(ld(row + c))) * inv_s) - mine[q]));
+      }
+  }
+};
+static inline size_t slot_lds(int K) { return (size_t)((K + 3) / 4 * 4) * 8; }
+
+// one wave a row
+template <typename T, int NV, int MODE>
+__global__ __launch_bounds__(64) void ds_wave_kernel(DsArgs a, const T* __restrict__ x, T* __restrict__ dx) {
   extern __shared__ __align__(16) char lds[];
+  const int C = a.v.C, K4 = (a.K + 3) / 4 * 4;
   float* t_of = reinterpret_cast<float*>(lds);
-  int* c_of = reinterpret_cast<int*>(lds) + a.K;
-  Red<64>::Buf red;
-  const int lane = threadIdx.x;
+  int* c_of = reinterpret_cast<int*>(lds) + K4;
   double total = 0.0;
   for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const int lane = renew(threadIdx.x);
     const float w = a.weight_of(r);
-    RowStat s{0.f, 0.f, 0.f};
-    if (w != 0.f) {
-      if (lane < parts) s = part_stat[r * parts + lane];
-      for (int o = 32; o > 0; o >>= 1) {
-        const RowStat u{__shfl_xor(s.m, o, 64), __shfl_xor(s.s, o, 64), 0.f};
-        s = lane & o ? join(u, s, a.c2) : join(s, u, a.c2);
-      }
-      const Teacher q = group_teacher<64>(a, r, lane, false, t_of, c_of, red);
-      const float kl = group_kl<T, 64>(a, r, x + a.v.base(r), lane, q, s, t_of, c_of, red);
-      if (q.sum != 0.f) total += (double)w * a.temperature * a.temperature * kl;
+    RowRegs<T, 64, NV> reg;
+    if (w == 0.f) {
+      if (MODE != 0) reg.map_store(dx + a.vo.base(r), C, lane, [](float) { return 0.f; });
+      if (MODE != 1 && a.stats && lane == 0) { a.stats[2 * r] = 0.f; a.stats[2 * r + 1] = 0.f; }
+      continue;
     }
-    if (lane == 0 && a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
+    const T* row = x + a.v.base(r);
+    SlotWave q;
+    q.load(a, r, lane);
+    reg.load(row, C, lane);
+    q.softmax(a, lane, t_of, c_of, MODE != 0);
+    RowStat s{0.f, 0.f, 0.f};
+    if constexpr (MODE == 1) {
+      s.m = a.stats[2 * r], s.s = a.stats[2 * r + 1];
+    } else {
+      s.m = group_max<64>(reg.lane_max(C));
+      if (s.m == -INFINITY) s.m = 0.f;
+      reg.fresh();
+      reg.template lane_sums<false>(RowRef(s.m, a.c2), C, s.s, s.t);
+      s.s = group_sum<64>(s.s);
+      const float kl = q.kl(a, row, s);
+      if (q.sum != 0.f) total += (double)w * a.temperature * a.temperature * kl;
+      if (lane == 0 && a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
+    }
+    if constexpr (MODE != 0) {
+      T* out = dx + a.vo.base(r);
+      const RowRef ref(s.m, a.c2);
+      const float inv_s = s.s == 0.f ? 0.f : 1.f / s.s, co = a.coef(w), dense = co * q.sum * inv_s;
+      reg.fresh();
+      if (q.sum == 0.f) reg.map_store(out, C, lane, [](float) { return 0.f; });
+      else {
+        reg.map_store(out, C, lane, [&](float v) { return dense * ex2(ref.z(v)); });
+        q.fix(a, row, out, 0, C, co, ref, inv_s);
+      }
+    }
   }
-  if (lane == 0) a.partial[blockIdx.x] = total;
+  if (MODE != 1 && threadIdx.x == 0) a.partial[blockIdx.x] = total;
+}
+
+// Long rows, or few: workgroups of 256 take a part of a row each.  The parts' (m, s) meet in memory, one 64-bit word a part
+// that is written and read whole, so that no fence is needed: every workgroup that needs the row's statistics (all of them for
+// a gradient, the first for the loss alone) waits for the other parts' words and keeps its own part in registers meanwhile: the
+// row is read once.  A wait ends after `spins` looks at the latest: what is still missing then the waiting wave works out
+// itself from the logits, operation for operation as the part's own workgroup does, so that no result depends on who did it and
+// no workgroup on another one's being scheduled.
+static constexpr unsigned long long UH_NO_WORD = ~0ull;          // m = s = a NaN that no arithmetic makes (0xffffffff)
+__global__ __launch_bounds__(256) void ds_words_kernel(unsigned long long* __restrict__ words, long long n) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) words[i] = UH_NO_WORD;
+}
+struct DsParts {
+  int parts, len, spins;
+  unsigned long long* words;
+};
+
+// statistics of a part as 256 lanes make them, by one wave
+template <typename T, int NV> __device__ __attribute__((noinline)) RowStat alone_part_stat(const T* __restrict__ p, int n, float c2) {
+  constexpr int E = 16 / sizeof(T);
+  const int lane = threadIdx.x & 63;
+  float m = -INFINITY;
+  for (int r = 0; r < NV; ++r)
+    for (int w = 0; w < 4; ++w) {
+      const int left = n - r * 256 * E;
+      if (left <= 0) continue;
+      RowRegs<T, 256, 1> v;
+      v.load(p + r * 256 * E, left, lane + 64 * w);
+      m = fmaxf(m, v.lane_max(left));
+    }
+  m = group_max<64>(m);
+  if (m == -INFINITY) m = 0.f;
+  const RowRef ref(m, c2);
+  float s = 0.f;
+  for (int w = 0; w < 4; ++w) {
+    float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f;
+    for (int r = 0; r < NV; ++r) {
+      const int left = n - r * 256 * E;
+      if (left <= 0) continue;
+      RowRegs<T, 256, 1> v;
+      v.load(p + r * 256 * E, left, lane + 64 * w);
+      v.template add_sums<false>(ref, left, s0, s1, t0, t1);
+    }
+    const float sw = group_sum<64>(s0 + s1);
+    s = w == 0 ? sw : s + sw;
+  }
+  return RowStat{m, s == s ? s : NAN, 0.f};
+}
+
+template <typename T, int NV, int MODE>
+__global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restrict__ x, T* __restrict__ dx, DsParts p) {
+  extern __shared__ __align__(16) char lds[];
+  __shared__ Red<256>::Buf red;
+  __shared__ float joined[3];                              // m, s of the row; sum of t
+  const int lane = threadIdx.x, K4 = (a.K + 3) / 4 * 4;
+  float* t_of = reinterpret_cast<float*>(lds);
+  int* c_of = reinterpret_cast<int*>(lds) + K4;
+  const long long r = blockIdx.y + (long long)blockIdx.z * 32768;
+  if (r >= a.rows) return;
+  const int part = blockIdx.x, c0 = part * p.len, n = min(p.len, a.v.C - c0);
+  const bool first = lane < 64;                            // the wave with the slots
+  const float w = a.weight_of(r);
+  T* out = MODE != 0 ? dx + a.vo.base(r) : nullptr;
+  RowRegs<T, 256, NV> reg;
+  if (w == 0.f) {
+    if (MODE != 0) reg.map_store(out + c0, n, lane, [](float) { return 0.f; });
+    if (MODE != 1 && part == 0 && lane == 0) {
+      a.partial[r] = 0.0;
+      if (a.stats) { a.stats[2 * r] = 0.f; a.stats[2 * r + 1] = 0.f; }
+    }
+    return;
+  }
+  const T* row = x + a.v.base(r);
+  SlotWave q;
+  const bool slots = first && (MODE != 0 || part == 0);
+  if (slots) q.load(a, r, lane);
+  reg.load(row + c0, n, lane);
+  if (slots) {
+    q.softmax(a, lane, t_of, c_of, MODE != 0);
+    if (lane == 0) joined[2] = q.sum;
+  }
+  RowStat s{0.f, 0.f, 0.f};
+  if constexpr (MODE == 1) {
+    s.m = a.stats[2 * r], s.s = a.stats[2 * r + 1];
+    __syncthreads();                                       // joined[2]
+  } else {
+    s.m = Red<256>::max_(reg.lane_max(n), red);
+    if (s.m == -INFINITY) s.m = 0.f;
+    reg.fresh();
+    reg.template lane_sums<false>(RowRef(s.m, a.c2), n, s.s, s.t);
+    s.s = Red<256>::sum_(s.s, red);
+    if (s.s != s.s) s.s = NAN;                             // never the bits of UH_NO_WORD
+    s.t = 0.f;
+    if (p.parts > 1) {
+      unsigned long long* words = p.words + r * p.parts;
+      if (lane == 0)
+        __hip_atomic_store(words + part, (unsigned long long)__float_as_uint(s.s) << 32 | __float_as_uint(s.m), __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+      if (MODE == 0 && part != 0) return;
+      if (first) {
+        unsigned long long word = lane == part ? (unsigned long long)__float_as_uint(s.s) << 32 | __float_as_uint(s.m) : UH_NO_WORD;
+        const bool other = lane < p.parts && lane != part;
+        for (int i = 0; i < p.spins; ++i) {
+          if (other && word == UH_NO_WORD) word = __hip_atomic_load(words + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          if (!__any(other && word == UH_NO_WORD)) break;
+          __builtin_amdgcn_s_sleep(2);
+        }
+        for (unsigned long long left = __ballot(other && word == UH_NO_WORD); left; left &= left - 1) {
+          const int who = __ffsll(left) - 1, at = who * p.len;
+          const RowStat u = alone_part_stat<T, NV>(row + at, min(p.len, a.v.C - at), a.c2);
+          if (lane == who) word = (unsigned long long)__float_as_uint(u.s) << 32 | __float_as_uint(u.m);
+        }
+        RowStat j{__uint_as_float((uint32_t)word), lane < p.parts ? __uint_as_float((uint32_t)(word >> 32)) : 0.f, 0.f};
+        if (lane >= p.parts) j.m = 0.f;
+        for (int o = 1; o < 64 && o < p.parts; o <<= 1) {
+          const RowStat u{__shfl_xor(j.m, o, 64), __shfl_xor(j.s, o, 64), 0.f};
+          j = lane & o ? join(u, j, a.c2) : join(j, u, a.c2);
+        }
+        if (lane == 0) joined[0] = j.m, joined[1] = j.s;
+      }
+      __syncthreads();
+      s.m = joined[0], s.s = joined[1];
+    }
+  }
+  const RowRef ref(s.m, a.c2);
+  const float sum_t = joined[2];
+  if constexpr (MODE != 0) {
+    const float inv_s = s.s == 0.f ? 0.f : 1.f / s.s, co = a.coef(w), dense = co * sum_t * inv_s;
+    reg.fresh();
+    if (sum_t == 0.f) reg.map_store(out + c0, n, lane, [](float) { return 0.f; });
+    else {
+      reg.map_store(out + c0, n, lane, [&](float v) { return dense * ex2(ref.z(v)); });
+      __syncthreads();                                     // another wave may have written the class
+      if (first) q.fix(a, row, out, c0, n, co, ref, inv_s);
+    }
+  }
+  if (MODE != 1 && part == 0 && first) {
+    const float kl = q.kl(a, row, s);
+    if (lane == 0) {
+      a.partial[r] = sum_t != 0.f ? (double)w * a.temperature * a.temperature * kl : 0.0;
+      if (a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
+    }
+  }
 }
 
 // ---- one thread per row ----------------------------------------------------------------------------------------------------------
-// The teacher's softmax of a thread's own row; the slots are read once for the maximum, once for the sum and once for use.
-struct ThreadTeacher {
+// The teacher's softmax of a thread's own row.  KS > 0: at most KS slots, read once and kept; KS = 0: any number, read once for
+// the maximum, once for the sum and again for every use.
+template <int KS> struct ThreadTeacher {
   float vm, ln_sv, inv, sum;
   RowRef ref;
-  __device__ __forceinline__ ThreadTeacher(const DsArgs& a, long long r, float w) : ref(0.f, a.c2) {
-    vm = -INFINITY;
-    bool bad = false;
-    float sv = 0.f;
-    if (w != 0.f) {
+  float val_[KS > 0 ? KS : 1];
+  int cls_[KS > 0 ? KS : 1];
+  template <typename F> __device__ __forceinline__ void each(const DsArgs& a, long long r, F f) const {
+    if constexpr (KS > 0) {
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        if (k < a.K) f(val_[k], cls_[k]);
+    } else {
       for (int k = 0; k < a.K; ++k) {
         float val;
         int cls;
         a.slot(r, k, val, cls);
-        bad |= val != val || cls >= a.v.C;
-        vm = fmaxf(vm, val);
-      }
-      if (vm == -INFINITY) vm = 0.f;
-      ref = RowRef(vm, a.c2);
-      for (int k = 0; k < a.K; ++k) {
-        float val;
-        int cls;
-        a.slot(r, k, val, cls);
-        sv += ex2(ref.z(val));
+        f(val, cls);
       }
     }
+  }
+  __device__ __forceinline__ ThreadTeacher(const DsArgs& a, long long r, float w) : ref(0.f, a.c2) {
+    float best = -INFINITY, sv = 0.f;
+    bool bad = false;
+    if (w != 0.f) {
+      if constexpr (KS > 0) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+          if (k < a.K) a.slot(r, k, val_[k], cls_[k]);
+      }
+      each(a, r, [&](float val, int cls) {
+        bad |= val != val || cls >= a.v.C;
+        best = fmaxf(best, val);
+      });
+      if (best == -INFINITY) best = 0.f;
+      ref = RowRef(best, a.c2);
+      each(a, r, [&](float val, int) { sv += ex2(ref.z(val)); });
+    }
+    vm = best;
     inv = bad ? NAN : sv == 0.f ? 0.f : 1.f / sv;
     ln_sv = w != 0.f ? ref.ln_s(vm, sv) : 0.f;
     sum = bad || !(sv >= 0.f) ? NAN : sv == 0.f ? 0.f : 1.f;
   }
-  __device__ __forceinline__ float t(const DsArgs& a, long long r, int k, float& val, int& cls) const {
-    a.slot(r, k, val, cls);
-    return ex2(ref.z(val)) * inv;
-  }
+  __device__ __forceinline__ float t(float val) const { return ex2(ref.z(val)) * inv; }
 };
-template <typename T> __device__ __forceinline__ float thread_kl(const DsArgs& a, long long r, const T* row, long long sc, const ThreadTeacher& q,
-                                                                 const RowStat& s) {
+template <typename T, int KS> __device__ __forceinline__ float thread_kl(const DsArgs& a, long long r, const T* row, long long sc,
+                                                                         const ThreadTeacher<KS>& q, const RowStat& s) {
   if (!(q.sum == q.sum)) return NAN;
   const float ln_s = s.s == 0.f ? 0.f : RowRef(s.m, a.c2).ln_s(s.m, s.s);      // no class left: ln p = -inf
   float kl = 0.f;
-  for (int k = 0; k < a.K; ++k) {
-    float val;
-    int cls;
-    const float t = q.t(a, r, k, val, cls);
+  q.each(a, r, [&](float val, int cls) {
+    const float t = q.t(val);
     if (t != 0.f) kl += slot_term(t, val, q.vm, q.ln_sv, ld(row + cls * sc), s.m, ln_s, a.temperature);
-  }
+  });
   return kl;
 }
 __device__ __forceinline__ double wave_total(double v) {
@@ -297,7 +498,7 @@ __device__ __forceinline__ double wave_total(double v) {
 
 // MODE 0: loss, 1: gradient with statistics given, 2: both.  Up to 64 classes; what the teacher holds of each class is added up
 // in LDS (tab), so that a class named twice costs nothing and every gradient is rounded once.
-template <typename T, int CREG, bool STAGED, int MODE>
+template <typename T, int CREG, bool STAGED, int MODE, int KS>
 __global__ __launch_bounds__(64) void ds_thread_kernel(DsArgs a, const T* __restrict__ x, T* __restrict__ dx, bool wide) {
   extern __shared__ __align__(16) char lds[];
   constexpr int E = 16 / sizeof(T);
@@ -321,13 +522,13 @@ __global__ __launch_bounds__(64) void ds_thread_kernel(DsArgs a, const T* __rest
     }
     const long long sc = STAGED ? 1 : a.v.sc;
     if (lane < here) {
-      const float w = a.weight_of(r);
-      const ThreadTeacher q(a, r, w);
       float v[CREG];
+      load_classes<T, CREG, STAGED>(v, row, sc, C, wide);  // on its way while the slots are
+      const float w = a.weight_of(r);
+      const ThreadTeacher<KS> q(a, r, w);
       const bool on = w != 0.f && q.sum != 0.f;
       RowStat s{0.f, 0.f, 0.f};
       if (on) {
-        load_classes<T, CREG, STAGED>(v, row, sc, C, wide);
         if (MODE == 1) s.m = a.stats[2 * r], s.s = a.stats[2 * r + 1];
         else s = thread_row_stat<CREG, false>(v, C, a.c2);
       }
@@ -344,12 +545,9 @@ __global__ __launch_bounds__(64) void ds_thread_kernel(DsArgs a, const T* __rest
           const RowRef ref(s.m, a.c2);
           const float inv_s = s.s == 0.f ? 0.f : 1.f / s.s, co = a.coef(w), scale_p = q.sum * inv_s;
           for (int c = 0; c < C; ++c) tab[c * 64 + lane] = 0.f;
-          for (int k = 0; k < a.K; ++k) {
-            float val;
-            int cls;
-            const float t = q.t(a, r, k, val, cls);
-            if (cls >= 0 && cls < C) tab[cls * 64 + lane] += t;
-          }
+          q.each(a, r, [&](float val, int cls) {
+            if (cls >= 0 && cls < C) tab[cls * 64 + lane] += q.t(val);
+          });
 #pragma unroll
           for (int c = 0; c < CREG; ++c)
             if (c < C) st(out + c * osc, co * (scale_p * ex2(ref.z(v[c])) - tab[c * 64 + lane]));
@@ -377,7 +575,7 @@ template <typename T, int MODE> __global__ __launch_bounds__(64) void ds_walk_ke
     if (r >= a.rows) continue;
     const T* row = x + a.v.base(r);
     const float w = a.weight_of(r);
-    const ThreadTeacher q(a, r, w);
+    const ThreadTeacher<0> q(a, r, w);
     const bool on = w != 0.f && q.sum != 0.f;
     RowStat s{0.f, 0.f, 0.f};
     if (on) {
@@ -403,13 +601,10 @@ template <typename T, int MODE> __global__ __launch_bounds__(64) void ds_walk_ke
       if (on)
         for (int k = 0; k < a.K; ++k) {
           float val, mine = 0.f;
-          int cls, other;
+          int cls;
           a.slot(r, k, val, cls);
           if (cls < 0 || cls >= C) continue;
-          for (int j = 0; j < a.K; ++j) {
-            const float t = q.t(a, r, j, val, other);
-            mine += other == cls ? t : 0.f;
-          }
+          q.each(a, r, [&](float v, int other) { mine += other == cls ? q.t(v) : 0.f; });
           st(out + cls * osc, co * (q.sum * (ex2(ref.z(ld(row + cls * sc))) * inv_s) - mine));
         }
     }
@@ -452,7 +647,7 @@ template <typename T, int MODE> __global__ __launch_bounds__(256) void ds_any_ke
       const float inv_s = s.s == 0.f ? 0.f : 1.f / s.s, co = a.coef(w), dense = co * q.sum * inv_s;
       for (int c = lane; c < C; c += 256) st(out + c * a.vo.sc, on ? dense * ex2(ref.z(ld(row + c * a.v.sc))) : 0.f);
       __syncthreads();
-      if (on) group_fix<T, 256>(a, row, out, lane, 0, C, q.sum, co, ref, inv_s, t_of, c_of);
+      if (on) group_fix<T, 256>(a, row, out, lane, q.sum, co, ref, inv_s, t_of, c_of);
     }
   }
   if (MODE != 1 && lane == 0) a.partial[blockIdx.x] = total;
@@ -502,20 +697,29 @@ static DsArgs ds_args(const uh_class_view* view, const uh_class_view* out, const
   return a;
 }
 
-// Workspace of a call: the workgroups' sums, then (rows that are cut) the rows' statistics and those of their parts.
+// How a call's rows are taken, and its workspace: partial sums (one a row where parts of rows are workgroups, else one a
+// workgroup), then the words of rows in parts.
 struct DsPlan {
   ClassPath path;
   RowCut cut;
-  size_t stats_at, parts_at, bytes;
+  bool parts;                     // rows by workgroups of 256
+  size_t words_at, bytes;
 };
 static DsPlan ds_plan(const RowView& v, const RowView* vo, long long rows, int dtype) {
   DsPlan p;
+  const int elem = uh_elem_bytes(dtype);
   p.path = uh_class_path(v, vo, rows);
-  p.cut = p.path == PATH_GROUP ? uh_row_cut(rows, v.C, dtype) : RowCut{1, v.C};
-  p.stats_at = UH_GRID_WAVES * sizeof(double);
-  p.parts_at = p.stats_at + (p.cut.parts > 1 ? ((size_t)rows * 8 + 15) / 16 * 16 : 0);
-  p.bytes = p.parts_at + (p.cut.parts > 1 ? (size_t)rows * p.cut.parts * sizeof(RowStat) : 0);
+  p.parts = p.path == PATH_GROUP && (long long)v.C * elem > 8192;
+  p.cut = p.parts ? uh_row_cut(rows, v.C, dtype) : RowCut{1, v.C};
+  const size_t sums = p.parts && rows > UH_GRID_WAVES ? rows : UH_GRID_WAVES;
+  p.words_at = (sums * sizeof(double) + 15) / 16 * 16;
+  p.bytes = p.words_at + (p.cut.parts > 1 ? (size_t)rows * p.cut.parts * 8 : 0);
   return p;
+}
+
+static int ds_spins() {
+  const char* e = getenv("UNET_AMD_DISTILL_SPINS");
+  return e ? atoi(e) : 1 << 14;
 }
 
 // MODE 0: loss, 1: gradient, 2: both; returns how many partial sums there are
@@ -527,56 +731,52 @@ template <typename T, int MODE> static int ds_launch(const DsArgs& a, const T* x
   if (p.path == PATH_STAGED || p.path == PATH_APART) {
     const bool staged = p.path == PATH_STAGED, wide = staged && (a.v.so * sizeof(T)) % 16 == 0;
     const size_t lds = (MODE ? (size_t)C * 64 * 4 : 0) + (staged ? ((64 * a.v.so + E - 1) / E * E + (MODE ? 64 * C : 0)) * sizeof(T) : 0);
-#define UH_GO2(R, ST) hipLaunchKernelGGL((ds_thread_kernel<T, R, ST, MODE>), dim3(waves), dim3(64), lds, s, a, x, dx, wide)
-#define UH_GO(ST) do { if (C <= 8) UH_GO2(8, ST); else if (C <= 16) UH_GO2(16, ST); else if (C <= 32) UH_GO2(32, ST); else UH_GO2(64, ST); } while (0)
+#define UH_GO3(R, ST, KS) hipLaunchKernelGGL((ds_thread_kernel<T, R, ST, MODE, KS>), dim3(waves), dim3(64), lds, s, a, x, dx, wide)
+#define UH_GO2(R, ST) do { if (a.K <= 4) UH_GO3(R, ST, 4); else UH_GO3(R, ST, 0); } while (0)
+#define UH_GO(ST) do { if (C <= 16) UH_GO2(16, ST); else if (C <= 32) UH_GO2(32, ST); else UH_GO2(64, ST); } while (0)
     if (staged) UH_GO(true); else UH_GO(false);
 #undef UH_GO
 #undef UH_GO2
+#undef UH_GO3
     return (int)waves;
   }
-  const size_t slots = (size_t)a.K * 8;
   if (p.path == PATH_WALK) {
     hipLaunchKernelGGL((ds_walk_kernel<T, MODE>), dim3(waves), dim3(64), 0, s, a, x, dx);
     return (int)waves;
   }
   if (p.path == PATH_ANY) {
-    hipLaunchKernelGGL((ds_any_kernel<T, MODE>), dim3(blocks), dim3(256), slots, s, a, x, dx);
+    hipLaunchKernelGGL((ds_any_kernel<T, MODE>), dim3(blocks), dim3(256), (size_t)a.K * 8, s, a, x, dx);
     return (int)blocks;
   }
-  if constexpr (MODE == 1) {
-    if (C <= 16 * 4 * E)
-      hipLaunchKernelGGL((ds_bwd_group_kernel<T, 16, 4>), dim3(uh_grid((rows + 3) / 4, UH_GRID_WAVES)), dim3(64), 4 * slots, s, a, x, dx, C);
-    else if (C <= 64 * 4 * E)
-      hipLaunchKernelGGL((ds_bwd_group_kernel<T, 64, 4>), dim3(blocks), dim3(64), slots, s, a, x, dx, C);
-    else {
-      const RowCut cut = uh_cut_parts(C, (C + 256 * 4 * E - 1) / (256 * 4 * E));
-      hipLaunchKernelGGL((ds_bwd_group_kernel<T, 256, 4>), dim3(blocks, (unsigned)cut.parts), dim3(256), slots, s, a, x, dx, cut.len);
-    }
-    return 0;
-  } else {
-    if (p.cut.parts > 1) {
-      RowStat* ps = (RowStat*)(ws + p.parts_at);
-      DsArgs j = a;
-      if (!j.stats) j.stats = (float*)(ws + p.stats_at);
-      const dim3 grid((unsigned)rows, (unsigned)p.cut.parts);
-#define UH_GO(NV) hipLaunchKernelGGL((ds_part_kernel<T, NV>), grid, dim3(256), 0, s, j, x, p.cut.parts, p.cut.len, ps)
-      if (p.cut.len <= 256 * E) UH_GO(1); else if (p.cut.len <= 256 * 4 * E) UH_GO(4); else if (p.cut.len <= 256 * 8 * E) UH_GO(8); else UH_GO(16);
-#undef UH_GO
-      hipLaunchKernelGGL((ds_join_kernel<T>), dim3(blocks), dim3(64), slots, s, j, x, p.cut.parts, ps);
-      if (MODE == 2) ds_launch<T, 1>(j, x, dx, p, ws, s);
-      return (int)blocks;
-    }
-#define UH_GO(G, NV, GR, R) hipLaunchKernelGGL((ds_group_kernel<T, G, NV, MODE == 2>), dim3(GR), dim3(G > 64 ? G : 64), R * slots, s, a, x, dx)
+  if (C <= 16 * 4 * E) {
     const unsigned quads = uh_grid((rows + 3) / 4, UH_GRID_WAVES);
-    if (C <= 16 * 4 * E) { UH_GO(16, 4, quads, 4); return (int)quads; }
-    if (C <= 64 * 4 * E) UH_GO(64, 4, blocks, 1);
-    else if (C <= 64 * 8 * E) UH_GO(64, 8, blocks, 1);
-    else if (C <= 256 * 4 * E) UH_GO(256, 4, blocks, 1);
-    else if (C <= 256 * 8 * E) UH_GO(256, 8, blocks, 1);
-    else UH_GO(256, 16, blocks, 1);
-#undef UH_GO
+    hipLaunchKernelGGL((ds_quad_kernel<T, 4, MODE>), dim3(quads), dim3(64), (size_t)a.K * 32, s, a, x, dx);
+    return (int)quads;
+  }
+  if (!p.parts) {
+    if (C <= 64 * 4 * E) hipLaunchKernelGGL((ds_wave_kernel<T, 4, MODE>), dim3(blocks), dim3(64), slot_lds(a.K), s, a, x, dx);
+    else hipLaunchKernelGGL((ds_wave_kernel<T, 8, MODE>), dim3(blocks), dim3(64), slot_lds(a.K), s, a, x, dx);
     return (int)blocks;
   }
+  // a gradient alone needs no joining: its parts are as long as suits a copy
+  const RowCut cut = MODE == 1 ? uh_cut_parts(C, (C + 256 * 4 * E - 1) / (256 * 4 * E)) : p.cut;
+  DsParts q{cut.parts, cut.len, 0, nullptr};
+  if (MODE != 1 && cut.parts > 1) {
+    q.spins = ds_spins();
+    q.words = (unsigned long long*)(ws + p.words_at);
+    const long long n = rows * cut.parts;
+    hipLaunchKernelGGL(ds_words_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, q.words, n);
+  }
+  const dim3 grid((unsigned)cut.parts, (unsigned)(rows < 32768 ? rows : 32768), (unsigned)((rows + 32767) / 32768));
+#define UH_GO(NV) hipLaunchKernelGGL((ds_rows_kernel<T, NV, MODE>), grid, dim3(256), slot_lds(a.K), s, a, x, dx, q)
+  if (cut.len <= 256 * E) UH_GO(1);
+  else if (MODE == 1 || cut.len <= 256 * 4 * E) UH_GO(4);
+  else if constexpr (MODE != 1) {
+    if (cut.len <= 256 * 8 * E) UH_GO(8);
+    else UH_GO(16);
+  }
+#undef UH_GO
+  return (int)rows;
 }
 
 template <int MODE> static int ds_dispatch(const DsArgs& a, int dtype, const void* x, void* dx, const DsPlan& p, void* ws, hipStream_t s) {
