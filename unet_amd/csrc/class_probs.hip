@@ -44,13 +44,12 @@ struct LpArgs {
   }
 };
 
-// ---- rows whose classes lie side by side: G lanes a row, the row in registers -------------------------------------------------
-// LIST > 0 (G = 16): up to LIST alternatives from the lanes' own falling lists; TOP (G >= 64): any number.
+// ---- rows whose classes lie side by side: 16 or 64 lanes a row, the row in registers -------------------------------------------
+// LIST > 0 (G = 16): up to LIST alternatives from the lanes' own falling lists; TOP (G = 64): any number.
 template <typename T, int G, int NV, int LIST, bool TOP>
-__global__ __launch_bounds__(G > 64 ? G : 64) void lp_group_kernel(LpArgs a, const T* __restrict__ x) {
-  constexpr int RPB = G > 64 ? 1 : 64 / G;
-  constexpr int E = RowRegs<T, G, NV>::E;
-  __shared__ typename Red<G>::Buf red;
+__global__ __launch_bounds__(64) void lp_group_kernel(LpArgs a, const T* __restrict__ x) {
+  constexpr int RPB = 64 / G, E = RowRegs<T, G, NV>::E;
+  typename Red<G>::Buf red;
   const int C = a.v.C;
   const long long blocks = (a.rows + RPB - 1) / RPB;
   for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
@@ -64,18 +63,17 @@ __global__ __launch_bounds__(G > 64 ? G : 64) void lp_group_kernel(LpArgs a, con
         if (lane == 0) a.write_ignored(r);
         for (int k = lane; k < a.top; k += G) a.write_top(r, k, 0.f, -1, 0.f, 0.f, 0.f);
       }
-      if (RPB == 1) continue;                              // the whole workgroup's row
+      if (RPB == 1) continue;                              // the whole wave's row
     }
     RowRegs<T, G, NV> reg;
     const T* row = x + (there ? a.v.base(r) : 0);
     if (!off) reg.load(row, C, lane);
-    const float lm = off ? -INFINITY : reg.lane_max(C);
+    float vmax[TOP ? NV : 1];
+    const float lm = off ? -INFINITY : reg.template lane_max<TOP ? NV : 0>(C, vmax);
     RowStat s;
-    s.m = Red<G>::max_(lm, red);
+    s.m = group_max<G>(lm);
     if (s.m == -INFINITY) s.m = 0.f;
-    reg.fresh();
-    reg.template lane_sums<true>(RowRef(s.m, a.c2), C, s.s, s.t);
-    Red<G>::sum2(s.s, s.t, red);
+    group_sums<T, G, NV>(reg, RowRef(s.m, a.c2), C, s, red);
     float ln_s = 0.f;
     if (!off) {
       if (lane == 0) ln_s = a.write_row(r, l, a.is_class(l) ? ld(row + l) : 0.f, s);
@@ -105,19 +103,19 @@ __global__ __launch_bounds__(G > 64 ? G : 64) void lp_group_kernel(LpArgs a, con
     if constexpr (TOP) {
       __shared__ TopBuf<G> tb;
       uint32_t low;
-      const int found = group_candidates<T, G, NV>(reg, C, lane, 0, a.top, lm, tb, low);
+      const int found = group_candidates<T, G, NV>(reg, C, lane, 0, a.top, lm, vmax, tb, low);
       const auto emit = [&](int k, uint64_t key) {
         a.write_top(r, k, key_value(key), key ? key_class(key) : -1, s.m, ln_s, s.s);
       };
-      if (found <= TopBuf<G>::CAP) group_rank<G>(tb.list, found, lane, a.top, emit);
+      if (found <= TopBuf<G>::CAP) group_rank<G>(tb.list, found, lane, a.top, &tb.left, emit);
       else group_rounds<T, G>(row, C, lane, 0, a.top, red, emit);
     }
   }
 }
 
-// ---- long rows, or few of them: a workgroup takes one part of a row, a wave joins a row's parts ---------------------------------
-// A part leaves its statistics and candidates for the alternatives in any order: all it found, or the `top` largest where
-// that is more than `keep`.  low: order32 of a value that at least `top` of the part's elements reach (0: there are fewer).
+// ---- longer rows: a workgroup of 256 takes a row, or one part of it ----------------------------------------------------------------
+// A part leaves its statistics and candidates for the alternatives: all it found, in any order, or the `top` largest where that
+// is more than `keep`.  low: order32 of a value that at least `top` of the part's elements reach (0: there are fewer).
 struct LpPart {
   float m, s, t;
   uint32_t low;
@@ -126,41 +124,56 @@ struct LpPart {
 static inline int lp_keep(int top) { return top ? top + 32 : 0; }
 
 template <typename T, int NV, bool TOP>
-__global__ __launch_bounds__(256) void lp_part_kernel(LpArgs a, const T* __restrict__ x, int parts, int part_len, int keep,
+__global__ __launch_bounds__(256) void lp_rows_kernel(LpArgs a, const T* __restrict__ x, int parts, int part_len, int keep,
                                                       LpPart* __restrict__ part, uint64_t* __restrict__ part_top) {
   __shared__ Red<256>::Buf red;
-  const long long r = blockIdx.x, me = r * parts + blockIdx.y;
-  const int c0 = blockIdx.y * part_len, lane = threadIdx.x;
-  if (a.ignored(a.label(r))) return;                       // the join does not look at the parts of such a row
+  const long long r = blockIdx.y + (long long)blockIdx.z * 32768, me = r * parts + blockIdx.x;
+  if (r >= a.rows) return;
+  const int c0 = blockIdx.x * part_len, lane = threadIdx.x;
+  const long long l = a.label(r);
+  if (a.ignored(l)) {                                      // (the join does not look at the parts of such a row)
+    if (parts == 1) {
+      if (lane == 0) a.write_ignored(r);
+      for (int k = lane; k < a.top; k += 256) a.write_top(r, k, 0.f, -1, 0.f, 0.f, 0.f);
+    }
+    return;
+  }
   const int n = min(part_len, a.v.C - c0);
   RowRegs<T, 256, NV> reg;
   const T* row = x + a.v.base(r) + c0;
-  reg.load(row, n, lane);
-  const float lm = reg.lane_max(n);
+  reg.template load<true>(row, n, lane);
+  float vmax[TOP ? NV : 1];
+  const float lm = reg.template lane_max<TOP ? NV : 0>(n, vmax);
   RowStat s;
   s.m = Red<256>::max_(lm, red);
   if (s.m == -INFINITY) s.m = 0.f;
-  reg.fresh();
-  reg.template lane_sums<true>(RowRef(s.m, a.c2), n, s.s, s.t);
-  Red<256>::sum2(s.s, s.t, red);
+  group_sums<T, 256, NV>(reg, RowRef(s.m, a.c2), n, s, red);
+  float ln_s = 0.f;
+  if (parts == 1) {
+    ln_s = RowRef(s.m, a.c2).ln_s(s.m, s.s);
+    if (lane == 0) a.write_row(r, l, a.is_class(l) ? ld(row + l) : 0.f, s);
+  }
   uint32_t low = 0;
   int found = 0;
   if constexpr (TOP) {
     __shared__ TopBuf<256> tb;
+    found = group_candidates<T, 256, NV>(reg, n, lane, c0, a.top, lm, vmax, tb, low);
     uint64_t* out = part_top + me * keep;
-    found = group_candidates<T, 256, NV>(reg, n, lane, c0, a.top, lm, tb, low);
-    if (found > TopBuf<256>::CAP) {
-      group_rounds<T, 256>(row, n, lane, c0, a.top, red, [&](int k, uint64_t key) { out[k] = key; });
+    const auto emit = [&](int k, uint64_t key) {
+      if (parts == 1) a.write_top(r, k, key_value(key), key ? key_class(key) : -1, s.m, ln_s, s.s);
+      else out[k] = key;
+    };
+    if (found > TopBuf<256>::CAP) {                        // too many equal values
+      group_rounds<T, 256>(row, n, lane, c0, a.top, red, emit);
       found = a.top;                                       // those left over are 0: below any bound
+    } else if (parts == 1 || found > keep) {
+      group_rank<256>(tb.list, found, lane, a.top, &tb.left, emit);
+      found = a.top;
     } else {
-      if (found > keep) {
-        if (lane < 64) wave_cut(tb.list, found, a.top);
-        found = a.top;
-        __syncthreads();
-      }
       for (int i = lane; i < found; i += 256) out[i] = tb.list[i];
     }
   }
+  if (parts == 1) return;
   if (lane == 0) {
     LpPart& p = part[me];
     p.m = s.m, p.s = s.s, p.t = s.t, p.low = low, p.count = found;
@@ -171,7 +184,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void lp_join_kernel(LpArgs a, const T* __restrict__ x, int parts, int keep, const LpPart* __restrict__ part,
                                                       const uint64_t* __restrict__ part_top) {
   extern __shared__ __align__(16) uint64_t keys[];         // parts * keep of them and two to spare
-  __shared__ int count;
+  __shared__ int count, left;
   const long long r = blockIdx.x;
   const int lane = threadIdx.x & 63;
   const long long l = a.label(r);
@@ -208,7 +221,7 @@ __global__ __launch_bounds__(256) void lp_join_kernel(LpArgs a, const T* __restr
     }
   }
   __syncthreads();
-  group_rank<256>(keys, count, threadIdx.x, a.top, [&](int k, uint64_t key) {
+  group_rank<256>(keys, count, threadIdx.x, a.top, &left, [&](int k, uint64_t key) {
     a.write_top(r, k, key_value(key), key ? key_class(key) : -1, s.m, ln_s, s.s);
   });
 }
@@ -390,7 +403,7 @@ __global__ __launch_bounds__(G > 64 ? G : 64) void lp_bwd_group_kernel(LpBwd k, 
       continue;
     }
     const T* row = x + k.v.base(r) + c0;
-    reg.load(row, n, lane);
+    reg.template load<true>(row, n, lane);
     const RowRef ref(q.m, k.c2);
     reg.map_store(out, n, lane, [&](float v) { return q.of(ref, v); });
     // the label's class once more, by the lane that has just written it
@@ -469,15 +482,18 @@ template <typename T> __global__ __launch_bounds__(256) void lp_bwd_any_kernel(L
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------------
-// how the rows of a forward call are cut (one part: they are not)
-static RowCut lp_cut(const RowView& v, long long rows, int dtype) {
-  return uh_class_path(v, nullptr, rows) == PATH_GROUP ? uh_row_cut(rows, v.C, dtype) : RowCut{1, v.C};
+// How the rows of a forward call are cut (one part: they are not).  With alternatives parts are 32 KB: looking for candidates
+// is what a workgroup's other waves wait for, and 68 registers leave room for seven workgroups a CU, 108 for four (1024 rows
+// of 131072 bf16 classes, top 64: see the table of measurements).  Without, 64 KB.
+static RowCut lp_cut(const RowView& v, long long rows, int dtype, int top) {
+  if (uh_class_path(v, nullptr, rows) != PATH_GROUP || (long long)v.C * uh_elem_bytes(dtype) <= 8192) return RowCut{1, v.C};
+  return uh_row_cut(rows, v.C, dtype, top ? 32768 : 65536);
 }
 
 extern "C" size_t uh_label_log_probs_workspace(const uh_class_view* view, int top) {
   if (uh_check_view(view, "label_log_probs_workspace") != UH_OK || top < 0 || top > UH_TOP_MAX) return 0;
   const long long rows = view->outer * view->inner;
-  const int parts = lp_cut(uh_row_view(view), rows, view->dtype).parts;
+  const int parts = lp_cut(uh_row_view(view), rows, view->dtype, top).parts;
   if (parts == 1) return 0;
   return (size_t)rows * parts * (sizeof(LpPart) + 8 * (size_t)lp_keep(top));
 }
@@ -505,36 +521,35 @@ template <typename T> static void lp_launch(const LpArgs& a, const T* x, int dty
     else hipLaunchKernelGGL((lp_walk_kernel<T, 8>), grid, dim3(64), 0, s, a, x);
   } else if (path == PATH_ANY) {
     hipLaunchKernelGGL((lp_any_kernel<T>), dim3(uh_grid(rows, UH_GRID_WAVES)), dim3(256), 0, s, a, x);
-  } else if (const auto [parts, len] = lp_cut(a.v, rows, dtype); parts > 1) {
+  } else if (C <= 16 * 4 * E && a.top <= 8) {
+    const dim3 quads(uh_grid((rows + 3) / 4, UH_GRID_WAVES));
+    if (a.top == 0) hipLaunchKernelGGL((lp_group_kernel<T, 16, 4, 0, false>), quads, dim3(64), 0, s, a, x);
+    else if (a.top <= 4) hipLaunchKernelGGL((lp_group_kernel<T, 16, 4, 4, false>), quads, dim3(64), 0, s, a, x);
+    else hipLaunchKernelGGL((lp_group_kernel<T, 16, 4, 8, false>), quads, dim3(64), 0, s, a, x);
+  } else if (C <= 64 * 8 * E) {
+    const dim3 blocks(uh_grid(rows, UH_GRID_WAVES));
+#define UH_GO(NV)                                                                                               \
+  do {                                                                                                          \
+    if (a.top) hipLaunchKernelGGL((lp_group_kernel<T, 64, NV, 0, true>), blocks, dim3(64), 0, s, a, x);         \
+    else hipLaunchKernelGGL((lp_group_kernel<T, 64, NV, 0, false>), blocks, dim3(64), 0, s, a, x);              \
+  } while (0)
+    if (C <= 64 * 4 * E) UH_GO(4); else UH_GO(8);
+#undef UH_GO
+  } else {
+    const RowCut cut = lp_cut(a.v, rows, dtype, a.top);
     const int keep = lp_keep(a.top);
     LpPart* ps = (LpPart*)ws;
-    uint64_t* pt = (uint64_t*)(ps + (size_t)rows * parts);
-    const dim3 grid((unsigned)rows, (unsigned)parts);
-#define UH_GO(NV)                                                                                            \
-  do {                                                                                                       \
-    if (a.top) hipLaunchKernelGGL((lp_part_kernel<T, NV, true>), grid, dim3(256), 0, s, a, x, parts, len, keep, ps, pt); \
-    else hipLaunchKernelGGL((lp_part_kernel<T, NV, false>), grid, dim3(256), 0, s, a, x, parts, len, keep, ps, pt);      \
-  } while (0)
-    if (len <= 256 * E) UH_GO(1); else if (len <= 256 * 4 * E) UH_GO(4); else if (len <= 256 * 8 * E) UH_GO(8); else UH_GO(16);
+    uint64_t* pt = (uint64_t*)(ps + (size_t)rows * cut.parts);
+    const dim3 grid((unsigned)cut.parts, (unsigned)(rows < 32768 ? rows : 32768), (unsigned)((rows + 32767) / 32768));
+#define UH_GO(NV, TOP) hipLaunchKernelGGL((lp_rows_kernel<T, NV, TOP>), grid, dim3(256), 0, s, a, x, cut.parts, cut.len, keep, ps, pt)
+#define UH_GO2(NV) do { if (a.top) UH_GO(NV, true); else UH_GO(NV, false); } while (0)
+    // (32 MB and more of fp32 in 64 parts would be more than 32 KB: only then a part with alternatives is 64 KB)
+    if (cut.len <= 256 * E) UH_GO2(1); else if (cut.len <= 256 * 4 * E) UH_GO2(4); else if (cut.len <= 256 * 8 * E) UH_GO2(8); else UH_GO2(16);
+#undef UH_GO2
 #undef UH_GO
-    hipLaunchKernelGGL((lp_join_kernel<T>), dim3((unsigned)rows), dim3(256), ((size_t)parts * keep + 2) * 8, s, a, x, parts, keep, ps, pt);
-  } else {
-    const dim3 blocks(uh_grid(rows, UH_GRID_WAVES)), quads(uh_grid((rows + 3) / 4, UH_GRID_WAVES));
-#define UH_GO(G, NV)                                                                                            \
-  do {                                                                                                          \
-    if (a.top) hipLaunchKernelGGL((lp_group_kernel<T, G, NV, 0, true>), blocks, dim3(G), 0, s, a, x);           \
-    else hipLaunchKernelGGL((lp_group_kernel<T, G, NV, 0, false>), blocks, dim3(G), 0, s, a, x);                \
-  } while (0)
-    if (C <= 16 * 4 * E && a.top <= 8) {
-      if (a.top == 0) hipLaunchKernelGGL((lp_group_kernel<T, 16, 4, 0, false>), quads, dim3(64), 0, s, a, x);
-      else if (a.top <= 4) hipLaunchKernelGGL((lp_group_kernel<T, 16, 4, 4, false>), quads, dim3(64), 0, s, a, x);
-      else hipLaunchKernelGGL((lp_group_kernel<T, 16, 4, 8, false>), quads, dim3(64), 0, s, a, x);
-    } else if (C <= 64 * 4 * E) UH_GO(64, 4);
-    else if (C <= 64 * 8 * E) UH_GO(64, 8);
-    else if (C <= 256 * 4 * E) UH_GO(256, 4);
-    else if (C <= 256 * 8 * E) UH_GO(256, 8);
-    else UH_GO(256, 16);
-#undef UH_GO
+    if (cut.parts > 1)
+      hipLaunchKernelGGL((lp_join_kernel<T>), dim3((unsigned)rows), dim3(256), ((size_t)cut.parts * keep + 2) * 8, s, a, x, cut.parts,
+                         keep, ps, pt);
   }
 }
 

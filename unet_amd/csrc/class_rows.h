@@ -162,6 +162,10 @@ template <int G> __device__ __forceinline__ uint32_t group_max(uint32_t v) {
   return v;
 }
 
+// The wave of a workgroup that does what one wave does alone: another one from workgroup to workgroup, so that this work is
+// spread over the four SIMDs of a CU (a wave's number in its workgroup decides its SIMD).
+template <int G> __device__ __forceinline__ bool serial_wave() { return G <= 64 || (threadIdx.x >> 6) == ((blockIdx.x + blockIdx.y) & (G / 64 - 1)); }
+
 // LDS of the reductions over a workgroup of NW waves; nothing for groups inside a wave
 template <int NW> struct RedBuf {
   float m[NW], s[NW], t[NW];
@@ -231,6 +235,8 @@ __device__ __forceinline__ long long load_int(const void* p, int bytes, long lon
 // 16 bytes wherever an element may lie: rows of odd sizes start anywhere (the hardware takes element-aligned vectors)
 template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Loose16 { uint32_t w[4]; };
 
+template <typename T> using LooseVec = __attribute__((ext_vector_type(4), aligned(sizeof(T)))) uint32_t;
+
 template <typename T, int G, int NV> struct RowRegs {
   static constexpr int E = 16 / sizeof(T);
   static constexpr int CAP = G * NV * E;
@@ -247,15 +253,16 @@ template <typename T, int G, int NV> struct RowRegs {
     const int e = (r * G + lane) * E;
     return e + E <= n ? e : n - E;
   }
-  __device__ __forceinline__ void load(const T* __restrict__ p, int n, int lane) {
+  template <bool ONCE = false> __device__ __forceinline__ void load(const T* __restrict__ p, int n, int lane) {
 #pragma unroll
     for (int r = 0; r < NV; ++r)
       if (r * G * E < n) {
         const int e = (r * G + lane) * E;
         if (e < n) {
-          const Loose16<T> u = *reinterpret_cast<const Loose16<T>*>(p + first(r, lane, n));
+          const LooseVec<T>* q = reinterpret_cast<const LooseVec<T>*>(p + first(r, lane, n));
+          const LooseVec<T> u = ONCE ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[r][i] = u.w[i];
+          for (int i = 0; i < 4; ++i) w[r][i] = u[i];
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) w[r][i] = neg_inf();
@@ -298,42 +305,49 @@ template <typename T, int G, int NV> struct RowRegs {
     } else
       return __uint_as_float(j & 1 ? w[r][j >> 1] & 0xffff0000u : w[r][j >> 1] << 16);
   }
-  // the same with an element that only the lane knows
-  __device__ __forceinline__ float pick(int r, int j) const {
-    const int i = sizeof(T) == 4 ? j : j >> 1;
-    const uint32_t lo = i & 1 ? w[r][1] : w[r][0], hi = i & 1 ? w[r][3] : w[r][2], u = i & 2 ? hi : lo;
-    if constexpr (sizeof(T) == 4) return __uint_as_float(u);
-    else return (float)__builtin_bit_cast(T, (uint16_t)(j & 1 ? u >> 16 : u));
-  }
-  __device__ __forceinline__ float lane_max(int n) const {
+  // the largest element, and (NM = NV) that of every vector
+  template <int NM = 0> __device__ __forceinline__ float lane_max(int n, float* vmax = nullptr) const {
     float m = -INFINITY;
 #pragma unroll
     for (int r = 0; r < NV; ++r)
       if (r * G * E < n) {
+        if constexpr (NM > 0) {
+          float v = fmaxf(get(r, 0), get(r, 1));
 #pragma unroll
-        for (int j = 0; j < E; j += 2) m = max3(m, get(r, j), get(r, j + 1));
+          for (int j = 2; j < E; j += 2) v = max3(v, get(r, j), get(r, j + 1));
+          vmax[r] = v;
+          m = fmaxf(m, v);
+        } else {
+#pragma unroll
+          for (int j = 0; j < E; j += 2) m = max3(m, get(r, j), get(r, j + 1));
+        }
         __builtin_amdgcn_sched_barrier(0);                  // one vector at a time: unpacked ones would pile up
       }
     return m;
   }
-  // s and (ENT) t of a lane's elements, even and odd ones apart
-  template <bool ENT> __device__ __forceinline__ void add_sums(const RowRef& ref, int n, float& s0, float& s1, float& t0, float& t1) const {
+  // s and (ENT) t of a lane's elements, even and odd ones apart.  Without CLAMP a class of -inf makes t a NaN; the -inf that
+  // fill the row's last vectors do not.
+  template <bool ENT, bool CLAMP = false> __device__ __forceinline__ void add_sums(const RowRef& ref, int n, float& s0, float& s1, float& t0, float& t1) const {
 #pragma unroll
     for (int r = 0; r < NV; ++r)
       if (r * G * E < n) {
-#pragma unroll
-        for (int j = 0; j < E; j += 2) {
-          const float z0 = ref.z(get(r, j)), z1 = ref.z(get(r, j + 1));
-          const float e0 = ex2(z0), e1 = ex2(z1);
-          s0 += e0, s1 += e1;
-          if (ENT) t0 = fmaf(e0, fmaxf(z0, UH_ZMIN), t0), t1 = fmaf(e1, fmaxf(z1, UH_ZMIN), t1);
-        }
+        if (!ENT || CLAMP || (r + 1) * G * E <= n) add_vector<ENT, ENT && CLAMP>(r, ref, s0, s1, t0, t1);
+        else add_vector<ENT, ENT>(r, ref, s0, s1, t0, t1);
         __builtin_amdgcn_sched_barrier(0);
       }
   }
-  template <bool ENT> __device__ __forceinline__ void lane_sums(const RowRef& ref, int n, float& s, float& t) const {
+  template <bool ENT, bool CLAMP> __device__ __forceinline__ void add_vector(int r, const RowRef& ref, float& s0, float& s1, float& t0, float& t1) const {
+#pragma unroll
+    for (int j = 0; j < E; j += 2) {
+      const float z0 = ref.z(get(r, j)), z1 = ref.z(get(r, j + 1));
+      const float e0 = ex2(z0), e1 = ex2(z1);
+      s0 += e0, s1 += e1;
+      if (ENT) t0 = fmaf(e0, CLAMP ? fmaxf(z0, UH_ZMIN) : z0, t0), t1 = fmaf(e1, CLAMP ? fmaxf(z1, UH_ZMIN) : z1, t1);
+    }
+  }
+  template <bool ENT, bool CLAMP = false> __device__ __forceinline__ void lane_sums(const RowRef& ref, int n, float& s, float& t) const {
     float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f;
-    add_sums<ENT>(ref, n, s0, s1, t0, t1);
+    add_sums<ENT, CLAMP>(ref, n, s0, s1, t0, t1);
     s = s0 + s1, t = t0 + t1;
   }
   // f(x) of every element to out[0 .. n)
@@ -363,6 +377,23 @@ template <typename T, int G, int NV> struct RowRegs {
       }
   }
 };
+
+// s and t of a whole row.  The clamp of its exponents, one instruction of nine an element, is only for classes of -inf (0 times
+// -inf): rows that hold one are found by their NaN and summed again with it.
+template <typename T, int G, int NV>
+__device__ __forceinline__ void group_sums(RowRegs<T, G, NV>& x, const RowRef& ref, int n, RowStat& s, typename Red<G>::Buf& red) {
+  x.fresh();
+  x.template lane_sums<true>(ref, n, s.s, s.t);
+  Red<G>::sum2(s.s, s.t, red);
+  const bool again = s.t != s.t && s.s == s.s;
+  if (G >= 64 ? again : (bool)__any(again)) {
+    float s2, t2;
+    x.fresh();
+    x.template lane_sums<true, true>(ref, n, s2, t2);
+    Red<G>::sum2(s2, t2, red);
+    if (again) s.t = t2;
+  }
+}
 
 // Inside a loop over rows: keeps the compiler from carrying every vector's place in a row from turn to turn (two registers
 // a vector, which cost a third of the waves).
@@ -422,12 +453,22 @@ __device__ __forceinline__ float behind(float x, int cls, float v, int c) { retu
 
 __device__ __forceinline__ int ballot_count(bool p) { return __popcll(__ballot(p)); }
 
-// a lower bound of the k-th largest of a wave's NK keys a lane, with at least k keys at or above it; 0 if there are fewer
+// A lower bound of the k-th largest of a wave's NK keys a lane, with at least k keys at or above it; 0 if there are fewer than k
+// keys.  Bit by bit from the highest in which the keys differ down to the 16th: what the lower bits would exclude is a few
+// candidates more than k.
 template <int NK> __device__ __forceinline__ uint32_t wave_kth(const uint32_t (&key)[NK], int k) {
-  uint32_t low = 0;
-  for (int bit = 31; bit >= 0; --bit) {
+  uint32_t any = 0, all = ~0u;
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < NK; ++i) any |= key[i], all &= key[i], n += ballot_count(key[i] != 0);
+  if (n < k) return 0;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) any |= __shfl_xor(any, o, 64), all &= __shfl_xor(all, o, 64);
+  const uint32_t differ = any ^ all;
+  uint32_t low = differ ? all & ~((2u << (31 - __clz(differ))) - 1u) : all;
+  for (int bit = differ ? 31 - __clz(differ) : 0; bit >= 15; --bit) {
     const uint32_t test = low | (1u << bit);
-    int n = 0;
+    n = 0;
 #pragma unroll
     for (int i = 0; i < NK; ++i) n += ballot_count(key[i] >= test);
     if (n >= k) {
@@ -438,18 +479,36 @@ template <int NK> __device__ __forceinline__ uint32_t wave_kth(const uint32_t (&
   return low;
 }
 
-// One wave cuts a list of n > k different keys in LDS down to its k largest, in any order: a search over the bits of the
-// k-th largest, then the keys move to the front (a step reads its 64 places before it writes, and no further than it has read).
-__device__ __forceinline__ void wave_cut(uint64_t* list, int n, int k) {
+// One wave cuts a list of n > k different keys in LDS down to fewer, the k largest among them, and returns how many are left: a
+// search for the k-th largest, bit by bit; it ends above the keys' lower halves unless so many values are equal that the classes
+// have to decide.  The keys move to the front: a step reads its 64 places before it writes, and no further than it has read.
+__device__ __forceinline__ int wave_cut(uint64_t* list, int n, int k) {
   const int lane = threadIdx.x & 63;
   uint64_t low = 0;
-  for (int bit = 63; bit >= 0; --bit) {
-    const uint64_t test = low | (1ull << bit);
-    int c = 0;
-    for (int i = 0; i < n; i += 64) c += ballot_count(i + lane < n && list[i + lane] >= test);
-    if (c >= k) {
-      low = test;
-      if (c == k) break;
+  if (n <= 512) {
+    uint32_t key[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) key[i] = i * 64 + lane < n ? (uint32_t)(list[i * 64 + lane] >> 32) : 0u;
+    low = (uint64_t)wave_kth<8>(key, k) << 32;
+  } else if (n <= 1024) {
+    uint32_t key[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) key[i] = i * 64 + lane < n ? (uint32_t)(list[i * 64 + lane] >> 32) : 0u;
+    low = (uint64_t)wave_kth<16>(key, k) << 32;
+  } else {
+    int above = n;
+    for (int bit = 63; bit >= 0 && (bit >= 47 || above > 2 * k + 128); --bit) {
+      const uint64_t test = low | (1ull << bit);
+      int c = 0;
+      for (int i = lane; i - lane < n; i += 256) {
+#pragma unroll
+        for (int j = 0; j < 256; j += 64) c += ballot_count(i + j < n && list[i + j] >= test);
+      }
+      if (c >= k) {
+        low = test;
+        above = c;
+        if (c == k) break;
+      }
     }
   }
   int at = 0;
@@ -461,15 +520,20 @@ __device__ __forceinline__ void wave_cut(uint64_t* list, int n, int k) {
     __builtin_amdgcn_wave_barrier();
     at += __popcll(who);
   }
+  return at;
 }
 // G lanes: emit(rank, key) of the k largest of n different keys in LDS (16-byte aligned, one place to spare), emit(rank, 0) for
-// the places left over.  A key's rank is the number of larger ones: up to two keys a lane are compared with all; more than that
-// are cut down first.  Ends with the list still being read: the caller's next write to it needs a barrier before.
-template <int G, typename F> __device__ __forceinline__ void group_rank(uint64_t* list, int n, int lane, int k, F emit) {
-  if (n > 2 * G && n > k) {
-    if (lane < 64) wave_cut(list, n, k);
-    n = k;
+// the places left over.  A key's rank is the number of larger ones, so that the list is cut down first where it is long; of many
+// equal values a long one may be left: then all is compared with all.  count: a word of LDS.  Ends with the list still being
+// read: the caller's next write to it needs a barrier before.
+template <int G, typename F> __device__ __forceinline__ void group_rank(uint64_t* list, int n, int lane, int k, int* count, F emit) {
+  if (n > 128 && n > k) {
+    if (lane < 64) {
+      const int left = wave_cut(list, n, k);
+      if (lane == 0) *count = left;
+    }
     __syncthreads();
+    n = *count;
   }
   if (lane == 0) list[n] = 0;                                // pairs of keys are read
   __syncthreads();
@@ -494,57 +558,65 @@ template <int G, typename F> __device__ __forceinline__ void group_rank(uint64_t
 // The k largest of a row in registers.  The k-th largest of the lanes' own maxima bounds the k-th largest element from
 // below (each of k lanes holds one at least as large): the few elements at or above it go to a list in LDS.
 template <int G> struct TopBuf {
-  static constexpr int CAP = G > 64 ? 2048 : 512;
+  static constexpr int CAP = G > 64 ? 1024 : 512;
   alignas(16) uint64_t list[CAP + 2];
   float lane_max[G > 64 ? G : 1];
   uint32_t low;
-  int count;
+  int count, left;
 };
 // Fills b.list and returns how many there are (more than CAP: the list is of no use); low: their bound's order32 (0: none).
 // All G lanes call; the list stays until the next call.
 template <typename T, int G, int NV>
-__device__ __forceinline__ int group_candidates(RowRegs<T, G, NV>& x, int n, int lane, int c0, int k,
-                                                float lane_max, TopBuf<G>& b, uint32_t& low) {
+__device__ __forceinline__ int group_candidates(RowRegs<T, G, NV>& x, int n, int lane, int c0, int k, float lane_max, const float* vmax, TopBuf<G>& b,
+                                                uint32_t& low) {
   constexpr int E = RowRegs<T, G, NV>::E;
-  const uint32_t mine = lane_max > -INFINITY ? order32(lane_max) : 0u;
-  __syncthreads();
+  __syncthreads();                                           // the list of the row before is read no more
   if (lane == 0) b.count = 0;
+  const uint32_t mine = lane_max > -INFINITY ? order32(lane_max) : 0u;
   if constexpr (G == 64) {
     const uint32_t key[1] = {mine};
     low = wave_kth<1>(key, k);
   } else {
     b.lane_max[lane] = lane_max;
     __syncthreads();
-    if (lane < 64) {
+    if (serial_wave<G>()) {
       uint32_t key[G / 64];
 #pragma unroll
       for (int i = 0; i < G / 64; ++i) {
-        const float v = b.lane_max[lane + 64 * i];
+        const float v = b.lane_max[(lane & 63) + 64 * i];
         key[i] = v > -INFINITY ? order32(v) : 0u;
       }
       const uint32_t l = wave_kth<G / 64>(key, k);
-      if (lane == 0) b.low = l;
+      if ((lane & 63) == 0) b.low = l;
     }
     __syncthreads();
     low = b.low;
   }
-  __syncthreads();
-  // lanes that hold one look for it again, and pick their few hits out of the vector's registers
   const float cut = low ? unorder32(low) : -3.402823466e38f;
   x.fresh();
-  if (mine != 0 && mine >= low) {
+  if (__any(mine != 0 && mine >= low)) {                     // one look per vector; its few hits are placed by ballots
 #pragma unroll
     for (int r = 0; r < NV; ++r)
       if (r * G * E < n) {
-        uint32_t hits = 0;
+        if (!__any(vmax[r] >= cut)) continue;
+        unsigned long long hit[E], some = 0;
 #pragma unroll
-        for (int j = 0; j < E; ++j) hits |= x.get(r, j) >= cut ? 1u << j : 0u;
-        const int e = RowRegs<T, G, NV>::first(r, lane, n);
-        while (hits) {
-          const int j = __ffs(hits) - 1;
-          hits &= hits - 1;
-          const int at = atomicAdd(&b.count, 1);
-          if (at < TopBuf<G>::CAP) b.list[at] = rank_key(x.pick(r, j), c0 + e + j);
+        for (int j = 0; j < E; ++j) some |= hit[j] = __ballot(x.get(r, j) >= cut);
+        if (some) {
+          int total = 0, at = 0;
+#pragma unroll
+          for (int j = 0; j < E; ++j) total += __popcll(hit[j]);
+          if ((lane & 63) == 0) at = atomicAdd(&b.count, total);
+          at = __builtin_amdgcn_readfirstlane(at);
+          const int e = c0 + RowRegs<T, G, NV>::first(r, lane, n);
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (hit[j]) {
+              const float v = x.get(r, j);
+              const int to = at + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(hit[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hit[j], 0));
+              if (v >= cut && to < TopBuf<G>::CAP) b.list[to] = rank_key(v, e + j);
+              at += __popcll(hit[j]);
+            }
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -658,8 +730,8 @@ static inline ClassPath uh_class_path(const RowView& v, const RowView* vo, long 
   return rows >= 256 ? PATH_WALK : PATH_ANY;
 }
 
-// A row is cut when it is longer than the 64 KB a workgroup of 256 holds in registers, or when there are too few rows to give
-// every CU two workgroups; a part is then about 2048 classes (8 a lane) or more.  At most 64 parts: a wave joins them, one a lane.
+// A row is cut when it is longer than the `most` bytes that a workgroup of 256 is to hold in registers (at most 64 KB), or when
+// there are too few rows to give every CU two workgroups; a part is then about 2048 classes (8 a lane) or more.  At most 64 parts: a wave joins them, one a lane.
 // Parts are multiples of 64 classes, the last one what is left (at least one class; its loads may reach back into the part
 // before it).
 struct RowCut { int parts, len; };
@@ -667,14 +739,14 @@ static inline RowCut uh_cut_parts(int C, long long parts) {
   const int len = (int)(((C + parts - 1) / parts + 63) / 64 * 64);
   return RowCut{(C + len - 1) / len, len};
 }
-static inline RowCut uh_row_cut(long long rows, int C, int dtype) {
-  const int most = 65536 / uh_elem_bytes(dtype);
+static inline RowCut uh_row_cut(long long rows, int C, int dtype, int most_bytes) {
+  const int most = most_bytes / uh_elem_bytes(dtype);
   long long parts = (C + most - 1) / most;
   if (rows * parts < 512) {
     long long want = (512 + rows - 1) / rows;
     if (want > (C + 2047) / 2048) want = (C + 2047) / 2048;
-    if (want > 64) want = 64;
     if (want > parts) parts = want;
   }
+  if (parts > 64) parts = 64;
   return uh_cut_parts(C, parts);
 }

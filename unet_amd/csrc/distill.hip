@@ -159,7 +159,7 @@ __global__ __launch_bounds__(64) void ds_quad_kernel(DsArgs a, const T* __restri
 // slot 64 q + lane of the row.  They are asked for before the row itself, so that their softmax is done while the row is on
 // its way (a wave's loads come back in order).
 struct SlotWave {
-  float val[4], t[4], mine[4];          // mine: what all slots of the same class hold
+  float val[4], t[4], mine[4], xk[4];   // mine: what all slots of the same class hold; xk: the student's logit of the class
   int cls[4];
   float vm, ln_sv, sum;
 
@@ -170,8 +170,19 @@ struct SlotWave {
       if (q * 64 < a.K && q * 64 + lane < a.K) a.slot(r, q * 64 + lane, val[q], cls[q]);
     }
   }
-  // t_of, c_of: K + 3 places, 16-byte aligned
-  __device__ __forceinline__ void softmax(const DsArgs& a, int lane, float* t_of, int* c_of, bool classes) {
+  __device__ __forceinline__ bool inside(const DsArgs& a, int q, int c0, int n) const {
+    return cls[q] >= c0 && cls[q] < c0 + n && cls[q] < a.v.C;
+  }
+  // The slots' softmax, and the student's logits of their classes between c0 and c0 + n (in lines that the row's own loads,
+  // issued before, bring).  t_of, c_of: K + 3 places, 16-byte aligned.
+  template <typename T>
+  __device__ __forceinline__ void softmax(const DsArgs& a, const T* __restrict__ row, int c0, int n, int lane, float* t_of, int* c_of,
+                                          bool classes) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      xk[q] = 0.f;
+      if (q * 64 < a.K && inside(a, q, c0, n)) xk[q] = ld(row + cls[q]);
+    }
     float best = -INFINITY, sv = 0.f, bad = 0.f;
 #pragma unroll
     for (int q = 0; q < 4; ++q)
@@ -215,27 +226,24 @@ struct SlotWave {
           mine[q] += ((c4.x == cls[q] ? t4.x : 0.f) + (c4.y == cls[q] ? t4.y : 0.f)) + ((c4.z == cls[q] ? t4.z : 0.f) + (c4.w == cls[q] ? t4.w : 0.f));
     }
   }
-  // sum_k t_k (ln t_k - ln p[i_k]) in all lanes
-  template <typename T> __device__ __forceinline__ float kl(const DsArgs& a, const T* __restrict__ row, const RowStat& s) const {
+  // sum_k t_k (ln t_k - ln p[i_k]) over the classes between c0 and c0 + n, in all lanes
+  __device__ __forceinline__ float kl(const DsArgs& a, const RowStat& s, int c0, int n) const {
     const float ln_s = s.s == 0.f ? 0.f : RowRef(s.m, a.c2).ln_s(s.m, s.s);    // no class left: ln p = -inf
     float part = 0.f;
     if (!(sum == sum)) part = NAN;
     else {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        if (q * 64 < a.K && t[q] != 0.f) part += slot_term(t[q], val[q], vm, ln_sv, ld(row + cls[q]), s.m, ln_s, a.temperature);
+        if (q * 64 < a.K && t[q] != 0.f && inside(a, q, c0, n)) part += slot_term(t[q], val[q], vm, ln_sv, xk[q], s.m, ln_s, a.temperature);
     }
     return group_sum<64>(part);
   }
-  // classes the teacher names between c0 and c0 + n, written again after the dense part
-  template <typename T> __device__ __forceinline__ void fix(const DsArgs& a, const T* __restrict__ row, T* __restrict__ out, int c0, int n,
-                                                            float coef, const RowRef& ref, float inv_s) const {
+  // the classes the teacher names there, written again after the dense part
+  template <typename T> __device__ __forceinline__ void fix(const DsArgs& a, T* __restrict__ out, int c0, int n, float coef, const RowRef& ref,
+                                                            float inv_s) const {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      if (q * 64 < a.K) {
-        const int c = cls[q];
-        if (c >= c0 && c < c0 + n && c < a.v.C) st(out + c, coef * (sum * (ex2(ref.z(ld(row + c))) * inv_s) - mine[q]));
-      }
+      if (q * 64 < a.K && inside(a, q, c0, n)) st(out + cls[q], coef * (sum * (ex2(ref.z(xk[q])) * inv_s) - mine[q]));
   }
 };
 static inline size_t slot_lds(int K) { return (size_t)((K + 3) / 4 * 4) * 8; }
@@ -261,7 +269,7 @@ __global__ __launch_bounds__(64) void ds_wave_kernel(DsArgs a, const T* __restri
     SlotWave q;
     q.load(a, r, lane);
     reg.load(row, C, lane);
-    q.softmax(a, lane, t_of, c_of, MODE != 0);
+    q.softmax(a, row, 0, C, lane, t_of, c_of, MODE != 0);
     RowStat s{0.f, 0.f, 0.f};
     if constexpr (MODE == 1) {
       s.m = a.stats[2 * r], s.s = a.stats[2 * r + 1];
@@ -271,7 +279,7 @@ __global__ __launch_bounds__(64) void ds_wave_kernel(DsArgs a, const T* __restri
       reg.fresh();
       reg.template lane_sums<false>(RowRef(s.m, a.c2), C, s.s, s.t);
       s.s = group_sum<64>(s.s);
-      const float kl = q.kl(a, row, s);
+      const float kl = q.kl(a, s, 0, C);
       if (q.sum != 0.f) total += (double)w * a.temperature * a.temperature * kl;
       if (lane == 0 && a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
     }
@@ -283,7 +291,7 @@ __global__ __launch_bounds__(64) void ds_wave_kernel(DsArgs a, const T* __restri
       if (q.sum == 0.f) reg.map_store(out, C, lane, [](float) { return 0.f; });
       else {
         reg.map_store(out, C, lane, [&](float v) { return dense * ex2(ref.z(v)); });
-        q.fix(a, row, out, 0, C, co, ref, inv_s);
+        q.fix(a, out, 0, C, co, ref, inv_s);
       }
     }
   }
@@ -343,32 +351,34 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
   extern __shared__ __align__(16) char lds[];
   __shared__ Red<256>::Buf red;
   __shared__ float joined[3];                              // m, s of the row; sum of t
-  const int lane = threadIdx.x, K4 = (a.K + 3) / 4 * 4;
+  const int lane = threadIdx.x, wl = threadIdx.x & 63, K4 = (a.K + 3) / 4 * 4;
   float* t_of = reinterpret_cast<float*>(lds);
   int* c_of = reinterpret_cast<int*>(lds) + K4;
   const long long r = blockIdx.y + (long long)blockIdx.z * 32768;
   if (r >= a.rows) return;
   const int part = blockIdx.x, c0 = part * p.len, n = min(p.len, a.v.C - c0);
-  const bool first = lane < 64;                            // the wave with the slots
+  const bool first = serial_wave<256>();                   // the wave with the slots
   const float w = a.weight_of(r);
   T* out = MODE != 0 ? dx + a.vo.base(r) : nullptr;
   RowRegs<T, 256, NV> reg;
   if (w == 0.f) {
     if (MODE != 0) reg.map_store(out + c0, n, lane, [](float) { return 0.f; });
-    if (MODE != 1 && part == 0 && lane == 0) {
-      a.partial[r] = 0.0;
-      if (a.stats) { a.stats[2 * r] = 0.f; a.stats[2 * r + 1] = 0.f; }
+    if (MODE != 1 && lane == 0) {
+      if (MODE == 2 || part == 0) a.partial[MODE == 2 ? r * p.parts + part : r] = 0.0;
+      if (MODE == 0 && part == 0 && a.stats) { a.stats[2 * r] = 0.f; a.stats[2 * r + 1] = 0.f; }
     }
     return;
   }
   const T* row = x + a.v.base(r);
   SlotWave q;
   const bool slots = first && (MODE != 0 || part == 0);
-  if (slots) q.load(a, r, lane);
-  reg.load(row + c0, n, lane);
+  if (slots) q.load(a, r, wl);
+  reg.template load<MODE == 2>(row + c0, n, lane);
   if (slots) {
-    q.softmax(a, lane, t_of, c_of, MODE != 0);
-    if (lane == 0) joined[2] = q.sum;
+    // the loss alone is the first part's to work out; for a gradient every part has its classes' share of it
+    if (MODE == 0) q.softmax(a, row, 0, a.v.C, wl, t_of, c_of, false);
+    else q.softmax(a, row, c0, n, wl, t_of, c_of, true);
+    if (wl == 0) joined[2] = q.sum;
   }
   RowStat s{0.f, 0.f, 0.f};
   if constexpr (MODE == 1) {
@@ -389,25 +399,25 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
                            __HIP_MEMORY_SCOPE_AGENT);
       if (MODE == 0 && part != 0) return;
       if (first) {
-        unsigned long long word = lane == part ? (unsigned long long)__float_as_uint(s.s) << 32 | __float_as_uint(s.m) : UH_NO_WORD;
-        const bool other = lane < p.parts && lane != part;
+        unsigned long long word = wl == part ? (unsigned long long)__float_as_uint(s.s) << 32 | __float_as_uint(s.m) : UH_NO_WORD;
+        const bool other = wl < p.parts && wl != part;
         for (int i = 0; i < p.spins; ++i) {
-          if (other && word == UH_NO_WORD) word = __hip_atomic_load(words + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          if (other && word == UH_NO_WORD) word = __hip_atomic_load(words + wl, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
           if (!__any(other && word == UH_NO_WORD)) break;
           __builtin_amdgcn_s_sleep(2);
         }
         for (unsigned long long left = __ballot(other && word == UH_NO_WORD); left; left &= left - 1) {
           const int who = __ffsll(left) - 1, at = who * p.len;
           const RowStat u = alone_part_stat<T, NV>(row + at, min(p.len, a.v.C - at), a.c2);
-          if (lane == who) word = (unsigned long long)__float_as_uint(u.s) << 32 | __float_as_uint(u.m);
+          if (wl == who) word = (unsigned long long)__float_as_uint(u.s) << 32 | __float_as_uint(u.m);
         }
-        RowStat j{__uint_as_float((uint32_t)word), lane < p.parts ? __uint_as_float((uint32_t)(word >> 32)) : 0.f, 0.f};
-        if (lane >= p.parts) j.m = 0.f;
+        RowStat j{__uint_as_float((uint32_t)word), wl < p.parts ? __uint_as_float((uint32_t)(word >> 32)) : 0.f, 0.f};
+        if (wl >= p.parts) j.m = 0.f;
         for (int o = 1; o < 64 && o < p.parts; o <<= 1) {
           const RowStat u{__shfl_xor(j.m, o, 64), __shfl_xor(j.s, o, 64), 0.f};
-          j = lane & o ? join(u, j, a.c2) : join(j, u, a.c2);
+          j = wl & o ? join(u, j, a.c2) : join(j, u, a.c2);
         }
-        if (lane == 0) joined[0] = j.m, joined[1] = j.s;
+        if (wl == 0) joined[0] = j.m, joined[1] = j.s;
       }
       __syncthreads();
       s.m = joined[0], s.s = joined[1];
@@ -422,14 +432,14 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
     else {
       reg.map_store(out + c0, n, lane, [&](float v) { return dense * ex2(ref.z(v)); });
       __syncthreads();                                     // another wave may have written the class
-      if (first) q.fix(a, row, out, c0, n, co, ref, inv_s);
+      if (first) q.fix(a, out, c0, n, co, ref, inv_s);
     }
   }
-  if (MODE != 1 && part == 0 && first) {
-    const float kl = q.kl(a, row, s);
-    if (lane == 0) {
-      a.partial[r] = sum_t != 0.f ? (double)w * a.temperature * a.temperature * kl : 0.0;
-      if (a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
+  if (MODE != 1 && first) {
+    const float kl = MODE == 0 ? q.kl(a, s, 0, a.v.C) : q.kl(a, s, c0, n);
+    if (wl == 0) {
+      a.partial[MODE == 2 ? r * p.parts + part : r] = sum_t != 0.f ? (double)w * a.temperature * a.temperature * kl : 0.0;
+      if (MODE == 0 && a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
     }
   }
 }
@@ -653,10 +663,10 @@ template <typename T, int MODE> __global__ __launch_bounds__(256) void ds_any_ke
   if (MODE != 1 && lane == 0) a.partial[blockIdx.x] = total;
 }
 
-__global__ __launch_bounds__(1024) void ds_finish_kernel(int n, const double* __restrict__ partial, double scale, float* __restrict__ loss) {
+__global__ __launch_bounds__(1024) void ds_finish_kernel(long long n, const double* __restrict__ partial, double scale, float* __restrict__ loss) {
   __shared__ double buf[16];
   double v = 0.0;
-  for (int i = threadIdx.x; i < n; i += 1024) v += partial[i];
+  for (long long i = threadIdx.x; i < n; i += 1024) v += partial[i];
   v = wave_total(v);
   if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -697,8 +707,7 @@ static DsArgs ds_args(const uh_class_view* view, const uh_class_view* out, const
   return a;
 }
 
-// How a call's rows are taken, and its workspace: partial sums (one a row where parts of rows are workgroups, else one a
-// workgroup), then the words of rows in parts.
+// How a call's rows are taken, and its workspace: partial sums (one a workgroup), then the words of rows in parts.
 struct DsPlan {
   ClassPath path;
   RowCut cut;
@@ -710,8 +719,8 @@ static DsPlan ds_plan(const RowView& v, const RowView* vo, long long rows, int d
   const int elem = uh_elem_bytes(dtype);
   p.path = uh_class_path(v, vo, rows);
   p.parts = p.path == PATH_GROUP && (long long)v.C * elem > 8192;
-  p.cut = p.parts ? uh_row_cut(rows, v.C, dtype) : RowCut{1, v.C};
-  const size_t sums = p.parts && rows > UH_GRID_WAVES ? rows : UH_GRID_WAVES;
+  p.cut = p.parts ? uh_row_cut(rows, v.C, dtype, 65536) : RowCut{1, v.C};
+  const size_t sums = p.parts && rows * p.cut.parts > UH_GRID_WAVES ? rows * p.cut.parts : UH_GRID_WAVES;
   p.words_at = (sums * sizeof(double) + 15) / 16 * 16;
   p.bytes = p.words_at + (p.cut.parts > 1 ? (size_t)rows * p.cut.parts * 8 : 0);
   return p;
@@ -723,7 +732,7 @@ static int ds_spins() {
 }
 
 // MODE 0: loss, 1: gradient, 2: both; returns how many partial sums there are
-template <typename T, int MODE> static int ds_launch(const DsArgs& a, const T* x, T* dx, const DsPlan& p, char* ws, hipStream_t s) {
+template <typename T, int MODE> static long long ds_launch(const DsArgs& a, const T* x, T* dx, const DsPlan& p, char* ws, hipStream_t s) {
   constexpr int E = 16 / sizeof(T);
   const int C = a.v.C;
   const long long rows = a.rows;
@@ -776,10 +785,10 @@ template <typename T, int MODE> static int ds_launch(const DsArgs& a, const T* x
     else UH_GO(16);
   }
 #undef UH_GO
-  return (int)rows;
+  return MODE == 2 ? (long long)rows * cut.parts : rows;
 }
 
-template <int MODE> static int ds_dispatch(const DsArgs& a, int dtype, const void* x, void* dx, const DsPlan& p, void* ws, hipStream_t s) {
+template <int MODE> static long long ds_dispatch(const DsArgs& a, int dtype, const void* x, void* dx, const DsPlan& p, void* ws, hipStream_t s) {
   if (dtype == UH_F32) return ds_launch<float, MODE>(a, (const float*)x, (float*)dx, p, (char*)ws, s);
   if (dtype == UH_BF16) return ds_launch<bf16, MODE>(a, (const bf16*)x, (bf16*)dx, p, (char*)ws, s);
   return ds_launch<f16, MODE>(a, (const f16*)x, (f16*)dx, p, (char*)ws, s);
@@ -801,7 +810,7 @@ extern "C" int uh_topk_distill(const uh_class_view* view, const void* logits, co
   DsArgs a = ds_args(view, view, slots, weight, temperature);
   a.stats = stats, a.partial = (double*)workspace;
   const DsPlan p = ds_plan(a.v, nullptr, a.rows, view->dtype);
-  const int n = ds_dispatch<0>(a, view->dtype, logits, nullptr, p, workspace, (hipStream_t)s);
+  const long long n = ds_dispatch<0>(a, view->dtype, logits, nullptr, p, workspace, (hipStream_t)s);
   hipLaunchKernelGGL(ds_finish_kernel, dim3(1), dim3(1024), 0, (hipStream_t)s, n, (const double*)workspace, scale, loss);
   return uh_check_launch("topk_distill");
 }
@@ -832,7 +841,7 @@ extern "C" int uh_topk_distill_step(const uh_class_view* view, const uh_class_vi
   DsArgs a = ds_args(view, out_view, slots, weight, temperature);
   a.grad_scale = (float)(scale * (double)grad_scale), a.partial = (double*)workspace;
   const DsPlan p = ds_plan(a.v, &a.vo, a.rows, view->dtype);
-  const int n = ds_dispatch<2>(a, view->dtype, logits, dlogits, p, workspace, (hipStream_t)s);
+  const long long n = ds_dispatch<2>(a, view->dtype, logits, dlogits, p, workspace, (hipStream_t)s);
   hipLaunchKernelGGL(ds_finish_kernel, dim3(1), dim3(1024), 0, (hipStream_t)s, n, (const double*)workspace, scale, loss);
   return uh_check_launch("topk_distill_step");
 }

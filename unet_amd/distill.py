@@ -14,7 +14,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import SLOTS_MAX, lib
-from .class_rows import DTYPE_CODE, INT_BYTES, Rows, byref, checked_temperature
+from .class_rows import DTYPE_CODE, INT_BYTES, Rows, byref, checked_temperature, fp32_rows
 from .label_probs import label_log_probs
 
 
@@ -65,19 +65,20 @@ class _TopKDistillFn(torch.autograd.Function):
     def forward(ctx, logits, r, t, temperature, scale):
         loss, stats = _forward(r, t, temperature, scale, True)
         ctx.save_for_backward(r.x, t.value, t.index, t.weight, stats)
-        ctx.args = (r.dim, temperature, scale)
+        r.x = None                                # the saved tensors hold the logits, and let go of them
+        ctx.args = (r, temperature, scale)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
         x, value, index, weight, stats = ctx.saved_tensors
-        dim, temperature, scale = ctx.args
-        r = Rows(x, dim, "topk_distill").bind("topk_distill")
-        dx, out_view = r.new_grad()
-        g = gout.float().contiguous()
-        r.call("uh_topk_distill_bwd", byref(r.view), byref(out_view), r.x.data_ptr(),
-               byref(_slots(value, index, value.shape[dim])), weight.data_ptr() if weight is not None else None,
+        r, temperature, scale = ctx.args
+        dx, out_view = r.new_grad(x)
+        g = fp32_rows(gout)
+        r.bind("topk_distill")
+        r.call("uh_topk_distill_bwd", byref(r.view), byref(out_view), x.data_ptr(),
+               byref(_slots(value, index, value.shape[r.dim])), None if weight is None else weight.data_ptr(),
                temperature, scale, g.data_ptr(), stats.data_ptr(), dx.data_ptr())
         return dx, None, None, None, None
 
@@ -129,7 +130,7 @@ def topk_distill_with_logits(logits, top_logits, top_index, temperature=1.0, wei
         r.bind(what)
         if r.rows == 0:
             return torch.zeros((), dtype=torch.float32, device=r.device), torch.empty_like(r.x)
-        dx, out_view = r.new_grad()
+        dx, out_view = r.new_grad(r.x)
         loss = torch.empty((), dtype=torch.float32, device=r.device)
         ws_bytes = lib.uh_topk_distill_workspace(byref(r.view))
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=r.device)

@@ -14,31 +14,36 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ._lib import TOP_MAX, lib
-from .class_rows import INT_BYTES, Rows, byref, checked_temperature
+from .class_rows import INT_BYTES, Rows, byref, checked_temperature, fp32_rows
 
 LabelLogProbs = namedtuple("LabelLogProbs", "log_prob entropy top_log_prob top_index")
 
 
 def _forward(r, labels, top, temperature, ignore_index, want_stats):
-    dev = r.device
-    log_prob = torch.empty(r.row_shape, dtype=torch.float32, device=dev) if labels is not None else None
-    entropy = torch.empty(r.row_shape, dtype=torch.float32, device=dev)
-    top_lp = top_idx = stats = ws = None
+    dev, rows, f32 = r.device, r.row_shape, torch.float32
+    entropy = torch.empty(rows, dtype=f32, device=dev)
+    log_prob = top_lp = top_idx = stats = ws = None
+    lab_ptr = lp_ptr = tl_ptr = ti_ptr = st_ptr = ws_ptr = None
+    lab_bytes = 0
+    if labels is not None:
+        log_prob = torch.empty(rows, dtype=f32, device=dev)
+        lab_ptr, lp_ptr, lab_bytes = labels.data_ptr(), log_prob.data_ptr(), INT_BYTES[labels.dtype]
     if top:
-        top_lp = torch.empty(r.entries(top), dtype=torch.float32, device=dev)
-        top_idx = torch.empty(r.entries(top), dtype=torch.int32, device=dev)
+        shape = r.entries(top)
+        top_lp = torch.empty(shape, dtype=f32, device=dev)
+        top_idx = torch.empty(shape, dtype=torch.int32, device=dev)
+        tl_ptr, ti_ptr = top_lp.data_ptr(), top_idx.data_ptr()
     if want_stats:
-        stats = torch.empty((r.rows, 2), dtype=torch.float32, device=dev)
+        stats = torch.empty((r.rows, 2), dtype=f32, device=dev)
+        st_ptr = stats.data_ptr()
     if r.rows:
         v = byref(r.view)
         ws_bytes = lib.uh_label_log_probs_workspace(v, top)
         if ws_bytes:
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        r.call("uh_label_log_probs", v, r.x.data_ptr(), labels.data_ptr() if labels is not None else None,
-               INT_BYTES[labels.dtype] if labels is not None else 0, ignore_index, top, temperature,
-               log_prob.data_ptr() if log_prob is not None else None, entropy.data_ptr(),
-               top_lp.data_ptr() if top else None, top_idx.data_ptr() if top else None,
-               stats.data_ptr() if want_stats else None, ws.data_ptr() if ws is not None else None, ws_bytes)
+            ws_ptr = ws.data_ptr()
+        r.call("uh_label_log_probs", v, r.x.data_ptr(), lab_ptr, lab_bytes, ignore_index, top, temperature, lp_ptr,
+               entropy.data_ptr(), tl_ptr, ti_ptr, st_ptr, ws_ptr, ws_bytes)
     return log_prob, entropy, top_lp, top_idx, stats
 
 
@@ -47,10 +52,11 @@ class _LabelLogProbsFn(torch.autograd.Function):
     def forward(ctx, logits, r, labels, top, temperature, ignore_index):
         log_prob, entropy, top_lp, top_idx, stats = _forward(r, labels, top, temperature, ignore_index, True)
         ctx.save_for_backward(r.x, labels, stats, entropy)
-        ctx.dim, ctx.temperature, ctx.ignore_index = r.dim, temperature, ignore_index
         ctx.set_materialize_grads(False)
         if top:
             ctx.mark_non_differentiable(top_lp, top_idx)
+        r.x = None                                # the saved tensors hold the logits, and let go of them
+        ctx.args = (r, temperature, ignore_index)
         return log_prob, entropy, top_lp, top_idx
 
     @staticmethod
@@ -59,16 +65,16 @@ class _LabelLogProbsFn(torch.autograd.Function):
         if g_lp is None and g_ent is None:
             return (None,) * 6
         x, labels, stats, entropy = ctx.saved_tensors
-        r = Rows(x, ctx.dim, "label_log_probs").bind("label_log_probs")
-        dx, out_view = r.new_grad()
+        r, temperature, ignore_index = ctx.args
+        dx, out_view = r.new_grad(x)
         if r.rows:
-            g_lp = None if g_lp is None else g_lp.float().contiguous()
-            g_ent = None if g_ent is None else g_ent.float().contiguous()
-            r.call("uh_label_log_probs_bwd", byref(r.view), byref(out_view), r.x.data_ptr(),
-                   labels.data_ptr() if labels is not None else None,
-                   INT_BYTES[labels.dtype] if labels is not None else 0, ctx.ignore_index, ctx.temperature,
-                   stats.data_ptr(), entropy.data_ptr(), g_lp.data_ptr() if g_lp is not None else None,
-                   g_ent.data_ptr() if g_ent is not None else None, dx.data_ptr())
+            g_lp, g_ent = fp32_rows(g_lp), fp32_rows(g_ent)
+            r.bind("label_log_probs")
+            lab = labels is not None
+            r.call("uh_label_log_probs_bwd", byref(r.view), byref(out_view), x.data_ptr(),
+                   labels.data_ptr() if lab else None, INT_BYTES[labels.dtype] if lab else 0, ignore_index, temperature,
+                   stats.data_ptr(), entropy.data_ptr(), None if g_lp is None else g_lp.data_ptr(),
+                   None if g_ent is None else g_ent.data_ptr(), dx.data_ptr())
         return dx, None, None, None, None, None
 
 
