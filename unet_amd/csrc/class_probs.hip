@@ -11,7 +11,7 @@ struct LpArgs {
   const void* labels;
   long long ignore;
   int label_bytes, top;
-  float temperature, c2;
+  float inv_t, c2;
   float *log_prob, *entropy, *top_lp;
   int* top_idx;
   float* stats;
@@ -27,10 +27,10 @@ struct LpArgs {
   // by one thread: values of a row; x_label: its label's logit where the label is a class.  Returns ln s.
   __device__ __forceinline__ float write_row(long long r, long long l, float x_label, const RowStat& s) const {
     const float ln_s = RowRef(s.m, c2).ln_s(s.m, s.s);
-    // ln s = log(s) - d and t share d (the rounding of M), so that the entropy takes log(s) itself
-    entropy[r] = s.s == 0.f ? 0.f : logf(s.s) - (s.t / s.s) * UH_LN2;
+    // ln s and t share the rounding of M, so that the entropy takes the logarithm of s itself
+    entropy[r] = s.s == 0.f ? 0.f : (lg2(s.s) - s.t * rcp(s.s)) * UH_LN2;
     if (labels)
-      log_prob[r] = l < 0 || l >= v.C ? NAN : s.s == 0.f ? -INFINITY : scaled(x_label, s.m, temperature) - ln_s;
+      log_prob[r] = l < 0 || l >= v.C ? NAN : s.s == 0.f ? -INFINITY : scaled(x_label, s.m, inv_t) - ln_s;
     if (stats) { stats[2 * r] = s.m; stats[2 * r + 1] = s.s; }
     return ln_s;
   }
@@ -39,7 +39,7 @@ struct LpArgs {
   __device__ __forceinline__ void write_top(long long r, int k, float value, int cls, float m, float ln_s, float s) const {
     const bool undefined = !(s >= 0.f);
     const long long e = v.entry(r, k, top);
-    top_lp[e] = undefined ? NAN : cls >= 0 ? scaled(value, m, temperature) - ln_s : -INFINITY;
+    top_lp[e] = undefined ? NAN : cls >= 0 ? scaled(value, m, inv_t) - ln_s : -INFINITY;
     top_idx[e] = undefined ? -1 : cls;
   }
 };
@@ -232,24 +232,23 @@ template <typename T, int CREG, bool STAGED, int LIST>
 __global__ __launch_bounds__(64) void lp_thread_kernel(LpArgs a, const T* __restrict__ x, bool wide) {
   extern __shared__ __align__(16) char lds[];
   T* tile = reinterpret_cast<T*>(lds);
-  const int lane = threadIdx.x, C = a.v.C;
+  const int lane = threadIdx.x, C = a.v.C, so = (int)a.v.so;
   const long long blocks = (a.rows + 63) / 64;
   for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
     const long long r = b * 64 + lane;
     const bool there = r < a.rows;
-    const T* row;
-    if (STAGED) {
+    if constexpr (STAGED) {
       const int here = (int)min(64ll, a.rows - b * 64);
       __syncthreads();
-      copy_to_lds(tile, x + b * 64 * a.v.so, (int)((here - 1) * a.v.so) + C);
+      copy_to_lds(tile, x + b * 64 * so, (here - 1) * so + C);
       __syncthreads();
-      row = tile + lane * (int)a.v.so;
-    } else {
-      row = x + (there ? a.v.base(r) : 0);
     }
+    const ApartRows at(a.v, b * 64, lane);
+    const auto cls = [&](int c) { return STAGED ? tile + lane * so + c : at.at(x, c * a.v.sc); };
     if (!there) continue;
     float v[CREG];
-    load_classes<T, CREG, STAGED>(v, row, a.v.sc, C, wide);                       // on its way while the label is
+    if (STAGED && wide) load_classes_wide<T, CREG>(v, tile + lane * so, C);
+    else load_classes<T, CREG>(v, C, cls);                                       // on its way while the label is
     const long long l = a.label(r);
     if (a.ignored(l)) {
       a.write_ignored(r);
@@ -257,26 +256,35 @@ __global__ __launch_bounds__(64) void lp_thread_kernel(LpArgs a, const T* __rest
       continue;
     }
     const RowStat s = thread_row_stat<CREG, true>(v, C, a.c2);
-    const float ln_s = a.write_row(r, l, a.is_class(l) ? ld(row + (STAGED ? l : l * a.v.sc)) : 0.f, s);
-    if constexpr (LIST > 0) {
-      float lv = 0.f;
-      int lc = 0;
-      for (int k0 = 0; k0 < a.top; k0 += LIST) {
-        TopList<LIST> list;
-        if constexpr (STAGED || CREG == 64) {              // from LDS or the caches again: 64 unrolled steps cost 256 registers
-          for (int c = 0; c < C; ++c) {
-            const float u = (float)row[STAGED ? c : c * a.v.sc];
-            list.insert(k0 ? behind(u, c, lv, lc) : u, c);
-          }
-        } else {
+    float x_label = 0.f;                                   // apart, 64 labels would be 64 lines: the registers hold them all
+    if (STAGED) x_label = a.is_class(l) ? ld(tile + lane * so + (int)l) : 0.f;
+    else if (a.labels) {
+      const int n = renew_uniform(C);
 #pragma unroll
-          for (int c = 0; c < CREG; ++c)
-            if (c < C) list.insert(k0 ? behind(v[c], c, lv, lc) : v[c], c);
-        }
+      for (int c = 0; c < CREG; ++c)
+        if (c < n) x_label = l == c ? v[c] : x_label;
+    }
+    const float ln_s = a.write_row(r, l, x_label, s);
+    if constexpr (LIST > 0) {
+      TopList<LIST> list;
+      if constexpr (STAGED || CREG == 64) {                // from LDS or the caches again: 64 unrolled steps cost 256 registers
+        for (int c = 0; c < C; ++c) list.insert((float)*cls(c), c);
+      } else {
+        const int n = renew_uniform(C);
+#pragma unroll
+        for (int c = 0; c < CREG; ++c)
+          if (c < n) list.insert(v[c], c);
+      }
+      for (int k0 = 0;;) {
 #pragma unroll
         for (int i = 0; i < LIST; ++i)
           if (k0 + i < a.top) a.write_top(r, k0 + i, list.v[i], list.c[i], s.m, ln_s, s.s);
-        lv = list.v[LIST - 1], lc = list.c[LIST - 1];
+        k0 += LIST;
+        if (k0 >= a.top) break;
+        const float lv = list.v[LIST - 1];                 // the next LIST are those behind the last of these
+        const int lc = list.c[LIST - 1];
+        list = TopList<LIST>();
+        for (int c = 0; c < C; ++c) list.insert(behind((float)*cls(c), c, lv, lc), c);
       }
     }
   }
@@ -370,7 +378,7 @@ struct LpCoef {
     m = k.stats[2 * r];
     const float s = k.stats[2 * r + 1];
     const float g = k.g_lp ? k.g_lp[r] : 0.f, h = k.g_ent ? k.g_ent[r] : 0.f;
-    const float l2 = log2f(s), inv = 1.f / s;
+    const float l2 = lg2(s), inv = rcp(s);
     const bool bad = k.g_lp && (l < 0 || l >= k.v.C);
     b = -h * UH_LN2 * k.inv_t;
     a = bad ? NAN : (-(g + h * k.entropy[r]) * k.inv_t - b * l2) * inv;
@@ -450,6 +458,28 @@ template <typename T> __global__ __launch_bounds__(64) void lp_bwd_thread_kernel
   }
 }
 
+// up to 64 classes that lie apart
+template <typename T> __global__ __launch_bounds__(64) void lp_bwd_apart_kernel(LpBwd k, const T* __restrict__ x, T* __restrict__ dx) {
+  const int lane = threadIdx.x, C = k.v.C;
+  const long long blocks = (k.rows + 63) / 64;
+  for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const long long r = b * 64 + lane;
+    const ApartRows at(k.v, b * 64, lane), to(k.vo, b * 64, lane);
+    if (r >= k.rows) continue;
+    const LpCoef q(k, r);
+    const RowRef ref(q.m, k.c2);
+    for (int c0 = 0; c0 < C; c0 += 16) {
+      float v[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (c0 + j < C) v[j] = (float)*at.at(x, (c0 + j) * k.v.sc);
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (c0 + j < C) *to.at(dx, (c0 + j) * k.vo.sc) = (T)(q.off ? 0.f : q.of(ref, v[j]) + (c0 + j == q.label ? q.own : 0.f));
+    }
+  }
+}
+
 // classes that lie apart: one thread per row
 template <typename T> __global__ __launch_bounds__(64) void lp_bwd_walk_kernel(LpBwd k, const T* __restrict__ x, T* __restrict__ dx) {
   const long long r = (long long)blockIdx.x * 64 + threadIdx.x;
@@ -486,7 +516,7 @@ template <typename T> __global__ __launch_bounds__(256) void lp_bwd_any_kernel(L
 // is what a workgroup's other waves wait for, and 68 registers leave room for seven workgroups a CU, 108 for four (1024 rows
 // of 131072 bf16 classes, top 64: see the table of measurements).  Without, 64 KB.
 static RowCut lp_cut(const RowView& v, long long rows, int dtype, int top) {
-  if (uh_class_path(v, nullptr, rows) != PATH_GROUP || (long long)v.C * uh_elem_bytes(dtype) <= 8192) return RowCut{1, v.C};
+  if (uh_class_path(v, nullptr, rows, dtype) != PATH_GROUP || (long long)v.C * uh_elem_bytes(dtype) <= 8192) return RowCut{1, v.C};
   return uh_row_cut(rows, v.C, dtype, top ? 32768 : 65536);
 }
 
@@ -502,7 +532,7 @@ template <typename T> static void lp_launch(const LpArgs& a, const T* x, int dty
   constexpr int E = 16 / sizeof(T);
   const int C = a.v.C;
   const long long rows = a.rows;
-  const ClassPath path = uh_class_path(a.v, nullptr, rows);
+  const ClassPath path = uh_class_path(a.v, nullptr, rows, dtype);
   const dim3 waves(uh_grid((rows + 63) / 64, UH_GRID_WAVES));
   if (path == PATH_STAGED || path == PATH_APART) {
     const bool staged = path == PATH_STAGED, wide = staged && (a.v.so * sizeof(T)) % 16 == 0;
@@ -573,7 +603,7 @@ extern "C" int uh_label_log_probs(const uh_class_view* view, const void* logits,
   a.v = uh_row_view(view);
   a.rows = view->outer * view->inner;
   a.labels = labels, a.label_bytes = label_bytes, a.ignore = ignore_index;
-  a.top = top, a.temperature = temperature, a.c2 = (float)(1.4426950408889634 / (double)temperature);
+  a.top = top, a.inv_t = 1.f / temperature, a.c2 = (float)(1.4426950408889634 / (double)temperature);
   a.log_prob = log_prob, a.entropy = entropy, a.top_lp = top_log_prob, a.top_idx = top_index, a.stats = stats;
   if (view->dtype == UH_F32) lp_launch<float>(a, (const float*)logits, view->dtype, workspace, (hipStream_t)s);
   else if (view->dtype == UH_BF16) lp_launch<bf16>(a, (const bf16*)logits, view->dtype, workspace, (hipStream_t)s);
@@ -581,16 +611,18 @@ extern "C" int uh_label_log_probs(const uh_class_view* view, const void* logits,
   return uh_check_launch("label_log_probs");
 }
 
-template <typename T> static void lp_bwd_launch(const LpBwd& k, const T* x, T* dx, hipStream_t s) {
+template <typename T> static void lp_bwd_launch(const LpBwd& k, const T* x, T* dx, int dtype, hipStream_t s) {
   constexpr int E = 16 / sizeof(T);
   const int C = k.v.C;
   const long long rows = k.rows;
-  const ClassPath path = uh_class_path(k.v, &k.vo, rows);
+  const ClassPath path = uh_class_path(k.v, &k.vo, rows, dtype);
   if (path == PATH_STAGED) {
     const bool wide = (k.v.so * sizeof(T)) % 16 == 0 && (C * sizeof(T)) % 16 == 0;
     const size_t lds = ((64 * k.v.so + E - 1) / E * E + 64 * C) * sizeof(T);
     hipLaunchKernelGGL((lp_bwd_thread_kernel<T>), dim3(uh_grid((rows + 63) / 64, UH_GRID_WAVES)), dim3(64), lds, s, k, x, dx, wide);
-  } else if (path == PATH_APART || path == PATH_WALK) {
+  } else if (path == PATH_APART) {
+    hipLaunchKernelGGL((lp_bwd_apart_kernel<T>), dim3(uh_grid((rows + 63) / 64, UH_GRID_WAVES)), dim3(64), 0, s, k, x, dx);
+  } else if (path == PATH_WALK) {
     hipLaunchKernelGGL((lp_bwd_walk_kernel<T>), dim3((unsigned)((rows + 63) / 64)), dim3(64), 0, s, k, x, dx);
   } else if (path == PATH_ANY) {
     hipLaunchKernelGGL((lp_bwd_any_kernel<T>), dim3(uh_grid(rows, UH_GRID_WAVES)), dim3(256), 0, s, k, x, dx);
@@ -625,8 +657,8 @@ extern "C" int uh_label_log_probs_bwd(const uh_class_view* view, const uh_class_
   k.labels = labels, k.label_bytes = label_bytes, k.ignore = ignore_index;
   k.inv_t = 1.f / temperature, k.c2 = (float)(1.4426950408889634 / (double)temperature);
   k.stats = stats, k.entropy = entropy, k.g_lp = g_log_prob, k.g_ent = g_entropy;
-  if (view->dtype == UH_F32) lp_bwd_launch<float>(k, (const float*)logits, (float*)dlogits, (hipStream_t)s);
-  else if (view->dtype == UH_BF16) lp_bwd_launch<bf16>(k, (const bf16*)logits, (bf16*)dlogits, (hipStream_t)s);
-  else lp_bwd_launch<f16>(k, (const f16*)logits, (f16*)dlogits, (hipStream_t)s);
+  if (view->dtype == UH_F32) lp_bwd_launch<float>(k, (const float*)logits, (float*)dlogits, view->dtype, (hipStream_t)s);
+  else if (view->dtype == UH_BF16) lp_bwd_launch<bf16>(k, (const bf16*)logits, (bf16*)dlogits, view->dtype, (hipStream_t)s);
+  else lp_bwd_launch<f16>(k, (const f16*)logits, (f16*)dlogits, view->dtype, (hipStream_t)s);
   return uh_check_launch("label_log_probs_bwd");
 }

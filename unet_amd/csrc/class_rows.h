@@ -66,21 +66,24 @@ template <typename T> __device__ __forceinline__ void st(T* p, float v) { *p = (
 static constexpr float UH_LN2 = 0.693147180559945309f;
 static constexpr float UH_ZMIN = -200.f;      // 2^-200 is 0 in fp32: below it a term of t is 0
 
+// v_exp_f32, v_log_f32, v_rcp_f32: good to a unit in the last place, results below the smallest normal number are 0
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float lg2(float x) { return __builtin_amdgcn_logf(x); }
+__device__ __forceinline__ float rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 
 struct RowRef {           // the point and the scale a row's exponents are taken in
   float c, M;
   __device__ __forceinline__ RowRef(float m, float c2) : c(fabsf(m) >= 0x1p100f ? 0x1p-20f : c2), M(m * c) {}
   __device__ __forceinline__ float z(float x) const { return fmaf(x, c, -M); }
-  __device__ __forceinline__ float ln_s(float m, float s) const { return logf(s) - fmaf(m, c, -M) * UH_LN2; }
+  __device__ __forceinline__ float ln_s(float m, float s) const { return (lg2(s) - fmaf(m, c, -M)) * UH_LN2; }
 };
 struct RowStat { float m, s, t; };
 
 // (x - m) / T of a reported value; x - m may overflow where its quotient does not (a class masked with the type's lowest
 // value, T > 1)
-__device__ __forceinline__ float scaled(float x, float m, float temperature) {
+__device__ __forceinline__ float scaled(float x, float m, float inv_t) {
   const float d = x - m;
-  return d == -INFINITY ? x / temperature - m / temperature : d / temperature;
+  return d == -INFINITY ? x * inv_t - m * inv_t : d * inv_t;
 }
 
 // joins the statistics of two parts of a row; a part without a finite logit (s = 0) has no say in m
@@ -395,6 +398,13 @@ __device__ __forceinline__ void group_sums(RowRegs<T, G, NV>& x, const RowRef& r
   }
 }
 
+// Keeps the compiler from working out every `c < C` of an unrolled sweep ahead of it (64 scalar registers, spilled to vectors).
+__device__ __forceinline__ int renew_uniform(int C) {
+  C = __builtin_amdgcn_readfirstlane(C);
+  asm volatile("" : "+s"(C));
+  return C;
+}
+
 // Inside a loop over rows: keeps the compiler from carrying every vector's place in a row from turn to turn (two registers
 // a vector, which cost a third of the waves).
 __device__ __forceinline__ int renew(int lane) {
@@ -434,13 +444,18 @@ template <int N> struct TopList {
   __device__ __forceinline__ void insert(float x, int cls) {
 #pragma unroll
     for (int i = N - 1; i > 0; --i) {
-      const bool above = x > v[i - 1], here = x > v[i];
-      c[i] = above ? c[i - 1] : here ? cls : c[i];
-      v[i] = above ? v[i - 1] : here ? x : v[i];
+      const int here = select(x > v[i], cls, c[i]);
+      c[i] = select(x > v[i - 1], c[i - 1], here);
+      v[i] = __builtin_amdgcn_fmed3f(x, v[i - 1], v[i]);
     }
-    const bool first = x > v[0];
-    c[0] = first ? cls : c[0];
-    v[0] = first ? x : v[0];
+    c[0] = select(x > v[0], cls, c[0]);
+    v[0] = max3(x, v[0], v[0]);
+  }
+  // a selection that stays one: the compiler makes branches of nested ones
+  __device__ __forceinline__ static int select(bool p, int a, int b) {
+    int d = p ? a : b;
+    asm("" : "+v"(d));
+    return d;
   }
   __device__ __forceinline__ void pop() {
 #pragma unroll
@@ -658,31 +673,64 @@ template <typename T> __device__ __forceinline__ void copy_from_lds(T* __restric
     *reinterpret_cast<Loose16<T>*>(dst + i) = __builtin_bit_cast(Loose16<T>, *reinterpret_cast<const U4*>(src + i));
   for (int e = n / E * E + lane; e < n; e += 64) dst[e] = src[e];
 }
-// a row of C <= CREG classes to registers, -inf behind its end
-template <typename T, int CREG, bool STAGED>
-__device__ __forceinline__ void load_classes(float (&x)[CREG], const T* __restrict__ p, long long sc, int C, bool wide) {
-  constexpr int E = 16 / sizeof(T);
-  if (STAGED && wide) {                                    // rows start on 16 bytes and are at least that far apart
-#pragma unroll
-    for (int c = 0; c < CREG; c += E)
-      if (c < C) {
-        T v[E];
-        *reinterpret_cast<U4*>(v) = *reinterpret_cast<const U4*>(p + c);
-#pragma unroll
-        for (int j = 0; j < E; ++j) x[c + j] = c + j < C ? (float)v[j] : -INFINITY;
-      } else {
-#pragma unroll
-        for (int j = 0; j < E; ++j) x[c + j] = -INFINITY;
-      }
-    return;
+// 64 rows that lie apart: one address for the wave and an offset of 32 bits for the lane (uh_apart checks that it fits), so that
+// an access to a class takes a scalar addition and no registers.
+struct ApartRows {
+  long long base;             // elements, of the wave's first row
+  uint32_t off;               // elements, the lane's row from there
+  __device__ __forceinline__ ApartRows(const RowView& v, long long r0, int lane) {
+    if (v.inner == 1) {
+      base = r0 * v.so;
+      off = (uint32_t)(lane * v.so);
+      return;
+    }
+    const unsigned inner = (unsigned)v.inner;
+    const unsigned o0 = __builtin_amdgcn_readfirstlane((unsigned)r0 / inner), i0 = (unsigned)r0 - o0 * inner;
+    base = o0 * v.so + i0 * v.si;
+    unsigned o = 0, i = i0 + lane;
+    if (i0 + 63 >= inner) {
+      o = i / inner;
+      i -= o * inner;
+    }
+    off = (uint32_t)(o * v.so + ((long long)i - i0) * v.si);
   }
+  template <typename T> __device__ __forceinline__ T* at(T* p, long long c_sc) const {
+    return (T*)((char*)(p + base + c_sc) + (size_t)(off * (uint32_t)sizeof(T)));
+  }
+};
+static inline bool uh_apart(const RowView& v, int elem) {
+  const long long most = 0x7fffffffll / elem;
+  if (v.inner == 1) return v.so < most / 64;
+  if (v.si > most / 64 || v.inner > most / (v.si ? v.si : 1) || v.so > most) return false;
+  return v.so >= (v.inner - 1) * v.si && (v.inner >= 64 ? v.so + 64 * v.si < most : v.so < most / 80);
+}
+// a row of C <= CREG classes to registers, -inf behind its end; p(c): where class c lies
+template <typename T, int CREG, typename F>
+__device__ __forceinline__ void load_classes(float (&x)[CREG], int C, F p) {
+  C = renew_uniform(C);
 #pragma unroll
-  for (int c = 0; c < CREG; ++c) x[c] = -INFINITY;
+  for (int c = 0; c < CREG; ++c) {
+    x[c] = -INFINITY;
+    if (c < C) x[c] = (float)*p(c);
+  }
+}
+// the same from LDS; wide: rows start on 16 bytes and are at least that far apart
+template <typename T, int CREG> __device__ __forceinline__ void load_classes_wide(float (&x)[CREG], const T* p, int C) {
+  constexpr int E = 16 / sizeof(T);
 #pragma unroll
-  for (int c = 0; c < CREG; ++c)
-    if (c < C) x[c] = STAGED ? (float)p[c] : (float)p[c * sc];
+  for (int c = 0; c < CREG; c += E)
+    if (c < C) {
+      T v[E];
+      *reinterpret_cast<U4*>(v) = *reinterpret_cast<const U4*>(p + c);
+#pragma unroll
+      for (int j = 0; j < E; ++j) x[c + j] = c + j < C ? (float)v[j] : -INFINITY;
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j) x[c + j] = -INFINITY;
+    }
 }
 template <int CREG, bool ENT> __device__ __forceinline__ RowStat thread_row_stat(const float (&x)[CREG], int C, float c2) {
+  C = renew_uniform(C);
   float m = x[0];
 #pragma unroll
   for (int c = 1; c < CREG; c += 2)
@@ -690,12 +738,16 @@ template <int CREG, bool ENT> __device__ __forceinline__ RowStat thread_row_stat
   if (m == -INFINITY) m = 0.f;
   const RowRef ref(m, c2);
   float s = 0.f, t = 0.f;
+  C = renew_uniform(C);
 #pragma unroll
   for (int c = 0; c < CREG; ++c)
     if (c < C) {
       const float z = ref.z(x[c]), e = ex2(z);
       s += e;
-      if (ENT) t = fmaf(e, fmaxf(z, UH_ZMIN), t);
+      if (ENT) {
+        t = fmaf(e, fmaxf(z, UH_ZMIN), t);
+        asm volatile("" : "+v"(s), "+v"(t));                 // now: left to be summed later, the terms take two registers a class
+      }
     }
   return RowStat{m, s, t};
 }
@@ -720,11 +772,14 @@ enum { UH_GRID_WAVES = 256 * 32 };               // workgroups that loop over ro
 // 16 bits: 2 of 16 at work).  STAGED needs one step from row to row, no more than 64 classes and a half further (LDS, and bytes
 // read between the rows), and a dense gradient.
 enum ClassPath { PATH_GROUP, PATH_STAGED, PATH_APART, PATH_WALK, PATH_ANY };
-static inline ClassPath uh_class_path(const RowView& v, const RowView* vo, long long rows) {
+static inline ClassPath uh_class_path(const RowView& v, const RowView* vo, long long rows, int dtype) {
+  const int elem = uh_elem_bytes(dtype);
   if (v.C <= 64) {
     const bool staged = v.sc == 1 && v.inner == 1 && v.so >= v.C && v.so <= 96 &&
                         (!vo || (vo->sc == 1 && vo->inner == 1 && vo->so == v.C));
-    return staged ? PATH_STAGED : PATH_APART;
+    if (staged) return PATH_STAGED;
+    if (uh_apart(v, elem) && (!vo || uh_apart(*vo, elem))) return PATH_APART;
+    return rows >= 256 ? PATH_WALK : PATH_ANY;
   }
   if (v.sc == 1 && (!vo || vo->sc == 1)) return PATH_GROUP;
   return rows >= 256 ? PATH_WALK : PATH_ANY;

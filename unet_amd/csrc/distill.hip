@@ -17,7 +17,7 @@ struct DsArgs {
   const void *value, *index;
   int K, value_dtype, index_bytes;
   const float* weight;
-  float temperature, c2;
+  float temperature, inv_t, c2;
   float grad_scale;               // scale * grad_scale, or scale where gout is given
   const float* gout;
   float* stats;                   // [rows][2]: m, s
@@ -41,8 +41,8 @@ struct DsArgs {
 };
 
 // ln t_k - ln p of a slot, weighted by t_k: e is 2^(..) of the slot against the teacher's maximum vm, sv their sum
-__device__ __forceinline__ float slot_term(float t, float val, float vm, float ln_sv, float x, float m, float ln_s, float temperature) {
-  return t > 0.f ? t * ((scaled(val, vm, temperature) - ln_sv) - (scaled(x, m, temperature) - ln_s)) : t == t ? 0.f : NAN;
+__device__ __forceinline__ float slot_term(float t, float val, float vm, float ln_sv, float x, float m, float ln_s, float inv_t) {
+  return t > 0.f ? t * ((scaled(val, vm, inv_t) - ln_sv) - (scaled(x, m, inv_t) - ln_s)) : t == t ? 0.f : NAN;
 }
 
 // ---- a row by 16 lanes, or by any group with any strides: the slots in LDS -------------------------------------------------------
@@ -65,7 +65,7 @@ template <int G> __device__ __forceinline__ Teacher group_teacher(const DsArgs& 
   float sv = 0.f;
   for (int k = lane; k < a.K; k += G) sv += ex2(ref.z(t_of[k]));
   Red<G>::sum2(sv, bad, red);
-  const float inv = bad != 0.f ? NAN : sv == 0.f ? 0.f : 1.f / sv;
+  const float inv = bad != 0.f ? NAN : sv == 0.f ? 0.f : rcp(sv);
   for (int k = lane; k < a.K; k += G) {
     const float val = t_of[k];
     t_of[k] = ex2(ref.z(val)) * inv;
@@ -82,7 +82,7 @@ template <typename T, int G> __device__ __forceinline__ float group_kl(const DsA
   else if (q.sum != 0.f)
     for (int k = lane; k < a.K; k += G) {
       const float t = t_of[k];
-      if (t != 0.f) part += slot_term(t, a.value_of(a.v.entry(r, k, a.K)), q.vm, q.ln_sv, ld(row + c_of[k] * a.v.sc), s.m, ln_s, a.temperature);
+      if (t != 0.f) part += slot_term(t, a.value_of(a.v.entry(r, k, a.K)), q.vm, q.ln_sv, ld(row + c_of[k] * a.v.sc), s.m, ln_s, a.inv_t);
     }
   return Red<G>::sum_(part, red);
 }
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(64) void ds_quad_kernel(DsArgs a, const T* __restri
       if (there) {
         T* out = dx + a.vo.base(r);
         const RowRef ref(s.m, a.c2);
-        const float inv_s = s.s == 0.f ? 0.f : 1.f / s.s, co = a.coef(w), dense = co * q.sum * inv_s;
+        const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * q.sum * inv_s;
         reg.fresh();
         if (off || q.sum == 0.f) reg.map_store(out, C, lane, [](float) { return 0.f; });
         else {
@@ -200,7 +200,7 @@ struct SlotWave {
     }
     sv = group_sum<64>(sv);
     const bool wrong = __any(bad != 0.f);
-    const float inv = wrong ? NAN : sv == 0.f ? 0.f : 1.f / sv;
+    const float inv = wrong ? NAN : sv == 0.f ? 0.f : rcp(sv);
 #pragma unroll
     for (int q = 0; q < 4; ++q) t[q] *= inv;
     ln_sv = ref.ln_s(vm, sv);
@@ -234,7 +234,7 @@ struct SlotWave {
     else {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        if (q * 64 < a.K && t[q] != 0.f && inside(a, q, c0, n)) part += slot_term(t[q], val[q], vm, ln_sv, xk[q], s.m, ln_s, a.temperature);
+        if (q * 64 < a.K && t[q] != 0.f && inside(a, q, c0, n)) part += slot_term(t[q], val[q], vm, ln_sv, xk[q], s.m, ln_s, a.inv_t);
     }
     return group_sum<64>(part);
   }
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(64) void ds_wave_kernel(DsArgs a, const T* __restri
     if constexpr (MODE != 0) {
       T* out = dx + a.vo.base(r);
       const RowRef ref(s.m, a.c2);
-      const float inv_s = s.s == 0.f ? 0.f : 1.f / s.s, co = a.coef(w), dense = co * q.sum * inv_s;
+      const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * q.sum * inv_s;
       reg.fresh();
       if (q.sum == 0.f) reg.map_store(out, C, lane, [](float) { return 0.f; });
       else {
@@ -426,7 +426,7 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
   const RowRef ref(s.m, a.c2);
   const float sum_t = joined[2];
   if constexpr (MODE != 0) {
-    const float inv_s = s.s == 0.f ? 0.f : 1.f / s.s, co = a.coef(w), dense = co * sum_t * inv_s;
+    const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * sum_t * inv_s;
     reg.fresh();
     if (sum_t == 0.f) reg.map_store(out + c0, n, lane, [](float) { return 0.f; });
     else {
@@ -484,20 +484,21 @@ template <int KS> struct ThreadTeacher {
       each(a, r, [&](float val, int) { sv += ex2(ref.z(val)); });
     }
     vm = best;
-    inv = bad ? NAN : sv == 0.f ? 0.f : 1.f / sv;
+    inv = bad ? NAN : sv == 0.f ? 0.f : rcp(sv);
     ln_sv = w != 0.f ? ref.ln_s(vm, sv) : 0.f;
     sum = bad || !(sv >= 0.f) ? NAN : sv == 0.f ? 0.f : 1.f;
   }
   __device__ __forceinline__ float t(float val) const { return ex2(ref.z(val)) * inv; }
 };
-template <typename T, int KS> __device__ __forceinline__ float thread_kl(const DsArgs& a, long long r, const T* row, long long sc,
-                                                                         const ThreadTeacher<KS>& q, const RowStat& s) {
+// at(c): where the student's class c lies
+template <int KS, typename F> __device__ __forceinline__ float thread_kl(const DsArgs& a, long long r, const ThreadTeacher<KS>& q, const RowStat& s,
+                                                                         F at) {
   if (!(q.sum == q.sum)) return NAN;
   const float ln_s = s.s == 0.f ? 0.f : RowRef(s.m, a.c2).ln_s(s.m, s.s);      // no class left: ln p = -inf
   float kl = 0.f;
   q.each(a, r, [&](float val, int cls) {
     const float t = q.t(val);
-    if (t != 0.f) kl += slot_term(t, val, q.vm, q.ln_sv, ld(row + cls * sc), s.m, ln_s, a.temperature);
+    if (t != 0.f) kl += slot_term(t, val, q.vm, q.ln_sv, ld(at(cls)), s.m, ln_s, a.inv_t);
   });
   return kl;
 }
@@ -506,34 +507,33 @@ __device__ __forceinline__ double wave_total(double v) {
   return v;
 }
 
-// MODE 0: loss, 1: gradient with statistics given, 2: both.  Up to 64 classes; what the teacher holds of each class is added up
-// in LDS (tab), so that a class named twice costs nothing and every gradient is rounded once.
+// MODE 0: loss, 1: gradient with statistics given, 2: both.  Up to 64 classes.  A thread's row lies in LDS as well (tab, [C][64]:
+// no bank is asked twice): first the logits, out of which the slots pick theirs (from memory, apart, 64 classes are 64 lines),
+// then what the teacher holds of each class, so that a class named twice costs nothing and every gradient is rounded once.
 template <typename T, int CREG, bool STAGED, int MODE, int KS>
 __global__ __launch_bounds__(64) void ds_thread_kernel(DsArgs a, const T* __restrict__ x, T* __restrict__ dx, bool wide) {
   extern __shared__ __align__(16) char lds[];
   constexpr int E = 16 / sizeof(T);
-  const int lane = threadIdx.x, C = a.v.C;
+  const int lane = threadIdx.x, C = a.v.C, so = (int)a.v.so;
   float* tab = reinterpret_cast<float*>(lds);                                     // [C][64]
-  T* tile = reinterpret_cast<T*>(lds + (MODE ? (size_t)C * 64 * 4 : 0));
-  T* res = tile + (64 * (int)a.v.so + E - 1) / E * E;                              // STAGED, MODE > 0: the gradient on its way out
+  T* tile = reinterpret_cast<T*>(lds + (MODE != 0 || !STAGED ? (size_t)C * 64 * 4 : 0));
+  T* res = tile + (64 * so + E - 1) / E * E;                                       // STAGED, MODE > 0: the gradient on its way out
   const long long blocks = (a.rows + 63) / 64;
   double total = 0.0;
   for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
     const long long r = b * 64 + lane;
     const int here = (int)min(64ll, a.rows - b * 64);
-    const T* row;
-    if (STAGED) {
+    if constexpr (STAGED) {
       __syncthreads();
-      copy_to_lds(tile, x + b * 64 * a.v.so, (here - 1) * (int)a.v.so + C);
+      copy_to_lds(tile, x + b * 64 * so, (here - 1) * so + C);
       __syncthreads();
-      row = tile + lane * (int)a.v.so;
-    } else {
-      row = x + (lane < here ? a.v.base(r) : 0);
     }
-    const long long sc = STAGED ? 1 : a.v.sc;
+    const ApartRows from(a.v, b * 64, lane);
+    const auto at = [&](int c) { return STAGED ? tile + lane * so + c : from.at(x, c * a.v.sc); };
     if (lane < here) {
       float v[CREG];
-      load_classes<T, CREG, STAGED>(v, row, sc, C, wide);  // on its way while the slots are
+      if (STAGED && wide) load_classes_wide<T, CREG>(v, tile + lane * so, C);
+      else load_classes<T, CREG>(v, C, at);                // on its way while the slots are
       const float w = a.weight_of(r);
       const ThreadTeacher<KS> q(a, r, w);
       const bool on = w != 0.f && q.sum != 0.f;
@@ -543,24 +543,37 @@ __global__ __launch_bounds__(64) void ds_thread_kernel(DsArgs a, const T* __rest
         else s = thread_row_stat<CREG, false>(v, C, a.c2);
       }
       if (MODE != 1) {
-        if (on) total += (double)w * a.temperature * a.temperature * thread_kl(a, r, row, sc, q, s);
+        if (on) {
+          float kl;
+          if constexpr (STAGED) kl = thread_kl(a, r, q, s, [&](int c) { return tile + lane * so + c; });
+          else {
+            const int n = renew_uniform(C);
+#pragma unroll
+            for (int c = 0; c < CREG; ++c)
+              if (c < n) tab[c * 64 + lane] = v[c];
+            kl = thread_kl(a, r, q, s, [&](int c) { return tab + c * 64 + lane; });
+          }
+          total += (double)w * a.temperature * a.temperature * kl;
+        }
         if (a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
       }
       if constexpr (MODE != 0) {
-        T* out = STAGED ? res + lane * C : dx + a.vo.base(r);
-        const long long osc = STAGED ? 1 : a.vo.sc;
+        const ApartRows to_rows(a.vo, b * 64, lane);
+        const auto to = [&](int c) { return STAGED ? res + lane * C + c : to_rows.at(dx, c * a.vo.sc); };
         if (!on) {
-          for (int c = 0; c < C; ++c) st(out + c * osc, 0.f);
+          for (int c = 0; c < C; ++c) *to(c) = (T)0.f;
         } else {
           const RowRef ref(s.m, a.c2);
-          const float inv_s = s.s == 0.f ? 0.f : 1.f / s.s, co = a.coef(w), scale_p = q.sum * inv_s;
+          const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * q.sum * inv_s;
+#pragma unroll 8
           for (int c = 0; c < C; ++c) tab[c * 64 + lane] = 0.f;
           q.each(a, r, [&](float val, int cls) {
-            if (cls >= 0 && cls < C) tab[cls * 64 + lane] += q.t(val);
+            if (cls >= 0 && cls < C) tab[cls * 64 + lane] -= q.t(val);
           });
+          const int n = renew_uniform(C);
 #pragma unroll
           for (int c = 0; c < CREG; ++c)
-            if (c < C) st(out + c * osc, co * (scale_p * ex2(ref.z(v[c])) - tab[c * 64 + lane]));
+            if (c < n) *to(c) = (T)fmaf(co, tab[c * 64 + lane], dense * ex2(ref.z(v[c])));
         }
       }
     }
@@ -593,13 +606,13 @@ template <typename T, int MODE> __global__ __launch_bounds__(64) void ds_walk_ke
       else s = walk_row_stat(row, sc, C, a.c2);
     }
     if (MODE != 1) {
-      if (on) total += (double)w * a.temperature * a.temperature * thread_kl(a, r, row, sc, q, s);
+      if (on) total += (double)w * a.temperature * a.temperature * thread_kl(a, r, q, s, [&](int c) { return row + c * sc; });
       if (a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
     }
     if constexpr (MODE != 0) {
       T* out = dx + a.vo.base(r);
       const RowRef ref(s.m, a.c2);
-      const float inv_s = s.s == 0.f ? 0.f : 1.f / s.s, co = a.coef(w), dense = co * q.sum * inv_s;
+      const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * q.sum * inv_s;
       for (int c0 = 0; c0 < C; c0 += 8) {
         float v[8];
 #pragma unroll
@@ -654,7 +667,7 @@ template <typename T, int MODE> __global__ __launch_bounds__(256) void ds_any_ke
     if constexpr (MODE != 0) {
       T* out = dx + a.vo.base(r);
       const RowRef ref(s.m, a.c2);
-      const float inv_s = s.s == 0.f ? 0.f : 1.f / s.s, co = a.coef(w), dense = co * q.sum * inv_s;
+      const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * q.sum * inv_s;
       for (int c = lane; c < C; c += 256) st(out + c * a.vo.sc, on ? dense * ex2(ref.z(ld(row + c * a.v.sc))) : 0.f);
       __syncthreads();
       if (on) group_fix<T, 256>(a, row, out, lane, q.sum, co, ref, inv_s, t_of, c_of);
@@ -702,7 +715,7 @@ static DsArgs ds_args(const uh_class_view* view, const uh_class_view* out, const
   a.v = uh_row_view(view), a.vo = uh_row_view(out);
   a.rows = view->outer * view->inner;
   a.value = s->value, a.index = s->index, a.K = s->slots, a.value_dtype = s->value_dtype, a.index_bytes = s->index_bytes;
-  a.weight = weight, a.temperature = temperature, a.c2 = (float)(1.4426950408889634 / (double)temperature);
+  a.weight = weight, a.temperature = temperature, a.inv_t = 1.f / temperature, a.c2 = (float)(1.4426950408889634 / (double)temperature);
   a.grad_scale = 0.f, a.gout = nullptr, a.stats = nullptr, a.partial = nullptr;
   return a;
 }
@@ -717,7 +730,7 @@ struct DsPlan {
 static DsPlan ds_plan(const RowView& v, const RowView* vo, long long rows, int dtype) {
   DsPlan p;
   const int elem = uh_elem_bytes(dtype);
-  p.path = uh_class_path(v, vo, rows);
+  p.path = uh_class_path(v, vo, rows, dtype);
   p.parts = p.path == PATH_GROUP && (long long)v.C * elem > 8192;
   p.cut = p.parts ? uh_row_cut(rows, v.C, dtype, 65536) : RowCut{1, v.C};
   const size_t sums = p.parts && rows * p.cut.parts > UH_GRID_WAVES ? rows * p.cut.parts : UH_GRID_WAVES;
@@ -739,7 +752,7 @@ template <typename T, int MODE> static long long ds_launch(const DsArgs& a, cons
   const unsigned waves = uh_grid((rows + 63) / 64, UH_GRID_WAVES), blocks = uh_grid(rows, UH_GRID_WAVES);
   if (p.path == PATH_STAGED || p.path == PATH_APART) {
     const bool staged = p.path == PATH_STAGED, wide = staged && (a.v.so * sizeof(T)) % 16 == 0;
-    const size_t lds = (MODE ? (size_t)C * 64 * 4 : 0) + (staged ? ((64 * a.v.so + E - 1) / E * E + (MODE ? 64 * C : 0)) * sizeof(T) : 0);
+    const size_t lds = (MODE != 0 || !staged ? (size_t)C * 64 * 4 : 0) + (staged ? ((64 * a.v.so + E - 1) / E * E + (MODE ? 64 * C : 0)) * sizeof(T) : 0);
 #define UH_GO3(R, ST, KS) hipLaunchKernelGGL((ds_thread_kernel<T, R, ST, MODE, KS>), dim3(waves), dim3(64), lds, s, a, x, dx, wide)
 #define UH_GO2(R, ST) do { if (a.K <= 4) UH_GO3(R, ST, 4); else UH_GO3(R, ST, 0); } while (0)
 #define UH_GO(ST) do { if (C <= 16) UH_GO2(16, ST); else if (C <= 32) UH_GO2(32, ST); else UH_GO2(64, ST); } while (0)
