@@ -67,7 +67,7 @@ __global__ __launch_bounds__(64) void lp_group_kernel(LpArgs a, const T* __restr
     }
     RowRegs<T, G, NV> reg;
     const T* row = x + (there ? a.v.base(r) : 0);
-    if (!off) reg.load(row, C, lane);
+    if (!off) reg.load(row, 0, C, lane);
     float vmax[TOP ? NV : 1];
     const float lm = off ? -INFINITY : reg.template lane_max<TOP ? NV : 0>(C, vmax);
     RowStat s;
@@ -140,8 +140,8 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(LpArgs a, const T* __restr
   }
   const int n = min(part_len, a.v.C - c0);
   RowRegs<T, 256, NV> reg;
-  const T* row = x + a.v.base(r) + c0;
-  reg.template load<true>(row, n, lane);
+  const T* row = x + a.v.base(r);
+  reg.template load<true>(row, c0, n, lane);
   float vmax[TOP ? NV : 1];
   const float lm = reg.template lane_max<TOP ? NV : 0>(n, vmax);
   RowStat s;
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(LpArgs a, const T* __restr
       else out[k] = key;
     };
     if (found > TopBuf<256>::CAP) {                        // too many equal values
-      group_rounds<T, 256>(row, n, lane, c0, a.top, red, emit);
+      group_rounds<T, 256>(row + c0, n, lane, c0, a.top, red, emit);
       found = a.top;                                       // those left over are 0: below any bound
     } else if (parts == 1 || found > keep) {
       group_rank<256>(tb.list, found, lane, a.top, &tb.left, emit);
@@ -404,19 +404,19 @@ __global__ __launch_bounds__(G > 64 ? G : 64) void lp_bwd_group_kernel(LpBwd k, 
     const long long r = b * RPB + threadIdx.x / G;
     if (r >= k.rows) continue;
     const LpCoef q(k, r);
-    T* out = dx + k.vo.base(r) + c0;
+    T* out = dx + k.vo.base(r);
     RowRegs<T, G, NV> reg;
     if (q.off) {
-      reg.map_store(out, n, lane, [](float) { return 0.f; });
+      reg.map_store(out, c0, n, lane, [](float) { return 0.f; });
       continue;
     }
-    const T* row = x + k.v.base(r) + c0;
-    reg.template load<true>(row, n, lane);
+    const T* row = x + k.v.base(r);
+    reg.load(row, c0, n, lane);
     const RowRef ref(q.m, k.c2);
-    reg.map_store(out, n, lane, [&](float v) { return q.of(ref, v); });
+    reg.map_store(out, c0, n, lane, [&](float v) { return q.of(ref, v); });
     // the label's class once more, by the lane that has just written it
     const int at = q.label - c0;
-    if (at >= 0 && at < n && (at / RowRegs<T, G, NV>::E) % G == lane) st(out + at, q.of(ref, ld(row + at)) + q.own);
+    if (at >= 0 && at < n && (at / RowRegs<T, G, NV>::E) % G == lane) st(out + q.label, q.of(ref, ld(row + q.label)) + q.own);
   }
 }
 

@@ -234,6 +234,14 @@ __device__ __forceinline__ long long load_int(const void* p, int bytes, long lon
   return bytes == 8 ? ((const long long*)p)[i] : (long long)((const int*)p)[i];
 }
 
+// Keeps the compiler from working out every `c < C` of an unrolled sweep ahead of it, or from
+// keeping them for the next (two scalar registers each, spilled to vector registers).
+__device__ __forceinline__ int renew_uniform(int C) {
+  C = __builtin_amdgcn_readfirstlane(C);
+  asm volatile("" : "+s"(C));
+  return C;
+}
+
 // ---- a row in the registers of a group of lanes ------------------------------------------------------------------------------
 // 16 bytes wherever an element may lie: rows of odd sizes start anywhere (the hardware takes element-aligned vectors)
 template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Loose16 { uint32_t w[4]; };
@@ -256,17 +264,24 @@ template <typename T, int G, int NV> struct RowRegs {
     const int e = (r * G + lane) * E;
     return e + E <= n ? e : n - E;
   }
-  template <bool ONCE = false> __device__ __forceinline__ void load(const T* __restrict__ p, int n, int lane) {
+  template <bool ONCE> __device__ __forceinline__ void fetch(int r, const char* p) {
+    const LooseVec<T>* q = reinterpret_cast<const LooseVec<T>*>(p);
+    const LooseVec<T> u = ONCE ? __builtin_nontemporal_load(q) : *q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[r][i] = u[i];
+  }
+  // elements c0 .. c0 + n of the row at p (the same for all lanes of a wave where G >= 64: one scalar address, and an offset of
+  // 32 bits a vector); n >= E or c0 >= E
+  template <bool ONCE = false> __device__ __forceinline__ void load(const T* __restrict__ p, int c0, int n, int lane) {
+    const uint32_t off = (uint32_t)(c0 + lane * E) * (uint32_t)sizeof(T);
+    n = renew_uniform(n);
 #pragma unroll
     for (int r = 0; r < NV; ++r)
-      if (r * G * E < n) {
-        const int e = (r * G + lane) * E;
-        if (e < n) {
-          const LooseVec<T>* q = reinterpret_cast<const LooseVec<T>*>(p + first(r, lane, n));
-          const LooseVec<T> u = ONCE ? __builtin_nontemporal_load(q) : *q;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[r][i] = u[i];
-        } else {
+      if ((r + 1) * G * E <= n) {
+        fetch<ONCE>(r, (const char*)p + r * G * 16 + (size_t)off);
+      } else if (r * G * E < n) {
+        if ((r * G + lane) * E < n) fetch<ONCE>(r, (const char*)p + (size_t)((uint32_t)(c0 + first(r, lane, n)) * (uint32_t)sizeof(T)));
+        else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) w[r][i] = neg_inf();
         }
@@ -311,6 +326,7 @@ template <typename T, int G, int NV> struct RowRegs {
   // the largest element, and (NM = NV) that of every vector
   template <int NM = 0> __device__ __forceinline__ float lane_max(int n, float* vmax = nullptr) const {
     float m = -INFINITY;
+    n = renew_uniform(n);
 #pragma unroll
     for (int r = 0; r < NV; ++r)
       if (r * G * E < n) {
@@ -331,6 +347,7 @@ template <typename T, int G, int NV> struct RowRegs {
   // s and (ENT) t of a lane's elements, even and odd ones apart.  Without CLAMP a class of -inf makes t a NaN; the -inf that
   // fill the row's last vectors do not.
   template <bool ENT, bool CLAMP = false> __device__ __forceinline__ void add_sums(const RowRef& ref, int n, float& s0, float& s1, float& t0, float& t1) const {
+    n = renew_uniform(n);
 #pragma unroll
     for (int r = 0; r < NV; ++r)
       if (r * G * E < n) {
@@ -353,31 +370,38 @@ template <typename T, int G, int NV> struct RowRegs {
     add_sums<ENT, CLAMP>(ref, n, s0, s1, t0, t1);
     s = s0 + s1, t = t0 + t1;
   }
-  // f(x) of every element to out[0 .. n)
-  template <typename F> __device__ __forceinline__ void map_store(T* __restrict__ out, int n, int lane, F f) const {
+  // f(x) of every element to out[c0 .. c0 + n)
+  template <typename F> __device__ __forceinline__ void map_store(T* __restrict__ out, int c0, int n, int lane, F f) const {
+    const uint32_t off = (uint32_t)(c0 + lane * E) * (uint32_t)sizeof(T);
+    n = renew_uniform(n);
 #pragma unroll
-    for (int r = 0; r < NV; ++r)
-      if (r * G * E < n) {
+    for (int r = 0; r < NV; ++r) {
+      if ((r + 1) * G * E <= n) {
+        put(r, (char*)out + r * G * 16 + (size_t)off, f);
+      } else if (r * G * E < n) {
         const int e = (r * G + lane) * E;
-        if (e + E <= n) {
-          Loose16<T> u;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if constexpr (sizeof(T) == 4) u.w[i] = __float_as_uint(f(get(r, i)));
-            else {
-              typedef __attribute__((ext_vector_type(2))) T T2;
-              const T2 v = {(T)f(get(r, 2 * i)), (T)f(get(r, 2 * i + 1))};
-              u.w[i] = __builtin_bit_cast(uint32_t, v);
-            }
-          }
-          *reinterpret_cast<Loose16<T>*>(out + e) = u;
-        } else if (e < n) {
+        if (e + E <= n) put(r, (char*)out + r * G * 16 + (size_t)off, f);
+        else if (e < n) {
 #pragma unroll
           for (int j = 0; j < E; ++j)
-            if (n - E + j >= e) out[n - E + j] = (T)f(get(r, j));
+            if (n - E + j >= e) out[c0 + n - E + j] = (T)f(get(r, j));
         }
-        __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  template <typename F> __device__ __forceinline__ void put(int r, char* p, F f) const {
+    Loose16<T> u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) u.w[i] = __float_as_uint(f(get(r, i)));
+      else {
+        typedef __attribute__((ext_vector_type(2))) T T2;
+        const T2 v = {(T)f(get(r, 2 * i)), (T)f(get(r, 2 * i + 1))};
+        u.w[i] = __builtin_bit_cast(uint32_t, v);
+      }
+    }
+    *reinterpret_cast<Loose16<T>*>(p) = u;
   }
 };
 
@@ -396,13 +420,6 @@ __device__ __forceinline__ void group_sums(RowRegs<T, G, NV>& x, const RowRef& r
     Red<G>::sum2(s2, t2, red);
     if (again) s.t = t2;
   }
-}
-
-// Keeps the compiler from working out every `c < C` of an unrolled sweep ahead of it (64 scalar registers, spilled to vectors).
-__device__ __forceinline__ int renew_uniform(int C) {
-  C = __builtin_amdgcn_readfirstlane(C);
-  asm volatile("" : "+s"(C));
-  return C;
 }
 
 // Inside a loop over rows: keeps the compiler from carrying every vector's place in a row from turn to turn (two registers
@@ -609,6 +626,7 @@ __device__ __forceinline__ int group_candidates(RowRegs<T, G, NV>& x, int n, int
   }
   const float cut = low ? unorder32(low) : -3.402823466e38f;
   x.fresh();
+  n = renew_uniform(n);
   if (__any(mine != 0 && mine >= low)) {                     // one look per vector; its few hits are placed by ballots
 #pragma unroll
     for (int r = 0; r < NV; ++r)

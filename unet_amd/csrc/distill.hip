@@ -117,7 +117,7 @@ __global__ __launch_bounds__(64) void ds_quad_kernel(DsArgs a, const T* __restri
     const bool off = w == 0.f;
     const T* row = x + (there ? a.v.base(r) : 0);
     RowRegs<T, 16, NV> reg;
-    if (!off) reg.load(row, C, lane);
+    if (!off) reg.load(row, 0, C, lane);
     const Teacher q = group_teacher<16>(a, r, lane, off, t_of, c_of, red);
     RowStat s{0.f, 0.f, 0.f};
     if constexpr (MODE == 1) {
@@ -140,9 +140,9 @@ __global__ __launch_bounds__(64) void ds_quad_kernel(DsArgs a, const T* __restri
         const RowRef ref(s.m, a.c2);
         const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * q.sum * inv_s;
         reg.fresh();
-        if (off || q.sum == 0.f) reg.map_store(out, C, lane, [](float) { return 0.f; });
+        if (off || q.sum == 0.f) reg.map_store(out, 0, C, lane, [](float) { return 0.f; });
         else {
-          reg.map_store(out, C, lane, [&](float v) { return dense * ex2(ref.z(v)); });
+          reg.map_store(out, 0, C, lane, [&](float v) { return dense * ex2(ref.z(v)); });
           group_fix<T, 16>(a, row, out, lane, q.sum, co, ref, inv_s, t_of, c_of);
         }
       }
@@ -261,14 +261,14 @@ __global__ __launch_bounds__(64) void ds_wave_kernel(DsArgs a, const T* __restri
     const float w = a.weight_of(r);
     RowRegs<T, 64, NV> reg;
     if (w == 0.f) {
-      if (MODE != 0) reg.map_store(dx + a.vo.base(r), C, lane, [](float) { return 0.f; });
+      if (MODE != 0) reg.map_store(dx + a.vo.base(r), 0, C, lane, [](float) { return 0.f; });
       if (MODE != 1 && a.stats && lane == 0) { a.stats[2 * r] = 0.f; a.stats[2 * r + 1] = 0.f; }
       continue;
     }
     const T* row = x + a.v.base(r);
     SlotWave q;
     q.load(a, r, lane);
-    reg.load(row, C, lane);
+    reg.load(row, 0, C, lane);
     q.softmax(a, row, 0, C, lane, t_of, c_of, MODE != 0);
     RowStat s{0.f, 0.f, 0.f};
     if constexpr (MODE == 1) {
@@ -288,9 +288,9 @@ __global__ __launch_bounds__(64) void ds_wave_kernel(DsArgs a, const T* __restri
       const RowRef ref(s.m, a.c2);
       const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * q.sum * inv_s;
       reg.fresh();
-      if (q.sum == 0.f) reg.map_store(out, C, lane, [](float) { return 0.f; });
+      if (q.sum == 0.f) reg.map_store(out, 0, C, lane, [](float) { return 0.f; });
       else {
-        reg.map_store(out, C, lane, [&](float v) { return dense * ex2(ref.z(v)); });
+        reg.map_store(out, 0, C, lane, [&](float v) { return dense * ex2(ref.z(v)); });
         q.fix(a, out, 0, C, co, ref, inv_s);
       }
     }
@@ -315,7 +315,7 @@ struct DsParts {
 };
 
 // statistics of a part as 256 lanes make them, by one wave
-template <typename T, int NV> __device__ __attribute__((noinline)) RowStat alone_part_stat(const T* __restrict__ p, int n, float c2) {
+template <typename T, int NV> __device__ __attribute__((noinline)) RowStat alone_part_stat(const T* __restrict__ p, int c0, int n, float c2) {
   constexpr int E = 16 / sizeof(T);
   const int lane = threadIdx.x & 63;
   float m = -INFINITY;
@@ -324,7 +324,7 @@ template <typename T, int NV> __device__ __attribute__((noinline)) RowStat alone
       const int left = n - r * 256 * E;
       if (left <= 0) continue;
       RowRegs<T, 256, 1> v;
-      v.load(p + r * 256 * E, left, lane + 64 * w);
+      v.load(p, c0 + r * 256 * E, left, lane + 64 * w);
       m = fmaxf(m, v.lane_max(left));
     }
   m = group_max<64>(m);
@@ -337,7 +337,7 @@ template <typename T, int NV> __device__ __attribute__((noinline)) RowStat alone
       const int left = n - r * 256 * E;
       if (left <= 0) continue;
       RowRegs<T, 256, 1> v;
-      v.load(p + r * 256 * E, left, lane + 64 * w);
+      v.load(p, c0 + r * 256 * E, left, lane + 64 * w);
       v.template add_sums<false>(ref, left, s0, s1, t0, t1);
     }
     const float sw = group_sum<64>(s0 + s1);
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
   T* out = MODE != 0 ? dx + a.vo.base(r) : nullptr;
   RowRegs<T, 256, NV> reg;
   if (w == 0.f) {
-    if (MODE != 0) reg.map_store(out + c0, n, lane, [](float) { return 0.f; });
+    if (MODE != 0) reg.map_store(out, c0, n, lane, [](float) { return 0.f; });
     if (MODE != 1 && lane == 0) {
       if (MODE == 2 || part == 0) a.partial[MODE == 2 ? r * p.parts + part : r] = 0.0;
       if (MODE == 0 && part == 0 && a.stats) { a.stats[2 * r] = 0.f; a.stats[2 * r + 1] = 0.f; }
@@ -373,7 +373,7 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
   SlotWave q;
   const bool slots = first && (MODE != 0 || part == 0);
   if (slots) q.load(a, r, wl);
-  reg.template load<MODE == 2>(row + c0, n, lane);
+  reg.template load<MODE == 2>(row, c0, n, lane);
   if (slots) {
     // the loss alone is the first part's to work out; for a gradient every part has its classes' share of it
     if (MODE == 0) q.softmax(a, row, 0, a.v.C, wl, t_of, c_of, false);
@@ -408,7 +408,7 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
         }
         for (unsigned long long left = __ballot(other && word == UH_NO_WORD); left; left &= left - 1) {
           const int who = __ffsll(left) - 1, at = who * p.len;
-          const RowStat u = alone_part_stat<T, NV>(row + at, min(p.len, a.v.C - at), a.c2);
+          const RowStat u = alone_part_stat<T, NV>(row, at, min(p.len, a.v.C - at), a.c2);
           if (wl == who) word = (unsigned long long)__float_as_uint(u.s) << 32 | __float_as_uint(u.m);
         }
         RowStat j{__uint_as_float((uint32_t)word), wl < p.parts ? __uint_as_float((uint32_t)(word >> 32)) : 0.f, 0.f};
@@ -428,9 +428,9 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
   if constexpr (MODE != 0) {
     const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * sum_t * inv_s;
     reg.fresh();
-    if (sum_t == 0.f) reg.map_store(out + c0, n, lane, [](float) { return 0.f; });
+    if (sum_t == 0.f) reg.map_store(out, c0, n, lane, [](float) { return 0.f; });
     else {
-      reg.map_store(out + c0, n, lane, [&](float v) { return dense * ex2(ref.z(v)); });
+      reg.map_store(out, c0, n, lane, [&](float v) { return dense * ex2(ref.z(v)); });
       __syncthreads();                                     // another wave may have written the class
       if (first) q.fix(a, out, c0, n, co, ref, inv_s);
     }
@@ -466,15 +466,19 @@ template <int KS> struct ThreadTeacher {
       }
     }
   }
-  __device__ __forceinline__ ThreadTeacher(const DsArgs& a, long long r, float w) : ref(0.f, a.c2) {
+  __device__ __forceinline__ ThreadTeacher(const DsArgs& a) : ref(0.f, a.c2) {}
+  // asks for the slots; what comes of them follows in softmax
+  __device__ __forceinline__ void fetch(const DsArgs& a, long long r) {
+    if constexpr (KS > 0) {
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        if (k < a.K) a.slot(r, k, val_[k], cls_[k]);
+    }
+  }
+  __device__ __forceinline__ void softmax(const DsArgs& a, long long r, float w) {
     float best = -INFINITY, sv = 0.f;
     bool bad = false;
     if (w != 0.f) {
-      if constexpr (KS > 0) {
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-          if (k < a.K) a.slot(r, k, val_[k], cls_[k]);
-      }
       each(a, r, [&](float val, int cls) {
         bad |= val != val || cls >= a.v.C;
         best = fmaxf(best, val);
@@ -523,6 +527,12 @@ __global__ __launch_bounds__(64) void ds_thread_kernel(DsArgs a, const T* __rest
   for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
     const long long r = b * 64 + lane;
     const int here = (int)min(64ll, a.rows - b * 64);
+    ThreadTeacher<KS> q(a);
+    float w = 0.f;
+    if (lane < here) {
+      w = a.weight_of(r);
+      q.fetch(a, r);
+    }
     if constexpr (STAGED) {
       __syncthreads();
       copy_to_lds(tile, x + b * 64 * so, (here - 1) * so + C);
@@ -533,9 +543,8 @@ __global__ __launch_bounds__(64) void ds_thread_kernel(DsArgs a, const T* __rest
     if (lane < here) {
       float v[CREG];
       if (STAGED && wide) load_classes_wide<T, CREG>(v, tile + lane * so, C);
-      else load_classes<T, CREG>(v, C, at);                // on its way while the slots are
-      const float w = a.weight_of(r);
-      const ThreadTeacher<KS> q(a, r, w);
+      else load_classes<T, CREG>(v, C, at);
+      q.softmax(a, r, w);
       const bool on = w != 0.f && q.sum != 0.f;
       RowStat s{0.f, 0.f, 0.f};
       if (on) {
@@ -598,7 +607,8 @@ template <typename T, int MODE> __global__ __launch_bounds__(64) void ds_walk_ke
     if (r >= a.rows) continue;
     const T* row = x + a.v.base(r);
     const float w = a.weight_of(r);
-    const ThreadTeacher<0> q(a, r, w);
+    ThreadTeacher<0> q(a);
+    q.softmax(a, r, w);
     const bool on = w != 0.f && q.sum != 0.f;
     RowStat s{0.f, 0.f, 0.f};
     if (on) {
