@@ -73,6 +73,7 @@ __global__ __launch_bounds__(64) void lp_group_kernel(LpArgs a, const T* __restr
     RowStat s;
     s.m = group_max<G>(lm);
     if (s.m == -INFINITY) s.m = 0.f;
+    reg.fresh();
     group_sums<T, G, NV>(reg, RowRef(s.m, a.c2), C, s, red);
     float ln_s = 0.f;
     if (!off) {
@@ -143,11 +144,8 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(LpArgs a, const T* __restr
   const T* row = x + a.v.base(r);
   reg.template load<true>(row, c0, n, lane);
   float vmax[TOP ? NV : 1];
-  const float lm = reg.template lane_max<TOP ? NV : 0>(n, vmax);
-  RowStat s;
-  s.m = Red<256>::max_(lm, red);
-  if (s.m == -INFINITY) s.m = 0.f;
-  group_sums<T, 256, NV>(reg, RowRef(s.m, a.c2), n, s, red);
+  float lm;
+  const RowStat s = arriving_stat<T, 256, NV, true, TOP ? NV : 0>(reg, a.c2, n, lm, vmax, red);
   float ln_s = 0.f;
   if (parts == 1) {
     ln_s = RowRef(s.m, a.c2).ln_s(s.m, s.s);

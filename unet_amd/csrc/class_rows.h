@@ -73,6 +73,7 @@ __device__ __forceinline__ float rcp(float x) { return __builtin_amdgcn_rcpf(x);
 
 struct RowRef {           // the point and the scale a row's exponents are taken in
   float c, M;
+  __device__ __forceinline__ RowRef(float c_, float M_, int) : c(c_), M(M_) {}
   __device__ __forceinline__ RowRef(float m, float c2) : c(fabsf(m) >= 0x1p100f ? 0x1p-20f : c2), M(m * c) {}
   __device__ __forceinline__ float z(float x) const { return fmaf(x, c, -M); }
   __device__ __forceinline__ float ln_s(float m, float s) const { return (lg2(s) - fmaf(m, c, -M)) * UH_LN2; }
@@ -246,6 +247,11 @@ __device__ __forceinline__ int renew_uniform(int C) {
 // 16 bytes wherever an element may lie: rows of odd sizes start anywhere (the hardware takes element-aligned vectors)
 template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Loose16 { uint32_t w[4]; };
 
+struct Online {
+  float top, M, s0, s1, t;
+  __device__ __forceinline__ explicit Online(float c2) : top(-INFINITY), M(-0x1p99f * c2), s0(0.f), s1(0.f), t(0.f) {}
+};
+
 template <typename T> using LooseVec = __attribute__((ext_vector_type(4), aligned(sizeof(T)))) uint32_t;
 
 template <typename T, int G, int NV> struct RowRegs {
@@ -370,6 +376,37 @@ template <typename T, int G, int NV> struct RowRegs {
     add_sums<ENT, CLAMP>(ref, n, s0, s1, t0, t1);
     s = s0 + s1, t = t0 + t1;
   }
+  // Largest element, s and (ENT) t of a lane in one sweep that takes the vectors as they arrive: against the running maximum,
+  // not below -2^99, whose M is returned; a vector that raises it rescales what is summed.  vmax as in lane_max.
+  template <bool ENT, int NM> __device__ __forceinline__ void online(float c2, int n, Online& o, float* vmax) const {
+    n = renew_uniform(n);
+#pragma unroll
+    for (int r = 0; r < NV; ++r)
+      if (r * G * E < n) {
+        float v = online_vector<ENT>(r, c2, ENT && (r + 1) * G * E > n, o);
+        if (NM > 0) vmax[r] = v;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  }
+  template <bool ENT> __device__ __forceinline__ float online_vector(int r, float c2, bool clamp, Online& o) const {
+    float v = fmaxf(get(r, 0), get(r, 1));
+#pragma unroll
+    for (int j = 2; j < E; j += 2) v = max3(v, get(r, j), get(r, j + 1));
+    o.top = fmaxf(o.top, v);
+    const float M = fmaxf(o.top, -0x1p99f) * c2, d = o.M - M, f = ex2(d);
+    if (ENT) o.t = f * fmaf(o.s0 + o.s1, d, o.t);
+    o.s0 *= f, o.s1 *= f;
+    o.M = M;
+    const RowRef ref(c2, M, 0);
+    float t1 = 0.f;
+    if (clamp) add_vector<ENT, ENT>(r, ref, o.s0, o.s1, o.t, t1);
+    else add_vector<ENT, false>(r, ref, o.s0, o.s1, o.t, t1);
+    if (ENT) o.t += t1;
+    // now: terms left to be summed later would take registers of their own
+    if (ENT) asm volatile("" : "+v"(o.s0), "+v"(o.s1), "+v"(o.t), "+v"(o.top));
+    else asm volatile("" : "+v"(o.s0), "+v"(o.s1), "+v"(o.top));
+    return v;
+  }
   // f(x) of every element to out[c0 .. c0 + n)
   template <typename F> __device__ __forceinline__ void map_store(T* __restrict__ out, int c0, int n, int lane, F f) const {
     const uint32_t off = (uint32_t)(c0 + lane * E) * (uint32_t)sizeof(T);
@@ -405,21 +442,60 @@ template <typename T, int G, int NV> struct RowRegs {
   }
 };
 
-// s and t of a whole row.  The clamp of its exponents, one instruction of nine an element, is only for classes of -inf (0 times
-// -inf): rows that hold one are found by their NaN and summed again with it.
+// A maximum against which the running sums of `online` are of no use: all logits, or the largest, of a size that only the other
+// scale of RowRef takes.
+__device__ __forceinline__ bool beyond_online(float m) { return fabsf(m) >= 0x1p99f && m != -INFINITY; }
+
+// s and t of a row in registers, given its maximum.  The clamp of its exponents, one instruction of nine an element, is only for
+// classes of -inf (0 times -inf): rows that hold one are found by their NaN and summed again with it.
 template <typename T, int G, int NV>
 __device__ __forceinline__ void group_sums(RowRegs<T, G, NV>& x, const RowRef& ref, int n, RowStat& s, typename Red<G>::Buf& red) {
-  x.fresh();
   x.template lane_sums<true>(ref, n, s.s, s.t);
   Red<G>::sum2(s.s, s.t, red);
   const bool again = s.t != s.t && s.s == s.s;
   if (G >= 64 ? again : (bool)__any(again)) {
     float s2, t2;
-    x.fresh();
     x.template lane_sums<true, true>(ref, n, s2, t2);
     Red<G>::sum2(s2, t2, red);
     if (again) s.t = t2;
   }
+}
+// Statistics of a row (or part) in registers of a workgroup, whose loads may still be on their way: the sums are done while they
+// arrive, instead of after the last of them, when nothing would be on its way.  lane_top: the lane's largest.
+template <typename T, int G, int NV, bool ENT, int NM>
+__device__ __forceinline__ RowStat arriving_stat(RowRegs<T, G, NV>& x, float c2, int n, float& lane_top, float* vmax, typename Red<G>::Buf& red) {
+  Online o(c2);
+  x.template online<ENT, NM>(c2, n, o, vmax);
+  lane_top = o.top;
+  x.fresh();                                                 // once, ahead of the branches: in them it would copy the row
+  RowStat s;
+  s.m = Red<G>::max_(o.top, red);
+  if (s.m == -INFINITY) s.m = 0.f;
+  const RowRef ref(s.m, c2);
+  if (beyond_online(s.m)) {
+    if (ENT) group_sums<T, G, NV>(x, ref, n, s, red);
+    else {
+      x.template lane_sums<false>(ref, n, s.s, s.t);
+      s.s = Red<G>::sum_(s.s, red);
+    }
+    return s;
+  }
+  const float d = o.M - ref.M, f = ex2(d);
+  s.s = (o.s0 + o.s1) * f;
+  if (ENT) {
+    s.t = f * fmaf(o.s0 + o.s1, d, o.t);
+    Red<G>::sum2(s.s, s.t, red);
+    if (s.t != s.t && s.s == s.s) {                          // a class of -inf
+      float s2, t2;
+      x.template lane_sums<true, true>(ref, n, s2, t2);
+      Red<G>::sum2(s2, t2, red);
+      s.t = t2;
+    }
+  } else {
+    s.t = 0.f;
+    s.s = Red<G>::sum_(s.s, red);
+  }
+  return s;
 }
 
 // Inside a loop over rows: keeps the compiler from carrying every vector's place in a row from turn to turn (two registers

@@ -314,36 +314,42 @@ struct DsParts {
   unsigned long long* words;
 };
 
-// statistics of a part as 256 lanes make them, by one wave
-template <typename T, int NV> __device__ __attribute__((noinline)) RowStat alone_part_stat(const T* __restrict__ p, int c0, int n, float c2) {
+// Statistics of a part as 256 lanes make them (arriving_stat), by one wave, to the bit.  Kept small rather than fast: it stands
+// where a part of a row waits in registers.
+template <typename T> __device__ __forceinline__ RowStat alone_part_stat(const T* __restrict__ p, int c0, int n, float c2) {
   constexpr int E = 16 / sizeof(T);
   const int lane = threadIdx.x & 63;
+  RowRegs<T, 256, 1> v;
   float m = -INFINITY;
-  for (int r = 0; r < NV; ++r)
-    for (int w = 0; w < 4; ++w) {
-      const int left = n - r * 256 * E;
-      if (left <= 0) continue;
-      RowRegs<T, 256, 1> v;
-      v.load(p, c0 + r * 256 * E, left, lane + 64 * w);
-      m = fmaxf(m, v.lane_max(left));
-    }
+#pragma unroll 1
+  for (int at = 0; at < n * 4; at += 256 * E) {            // a quarter of the lanes a turn
+    const int first = at / (1024 * E) * 256 * E, w = at / (256 * E) % 4;
+    v.load(p, c0 + first, n - first, lane + 64 * w);
+    m = fmaxf(m, v.lane_max(n - first));
+  }
   m = group_max<64>(m);
   if (m == -INFINITY) m = 0.f;
   const RowRef ref(m, c2);
-  float s = 0.f;
+  float total = 0.f;
+#pragma unroll 1
   for (int w = 0; w < 4; ++w) {
-    float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f;
-    for (int r = 0; r < NV; ++r) {
-      const int left = n - r * 256 * E;
-      if (left <= 0) continue;
-      RowRegs<T, 256, 1> v;
-      v.load(p, c0 + r * 256 * E, left, lane + 64 * w);
-      v.template add_sums<false>(ref, left, s0, s1, t0, t1);
+    Online o(c2);
+#pragma unroll 1
+    for (int first = 0; first < n; first += 256 * E) {
+      v.load(p, c0 + first, n - first, lane + 64 * w);
+      if (beyond_online(m)) {
+        float t0 = 0.f, t1 = 0.f;
+        v.template add_sums<false>(ref, n - first, o.s0, o.s1, t0, t1);
+      } else {
+        v.template online_vector<false>(0, c2, false, o);
+      }
     }
-    const float sw = group_sum<64>(s0 + s1);
-    s = w == 0 ? sw : s + sw;
+    float s = o.s0 + o.s1;
+    if (!beyond_online(m)) s *= ex2(o.M - ref.M);
+    s = group_sum<64>(s);
+    total = w == 0 ? s : total + s;
   }
-  return RowStat{m, s == s ? s : NAN, 0.f};
+  return RowStat{m, total == total ? total : NAN, 0.f};
 }
 
 template <typename T, int NV, int MODE>
@@ -385,13 +391,9 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
     s.m = a.stats[2 * r], s.s = a.stats[2 * r + 1];
     __syncthreads();                                       // joined[2]
   } else {
-    s.m = Red<256>::max_(reg.lane_max(n), red);
-    if (s.m == -INFINITY) s.m = 0.f;
-    reg.fresh();
-    reg.template lane_sums<false>(RowRef(s.m, a.c2), n, s.s, s.t);
-    s.s = Red<256>::sum_(s.s, red);
+    float lane_top;
+    s = arriving_stat<T, 256, NV, false, 0>(reg, a.c2, n, lane_top, nullptr, red);
     if (s.s != s.s) s.s = NAN;                             // never the bits of UH_NO_WORD
-    s.t = 0.f;
     if (p.parts > 1) {
       unsigned long long* words = p.words + r * p.parts;
       if (lane == 0)
@@ -408,7 +410,7 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
         }
         for (unsigned long long left = __ballot(other && word == UH_NO_WORD); left; left &= left - 1) {
           const int who = __ffsll(left) - 1, at = who * p.len;
-          const RowStat u = alone_part_stat<T, NV>(row, at, min(p.len, a.v.C - at), a.c2);
+          const RowStat u = alone_part_stat<T>(row, at, min(p.len, a.v.C - at), a.c2);
           if (wl == who) word = (unsigned long long)__float_as_uint(u.s) << 32 | __float_as_uint(u.m);
         }
         RowStat j{__uint_as_float((uint32_t)word), wl < p.parts ? __uint_as_float((uint32_t)(word >> 32)) : 0.f, 0.f};
@@ -427,7 +429,6 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
   const float sum_t = joined[2];
   if constexpr (MODE != 0) {
     const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * sum_t * inv_s;
-    reg.fresh();
     if (sum_t == 0.f) reg.map_store(out, c0, n, lane, [](float) { return 0.f; });
     else {
       reg.map_store(out, c0, n, lane, [&](float v) { return dense * ex2(ref.z(v)); });
