@@ -142,7 +142,9 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(LpArgs a, const T* __restr
   const int n = min(part_len, a.v.C - c0);
   RowRegs<T, 256, NV> reg;
   const T* row = x + a.v.base(r);
-  reg.template load<true>(row, c0, n, lane);
+  // rows that no backward pass will read again go past the caches
+  if (!a.stats) reg.template load<true>(row, c0, n, lane);
+  else reg.load(row, c0, n, lane);
   float vmax[TOP ? NV : 1];
   float lm;
   const RowStat s = arriving_stat<T, 256, NV, true, TOP ? NV : 0>(reg, a.c2, n, lm, vmax, red);

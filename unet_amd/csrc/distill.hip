@@ -379,7 +379,9 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
   SlotWave q;
   const bool slots = first && (MODE != 0 || part == 0);
   if (slots) q.load(a, r, wl);
-  reg.template load<MODE == 2>(row, c0, n, lane);
+  // rows that no backward pass will read again go past the caches
+  if (MODE == 2 || (MODE == 0 && !a.stats)) reg.template load<true>(row, c0, n, lane);
+  else reg.load(row, c0, n, lane);
   if (slots) {
     // the loss alone is the first part's to work out; for a gradient every part has its classes' share of it
     if (MODE == 0) q.softmax(a, row, 0, a.v.C, wl, t_of, c_of, false);
@@ -738,12 +740,12 @@ struct DsPlan {
   bool parts;                     // rows by workgroups of 256
   size_t words_at, bytes;
 };
-static DsPlan ds_plan(const RowView& v, const RowView* vo, long long rows, int dtype) {
+static DsPlan ds_plan(const RowView& v, const RowView* vo, long long rows, int dtype, bool step) {
   DsPlan p;
   const int elem = uh_elem_bytes(dtype);
   p.path = uh_class_path(v, vo, rows, dtype);
   p.parts = p.path == PATH_GROUP && (long long)v.C * elem > 8192;
-  p.cut = p.parts ? uh_row_cut(rows, v.C, dtype, 65536) : RowCut{1, v.C};
+  p.cut = p.parts ? uh_row_cut(rows, v.C, dtype, step ? 65536 : 32768) : RowCut{1, v.C};
   const size_t sums = p.parts && rows * p.cut.parts > UH_GRID_WAVES ? rows * p.cut.parts : UH_GRID_WAVES;
   p.words_at = (sums * sizeof(double) + 15) / 16 * 16;
   p.bytes = p.words_at + (p.cut.parts > 1 ? (size_t)rows * p.cut.parts * 8 : 0);
@@ -821,7 +823,9 @@ template <int MODE> static long long ds_dispatch(const DsArgs& a, int dtype, con
 extern "C" size_t uh_topk_distill_workspace(const uh_class_view* view) {
   if (uh_check_view(view, "topk_distill_workspace") != UH_OK) return 0;
   const RowView v = uh_row_view(view);
-  return ds_plan(v, nullptr, view->outer * view->inner, view->dtype).bytes;
+  const size_t loss = ds_plan(v, nullptr, view->outer * view->inner, view->dtype, false).bytes;
+  const size_t step = ds_plan(v, nullptr, view->outer * view->inner, view->dtype, true).bytes;
+  return loss > step ? loss : step;
 }
 
 extern "C" int uh_topk_distill(const uh_class_view* view, const void* logits, const uh_slots* slots, const float* weight,
@@ -833,7 +837,7 @@ extern "C" int uh_topk_distill(const uh_class_view* view, const void* logits, co
              "topk_distill: null pointer or workspace of %zu bytes", workspace_bytes);
   DsArgs a = ds_args(view, view, slots, weight, temperature);
   a.stats = stats, a.partial = (double*)workspace;
-  const DsPlan p = ds_plan(a.v, nullptr, a.rows, view->dtype);
+  const DsPlan p = ds_plan(a.v, nullptr, a.rows, view->dtype, false);
   const long long n = ds_dispatch<0>(a, view->dtype, logits, nullptr, p, workspace, (hipStream_t)s);
   hipLaunchKernelGGL(ds_finish_kernel, dim3(1), dim3(1024), 0, (hipStream_t)s, n, (const double*)workspace, scale, loss);
   return uh_check_launch("topk_distill");
@@ -848,7 +852,7 @@ extern "C" int uh_topk_distill_bwd(const uh_class_view* view, const uh_class_vie
   UH_REQUIRE(gout && stats && dlogits, "topk_distill_bwd: null pointer");
   DsArgs a = ds_args(view, out_view, slots, weight, temperature);
   a.gout = gout, a.grad_scale = (float)scale, a.stats = const_cast<float*>(stats);
-  const DsPlan p = ds_plan(a.v, &a.vo, a.rows, view->dtype);
+  const DsPlan p = ds_plan(a.v, &a.vo, a.rows, view->dtype, false);
   ds_dispatch<1>(a, view->dtype, logits, dlogits, p, nullptr, (hipStream_t)s);
   return uh_check_launch("topk_distill_bwd");
 }
@@ -864,7 +868,7 @@ extern "C" int uh_topk_distill_step(const uh_class_view* view, const uh_class_vi
              "topk_distill_step: null pointer or workspace of %zu bytes", workspace_bytes);
   DsArgs a = ds_args(view, out_view, slots, weight, temperature);
   a.grad_scale = (float)(scale * (double)grad_scale), a.partial = (double*)workspace;
-  const DsPlan p = ds_plan(a.v, &a.vo, a.rows, view->dtype);
+  const DsPlan p = ds_plan(a.v, &a.vo, a.rows, view->dtype, true);
   const long long n = ds_dispatch<2>(a, view->dtype, logits, dlogits, p, workspace, (hipStream_t)s);
   hipLaunchKernelGGL(ds_finish_kernel, dim3(1), dim3(1024), 0, (hipStream_t)s, n, (const double*)workspace, scale, loss);
   return uh_check_launch("topk_distill_step");
