@@ -303,29 +303,34 @@ __global__ __launch_bounds__(64) void lp_walk_kernel(LpArgs a, const T* __restri
     for (int k = 0; k < a.top; ++k) a.write_top(r, k, 0.f, -1, 0.f, 0.f, 0.f);
     return;
   }
-  const RowStat s = walk_row_stat(row, a.v.sc, C, a.c2);
+  TopList<LIST ? LIST : 1> list;
+  const RowStat s = walk_row_stat(row, a.v.sc, C, a.c2, [&](const float (&v)[16], int c0) {
+    if constexpr (LIST > 0)
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (v[j] > list.v[LIST - 1]) list.insert(v[j], c0 + j);
+  });
   const float ln_s = a.write_row(r, l, a.is_class(l) ? ld(row + l * a.v.sc) : 0.f, s);
-  if constexpr (LIST > 0) {
-    float lv = 0.f;
-    int lc = 0;
-    for (int k0 = 0; k0 < a.top; k0 += LIST) {
-      TopList<LIST> list;
+  if constexpr (LIST > 0)
+    for (int k0 = 0;;) {
+#pragma unroll
+      for (int i = 0; i < LIST; ++i)
+        if (k0 + i < a.top) a.write_top(r, k0 + i, list.v[i], list.c[i], s.m, ln_s, s.s);
+      if ((k0 += LIST) >= a.top) break;
+      const float lv = list.v[LIST - 1];                           // more than a list holds: another walk for those behind it
+      const int lc = list.c[LIST - 1];
+      list = TopList<LIST>();
       for (int c0 = 0; c0 < C; c0 += 8) {
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = c0 + j < C ? ld(row + (c0 + j) * a.v.sc) : -INFINITY;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float u = k0 ? behind(v[j], c0 + j, lv, lc) : v[j];
+          const float u = behind(v[j], c0 + j, lv, lc);
           if (u > list.v[LIST - 1]) list.insert(u, c0 + j);
         }
       }
-#pragma unroll
-      for (int i = 0; i < LIST; ++i)
-        if (k0 + i < a.top) a.write_top(r, k0 + i, list.v[i], list.c[i], s.m, ln_s, s.s);
-      lv = list.v[LIST - 1], lc = list.c[LIST - 1];
     }
-  }
 }
 
 // ---- one workgroup per row, any strides ----------------------------------------------------------------------------------------

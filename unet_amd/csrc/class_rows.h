@@ -845,14 +845,24 @@ template <int CREG, bool ENT> __device__ __forceinline__ RowStat thread_row_stat
     }
   return RowStat{m, s, t};
 }
-// the same of a row of any length that one thread walks, eight classes at a time
-template <typename T> __device__ __forceinline__ RowStat walk_row_stat(const T* __restrict__ p, long long sc, int C, float c2) {
+// the same of a row of any length that one thread walks, 16 classes at a time, the next 16 on their way; each(x, c0) sees them
+template <typename T, typename F>
+__device__ __forceinline__ RowStat walk_row_stat(const T* __restrict__ p, long long sc, int C, float c2, F each) {
+  constexpr int N = 16;
   RowStat a{0.f, 0.f, 0.f};
-  for (int c0 = 0; c0 < C; c0 += 8) {
-    float x[8];
+  T next[N];
+  auto fetch = [&](int c0) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = c0 + j < C ? ld(p + (c0 + j) * sc) : -INFINITY;
-    a = join(a, thread_row_stat<8, true>(x, 8, c2), c2);
+    for (int j = 0; j < N; ++j) next[j] = c0 + j < C ? p[(c0 + j) * sc] : (T)-INFINITY;
+  };
+  fetch(0);
+  for (int c0 = 0; c0 < C; c0 += N) {
+    float x[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = (float)next[j];
+    if (c0 + N < C) fetch(c0 + N);
+    a = join(a, thread_row_stat<N, true>(x, N, c2), c2);
+    each(x, c0);
   }
   return a;
 }
@@ -864,18 +874,22 @@ enum { UH_GRID_WAVES = 256 * 32 };               // workgroups that loop over ro
 
 // Rows of at most 64 classes are a thread's: a group of 16 lanes, four loads each, would leave most lanes empty (12 classes of
 // 16 bits: 2 of 16 at work).  STAGED needs one step from row to row, no more than 64 classes and a half further (LDS, and bytes
-// read between the rows), and a dense gradient.
+// read between the rows), and a dense gradient.  With eight slots of a teacher or more the lanes have those to share, which a
+// thread walks alone, three times over: 16 lanes take such rows of 16 classes and more (166874 rows of 53 fp16 classes by threads
+// and by 16 lanes, 8 slots: 67 and 55 us, 22 slots: 138 and 90 us; 24 fp32 classes, 8 slots: 42 and 44 us; 20 classes of fp16,
+// 6 slots: 17 and 51 us).
 enum ClassPath { PATH_GROUP, PATH_STAGED, PATH_APART, PATH_WALK, PATH_ANY };
-static inline ClassPath uh_class_path(const RowView& v, const RowView* vo, long long rows, int dtype) {
+static inline ClassPath uh_class_path(const RowView& v, const RowView* vo, long long rows, int dtype, int slots = 0) {
   const int elem = uh_elem_bytes(dtype);
-  if (v.C <= 64) {
+  const bool side_by_side = v.sc == 1 && (!vo || vo->sc == 1);
+  if (v.C <= 64 && !(side_by_side && v.C >= 16 && slots >= 8)) {
     const bool staged = v.sc == 1 && v.inner == 1 && v.so >= v.C && v.so <= 96 &&
                         (!vo || (vo->sc == 1 && vo->inner == 1 && vo->so == v.C));
     if (staged) return PATH_STAGED;
     if (uh_apart(v, elem) && (!vo || uh_apart(*vo, elem))) return PATH_APART;
     return rows >= 256 ? PATH_WALK : PATH_ANY;
   }
-  if (v.sc == 1 && (!vo || vo->sc == 1)) return PATH_GROUP;
+  if (side_by_side) return PATH_GROUP;
   return rows >= 256 ? PATH_WALK : PATH_ANY;
 }
 

@@ -616,7 +616,7 @@ template <typename T, int MODE> __global__ __launch_bounds__(64) void ds_walk_ke
     RowStat s{0.f, 0.f, 0.f};
     if (on) {
       if (MODE == 1) s.m = a.stats[2 * r], s.s = a.stats[2 * r + 1];
-      else s = walk_row_stat(row, sc, C, a.c2);
+      else s = walk_row_stat(row, sc, C, a.c2, [](const float (&)[16], int) {});
     }
     if (MODE != 1) {
       if (on) total += (double)w * a.temperature * a.temperature * thread_kl(a, r, q, s, [&](int c) { return row + c * sc; });
@@ -740,10 +740,10 @@ struct DsPlan {
   bool parts;                     // rows by workgroups of 256
   size_t words_at, bytes;
 };
-static DsPlan ds_plan(const RowView& v, const RowView* vo, long long rows, int dtype, bool step) {
+static DsPlan ds_plan(const RowView& v, const RowView* vo, long long rows, int dtype, int slots, bool step) {
   DsPlan p;
   const int elem = uh_elem_bytes(dtype);
-  p.path = uh_class_path(v, vo, rows, dtype);
+  p.path = uh_class_path(v, vo, rows, dtype, slots);
   p.parts = p.path == PATH_GROUP && (long long)v.C * elem > 8192;
   p.cut = p.parts ? uh_row_cut(rows, v.C, dtype, step ? 65536 : 32768) : RowCut{1, v.C};
   const size_t sums = p.parts && rows * p.cut.parts > UH_GRID_WAVES ? rows * p.cut.parts : UH_GRID_WAVES;
@@ -823,8 +823,8 @@ template <int MODE> static long long ds_dispatch(const DsArgs& a, int dtype, con
 extern "C" size_t uh_topk_distill_workspace(const uh_class_view* view) {
   if (uh_check_view(view, "topk_distill_workspace") != UH_OK) return 0;
   const RowView v = uh_row_view(view);
-  const size_t loss = ds_plan(v, nullptr, view->outer * view->inner, view->dtype, false).bytes;
-  const size_t step = ds_plan(v, nullptr, view->outer * view->inner, view->dtype, true).bytes;
+  const size_t loss = ds_plan(v, nullptr, view->outer * view->inner, view->dtype, 0, false).bytes;
+  const size_t step = ds_plan(v, nullptr, view->outer * view->inner, view->dtype, 0, true).bytes;
   return loss > step ? loss : step;
 }
 
@@ -837,7 +837,7 @@ extern "C" int uh_topk_distill(const uh_class_view* view, const void* logits, co
              "topk_distill: null pointer or workspace of %zu bytes", workspace_bytes);
   DsArgs a = ds_args(view, view, slots, weight, temperature);
   a.stats = stats, a.partial = (double*)workspace;
-  const DsPlan p = ds_plan(a.v, nullptr, a.rows, view->dtype, false);
+  const DsPlan p = ds_plan(a.v, nullptr, a.rows, view->dtype, a.K, false);
   const long long n = ds_dispatch<0>(a, view->dtype, logits, nullptr, p, workspace, (hipStream_t)s);
   hipLaunchKernelGGL(ds_finish_kernel, dim3(1), dim3(1024), 0, (hipStream_t)s, n, (const double*)workspace, scale, loss);
   return uh_check_launch("topk_distill");
@@ -852,7 +852,7 @@ extern "C" int uh_topk_distill_bwd(const uh_class_view* view, const uh_class_vie
   UH_REQUIRE(gout && stats && dlogits, "topk_distill_bwd: null pointer");
   DsArgs a = ds_args(view, out_view, slots, weight, temperature);
   a.gout = gout, a.grad_scale = (float)scale, a.stats = const_cast<float*>(stats);
-  const DsPlan p = ds_plan(a.v, &a.vo, a.rows, view->dtype, false);
+  const DsPlan p = ds_plan(a.v, &a.vo, a.rows, view->dtype, a.K, false);
   ds_dispatch<1>(a, view->dtype, logits, dlogits, p, nullptr, (hipStream_t)s);
   return uh_check_launch("topk_distill_bwd");
 }
@@ -868,7 +868,7 @@ extern "C" int uh_topk_distill_step(const uh_class_view* view, const uh_class_vi
              "topk_distill_step: null pointer or workspace of %zu bytes", workspace_bytes);
   DsArgs a = ds_args(view, out_view, slots, weight, temperature);
   a.grad_scale = (float)(scale * (double)grad_scale), a.partial = (double*)workspace;
-  const DsPlan p = ds_plan(a.v, &a.vo, a.rows, view->dtype, true);
+  const DsPlan p = ds_plan(a.v, &a.vo, a.rows, view->dtype, a.K, true);
   const long long n = ds_dispatch<2>(a, view->dtype, logits, dlogits, p, workspace, (hipStream_t)s);
   hipLaunchKernelGGL(ds_finish_kernel, dim3(1), dim3(1024), 0, (hipStream_t)s, n, (const double*)workspace, scale, loss);
   return uh_check_launch("topk_distill_step");
