@@ -494,12 +494,20 @@ template <typename T> __global__ __launch_bounds__(64) void lp_bwd_walk_kernel(L
   const T* row = x + k.v.base(r);
   T* out = dx + k.vo.base(r);
   const int C = k.v.C;
-  for (int c0 = 0; c0 < C; c0 += 8) {
-    float v[8];
+  constexpr int N = 16;                                              // a turn; the next ones are on their way
+  T next[N];
+  auto fetch = [&](int c0) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c0 + j < C && !q.off ? ld(row + (c0 + j) * k.v.sc) : 0.f;
+    for (int j = 0; j < N; ++j) next[j] = c0 + j < C && !q.off ? row[(c0 + j) * k.v.sc] : (T)0.f;
+  };
+  fetch(0);
+  for (int c0 = 0; c0 < C; c0 += N) {
+    float v[N];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < N; ++j) v[j] = (float)next[j];
+    if (c0 + N < C) fetch(c0 + N);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
       if (c0 + j < C) st(out + (c0 + j) * k.vo.sc, q.off ? 0.f : q.of(ref, v[j]) + (c0 + j == q.label ? q.own : 0.f));
   }
 }

@@ -626,12 +626,20 @@ template <typename T, int MODE> __global__ __launch_bounds__(64) void ds_walk_ke
       T* out = dx + a.vo.base(r);
       const RowRef ref(s.m, a.c2);
       const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * q.sum * inv_s;
-      for (int c0 = 0; c0 < C; c0 += 8) {
-        float v[8];
+      constexpr int N = 16;
+      T next[N];
+      auto fetch = [&](int c0) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c0 + j < C && on ? ld(row + (c0 + j) * sc) : 0.f;
+        for (int j = 0; j < N; ++j) next[j] = c0 + j < C && on ? row[(c0 + j) * sc] : (T)0.f;
+      };
+      fetch(0);
+      for (int c0 = 0; c0 < C; c0 += N) {
+        float v[N];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < N; ++j) v[j] = (float)next[j];
+        if (c0 + N < C) fetch(c0 + N);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
           if (c0 + j < C) st(out + (c0 + j) * osc, on ? dense * ex2(ref.z(v[j])) : 0.f);
       }
       if (on)
