@@ -588,12 +588,13 @@ typedef struct {
   int slots, value_dtype, index_bytes;
 } uh_slots;
 
-/* z = (x - max x)/temperature, s = sum e^z:  log_prob = z[label] - ln s (fp32; only with labels, of 4 or 8 bytes),
+/* (temperatures: 1e-6 to 1e6)
+ * z = (x - max x)/temperature, s = sum e^z:  log_prob = z[label] - ln s (fp32; only with labels, of 4 or 8 bytes),
  * entropy = ln s - (sum e^z z)/s, and the `top` largest logits > -inf (equal ones: lowest class first) as
  * top_log_prob = z - ln s with top_index their classes; places left over hold -inf and -1.
  * label == ignore_index: log_prob = entropy = 0, no alternatives.  A label outside [0, classes): log_prob = NaN.
  * A row with a NaN or +inf: NaN everywhere, indices -1.  A row of -inf: log_prob = -inf, entropy = 0, no alternatives.
- * stats (may be NULL): [rows][2] fp32 for the backward call.  workspace: uh_label_log_probs_workspace() bytes. */
+ * stats (may be NULL): [rows][2] fp32 for the backward call.  workspace: uh_label_log_probs_workspace() bytes, 16-byte aligned. */
 size_t uh_label_log_probs_workspace(const uh_class_view* view, int top);
 int uh_label_log_probs(const uh_class_view* view, const void* logits, const void* labels, int label_bytes,
                        long long ignore_index, int top, float temperature, float* log_prob, float* entropy,
@@ -611,7 +612,7 @@ int uh_label_log_probs_bwd(const uh_class_view* view, const uh_class_view* out_v
  *   dlogits_j = g * scale * w T (p_j - sum_{k: i_k = j} t_k)                    (g: gout[0], or grad_scale in the step)
  * Rows with w = 0 or without a filled slot count as 0 and get zero gradients, whatever they hold.  An index >= classes or a
  * NaN among a row's slots makes that row's loss and gradient NaN.  The loss is summed in a fixed order.
- * uh_topk_distill_step gives loss and gradient in one call; stats ([rows][2], may be NULL) carries the rows' statistics
+ * uh_topk_distill_step gives loss and gradient in one call; stats ([rows][2] fp32, may be NULL) carries the rows' statistics
  * from uh_topk_distill to uh_topk_distill_bwd.  workspace: uh_topk_distill_workspace() bytes, 16-byte aligned. */
 size_t uh_topk_distill_workspace(const uh_class_view* view);
 int uh_topk_distill(const uh_class_view* view, const void* logits, const uh_slots* slots, const float* weight,

@@ -93,9 +93,15 @@ def distill(x, v, idx, temperature, weight, scale):
 
 
 def sum_error(c):
-    """Relative error of s = sum of c positive terms as any of the kernels adds them, in half steps of fp32: a thread adds
-    at most max(ceil(c / 64), 64) terms one after the other (rows of up to 64 classes, and maps, lie in one thread: c), and
-    at most 10 levels of a tree join the threads (and 10 more the parts of a split row)."""
+    """Relative error of s = sum of c positive terms as the kernels add them, in half steps of fp32.  An addition costs 1; a
+    rescaling by 2^d 3.5 (the product 1, the exponential 2, the rounding of d 0.5: |d| 2^d < 0.6).  Counted for one term:
+      a thread's row of up to 64 classes: c additions;
+      16 or 64 lanes, at most 32 elements a lane in two chains, a tree of 7 additions: below 64 + 20;
+      a workgroup, NV vectors of E elements a lane: NV E / 2 additions, a rescaling a vector and one for the row, a tree of 10,
+        and 6 levels that join parts (4.5 each): NV (E / 2 + 3.5) + 40.5.  NV = 4: 70, NV = 8: 84 (E = 4) and 100 (E = 8, a part of
+        more than 8192: c/64 + 20 >= 148), NV = 16: 128 and 160 (parts of more than 8192 and 16384: >= 148 and 276);
+      a thread that walks more than 64 classes, 16 a turn: 16 + c/16 and 3.5 for each turn that raises its maximum, which may be
+        more than the number returned; the smaller one is asked of it all the same (roundings do not all point one way)."""
     return min(c, max(-(-c // 64), 64)) + 20
 
 

@@ -107,6 +107,8 @@ def test_c_entry_points_refuse():
     no("top=7", *probs(top=7, tl=p, ti=p))
     no("null", *probs(top=3))
     no("temperature", *probs(t=0.0))
+    no("temperature", *probs(t=5e-7))
+    no("temperature", *probs(t=2e6))
     for bad in ((0, 1, 6, 0, 1, 6, 0), (4, 1, 6, 0, 1, 0, 0), (4, 1, 6, 0, 1, (1 << 20) + 1, 0), (4, 1, 6, 0, 1, 6, 3), (4, 1, 6, 0, -1, 6, 0),
                 (1 << 20, 1 << 20, 6, 0, 1, 6, 0)):
         no("", *probs(v=ctypes.byref(_lib.ClassView(*bad))))

@@ -329,3 +329,44 @@ def test_captured_and_replayed(shape):
             want = go(f.clone().requires_grad_(True))
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(o, want)), turn
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_most_classes(dtype):
+    x = made((2, 1 << 20), dtype, 41)
+    check(x, labels_for(x, 1, 41), top=64, temperature=0.9)
+    check(x, None, grads=False)
+
+
+def test_rows_behind_32768():
+    """rows in parts are a launch's second dimension, and its third past 32768 of them"""
+    x = made((5, 5000), torch.bfloat16, 42)
+    y = labels_for(x, 1, 42)
+    few = label_log_probs(x.repeat(120, 1), y.repeat(120), top=9)          # enough rows for them not to be cut
+    many = label_log_probs(x.repeat(7001, 1), y.repeat(7001), top=9)
+    for a, b in zip(few, many):
+        assert torch.equal(b.view(7001, *a[:5].shape), a[:5].expand(7001, *a[:5].shape))
+
+
+@pytest.mark.parametrize("c", [40, 300, 3000, 9000, 40000])
+def test_logits_past_2_to_99(c):
+    """the scale of the exponents changes at 2^100, and the running sums give way at 2^99"""
+    x = made((6, c), torch.float32, 43)
+    x[0] *= 2.0 ** 99
+    x[1] *= 2.0 ** 102
+    x[2] = x[2] - 2.0 ** 101
+    x[3, c // 2] = 2.0 ** 99
+    x[4, c // 3] = -2.0 ** 99
+    x[5] = -x[5].abs() * 2.0 ** 120 - 2.0 ** 122
+    r = label_log_probs(x, labels_for(x, 1, 43), top=4)
+    want = ref.label_probs(ref.rows_of(x, 1), labels_for(x, 1, 43).cpu(), 4, 1.0)
+    assert torch.equal(r.top_index.cpu().long(), want["index"])
+    ref.close(r.entropy, want["entropy"], ref.entropy_tol(ref.rows_of(x, 1), 1.0), "entropy")
+    ref.close(r.top_log_prob[:, 0], want["top"][:, 0], ref.log_tol(ref.rows_of(x, 1), c, 1.0).amin(1), "largest")
+
+
+@pytest.mark.parametrize("temperature", [1e-6, 1e6])
+@pytest.mark.parametrize("shape", [(70, 12), (20, 300), (9, 3000), (4, 40000), (1, 12, 9, 9), (2, 90, 16, 17)])
+def test_widest_temperatures(shape, temperature):
+    x = made(shape, torch.bfloat16, 44)
+    check(x, labels_for(x, 1, 44), top=3, temperature=temperature, grads=temperature > 1)

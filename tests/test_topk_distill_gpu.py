@@ -348,3 +348,81 @@ def test_light_network_learns_from_the_heavy_one():
     with torch.no_grad():
         lp = label_log_probs(student(images), targets[1][:, 0], top=2)
     assert lp.log_prob.shape == (2, 32, 48) and (lp.entropy >= 0).all() and (lp.top_index[:, 0] >= 0).all()
+
+
+PARTS = [(1, 4097), (3, 20000), (2, 131072), (700, 70001)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape", PARTS)
+def test_parts_that_nobody_waits_for(shape, dtype, monkeypatch):
+    """a row's parts give the same bits whether their statistics arrive or are worked out by those who need them"""
+    x = made(shape, dtype, 61)
+    x[0, 5] = -INF
+    if shape[0] > 2:
+        x[1] *= 2.0 ** 7
+        x[2] = -INF
+        x[2, -3:] = 1.0
+    if dtype == torch.float32:
+        x[-1] *= 2.0 ** 100
+    v, i = targets_for(x.clamp(min=-50, max=50), 7, 61)
+    if shape[0] > 2:
+        i[2] = shape[1] - 1
+
+    def run():
+        leaf = x.detach().requires_grad_(True)
+        loss = topk_distill(leaf, v, i, 2.0)
+        (dx,) = torch.autograd.grad(loss, leaf)
+        return (topk_distill(x, v, i, 2.0), loss.detach(), dx) + tuple(topk_distill_with_logits(x, v, i, 2.0))
+
+    want = run()
+    monkeypatch.setenv("UNET_AMD_DISTILL_SPINS", "0")
+    for a, b in zip(run(), want):
+        assert torch.equal(a.view(torch.uint8) if a.dim() else a.view(1).view(torch.uint8),
+                           b.view(torch.uint8) if b.dim() else b.view(1).view(torch.uint8))
+
+
+def test_two_calls_at_once():
+    """the parts of two calls on two streams, side by side on the card, meet only their own"""
+    xs = [made((96, 131072), torch.bfloat16, 62 + j) for j in range(2)]
+    ts = [targets_for(x, 9, 62) for x in xs]
+    want = [topk_distill_with_logits(x, *t) for x, t in zip(xs, ts)]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[j].append(topk_distill_with_logits(xs[j], *ts[j]))
+    torch.cuda.synchronize()
+    for j in range(2):
+        for loss, dx in got[j]:
+            assert torch.equal(loss, want[j][0]) and torch.equal(dx, want[j][1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_most_classes(dtype):
+    x = made((2, 1 << 20), dtype, 63)
+    check(x, *targets_for(x, 64, 63), temperature=1.5, reduction="sum")
+
+
+def test_rows_behind_32768():
+    x = made((5, 5000), torch.bfloat16, 64)
+    v, i = targets_for(x, 6, 64)
+    few, dfew = topk_distill_with_logits(*(t.repeat(120, 1) for t in (x, v, i)), reduction="sum")    # enough not to be cut
+    loss, dx = topk_distill_with_logits(*(t.repeat(7001, 1) for t in (x, v, i)), reduction="sum")
+    assert torch.equal(dx.view(7001, 5, 5000), dfew[:5].expand(7001, 5, 5000))
+    # the rows' losses, equal on both sides, summed in 64 bits and rounded once
+    want = few.double().item() * 7001 / 120
+    assert abs(loss.double().item() - want) <= 2.0 ** -24 * 2.01 * want
+
+
+@pytest.mark.parametrize("shape,k", [((90, 15), 9), ((90, 16), 7), ((90, 16), 8), ((90, 40), 30), ((91, 64), 64), ((1, 8, 5, 9, 24), 8)])
+def test_many_slots_of_short_rows(shape, k):
+    """16 classes and eight slots: from there on 16 lanes take a row"""
+    k = min(k, shape[-1])
+    for dtype in TYPES:
+        x = made(shape, dtype, 65)
+        check(x, *targets_for(x, k, 65, dim=-1), temperature=1.5, reduction="sum", dim=-1)
+        padded = made(shape[:-1] + (shape[-1] + 3,), dtype, 66)[..., :shape[-1]]
+        check(padded, *targets_for(padded, k, 66, dim=-1), temperature=0.7, dim=-1)

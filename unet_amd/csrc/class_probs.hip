@@ -290,7 +290,8 @@ __global__ __launch_bounds__(64) void lp_thread_kernel(LpArgs a, const T* __rest
   }
 }
 
-// more classes, lying apart: the thread walks its row, once for the statistics and once for every LIST alternatives
+// more classes, lying apart: the thread walks its row, once for the statistics and the first LIST alternatives, and again for
+// every LIST more
 template <typename T, int LIST>
 __global__ __launch_bounds__(64) void lp_walk_kernel(LpArgs a, const T* __restrict__ x) {
   const long long r = (long long)blockIdx.x * 64 + threadIdx.x;
@@ -527,7 +528,7 @@ template <typename T> __global__ __launch_bounds__(256) void lp_bwd_any_kernel(L
 // ---- host ---------------------------------------------------------------------------------------------------------------------------
 // How the rows of a forward call are cut (one part: they are not).  With alternatives parts are 32 KB: looking for candidates
 // is what a workgroup's other waves wait for, and 68 registers leave room for seven workgroups a CU, 108 for four (1024 rows
-// of 131072 bf16 classes, top 64: see the table of measurements).  Without, 64 KB.
+// of 131072 bf16 classes, top 64: 110 us from 64 KB, 105 us from 32 KB).  Without, 64 KB: fewer parts to join.
 static RowCut lp_cut(const RowView& v, long long rows, int dtype, int top) {
   if (uh_class_path(v, nullptr, rows, dtype) != PATH_GROUP || (long long)v.C * uh_elem_bytes(dtype) <= 8192) return RowCut{1, v.C};
   return uh_row_cut(rows, v.C, dtype, top ? 32768 : 65536);
@@ -586,8 +587,14 @@ template <typename T> static void lp_launch(const LpArgs& a, const T* x, int dty
     const dim3 grid((unsigned)cut.parts, (unsigned)(rows < 32768 ? rows : 32768), (unsigned)((rows + 32767) / 32768));
 #define UH_GO(NV, TOP) hipLaunchKernelGGL((lp_rows_kernel<T, NV, TOP>), grid, dim3(256), 0, s, a, x, cut.parts, cut.len, keep, ps, pt)
 #define UH_GO2(NV) do { if (a.top) UH_GO(NV, true); else UH_GO(NV, false); } while (0)
-    // (32 MB and more of fp32 in 64 parts would be more than 32 KB: only then a part with alternatives is 64 KB)
-    if (cut.len <= 256 * E) UH_GO2(1); else if (cut.len <= 256 * 4 * E) UH_GO2(4); else if (cut.len <= 256 * 8 * E) UH_GO2(8); else UH_GO2(16);
+    // parts of 32 bits are longer than 1024 classes; with alternatives longer than 32 KB only where 64 of those are not enough
+    // (more than 524288 classes of 32 bits)
+    if (cut.len <= 256 * 4 * E) {
+      if constexpr (sizeof(T) == 2) { if (cut.len <= 256 * E) UH_GO2(1); else UH_GO2(4); }
+      else UH_GO2(4);
+    } else if (cut.len <= 256 * 8 * E) UH_GO2(8);
+    else if constexpr (sizeof(T) == 2) UH_GO(16, false);
+    else UH_GO2(16);
 #undef UH_GO2
 #undef UH_GO
     if (cut.parts > 1)
@@ -608,7 +615,7 @@ extern "C" int uh_label_log_probs(const uh_class_view* view, const void* logits,
   UH_REQUIRE(top >= 0 && top <= UH_TOP_MAX && top <= view->classes, "label_log_probs: top=%d of %d classes (at most %d)", top,
              view->classes, UH_TOP_MAX);
   UH_REQUIRE(top == 0 || (top_log_prob && top_index), "label_log_probs: null pointer");
-  UH_REQUIRE(temperature > 0.f && temperature < INFINITY, "label_log_probs: temperature %g", temperature);
+  UH_REQUIRE(uh_temperature(temperature), "label_log_probs: temperature %g (1e-6 to 1e6)", temperature);
   const size_t need = uh_label_log_probs_workspace(view, top);
   UH_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
              "label_log_probs: workspace of %zu bytes, %zu needed on 16 bytes", workspace_bytes, need);
@@ -663,7 +670,7 @@ extern "C" int uh_label_log_probs_bwd(const uh_class_view* view, const uh_class_
   UH_REQUIRE(logits && stats && entropy && dlogits, "label_log_probs_bwd: null pointer");
   UH_REQUIRE(!labels || label_bytes == 4 || label_bytes == 8, "label_log_probs_bwd: labels of %d bytes", label_bytes);
   UH_REQUIRE(labels || !g_log_prob, "label_log_probs_bwd: a gradient of log_prob without labels");
-  UH_REQUIRE(temperature > 0.f && temperature < INFINITY, "label_log_probs_bwd: temperature %g", temperature);
+  UH_REQUIRE(uh_temperature(temperature), "label_log_probs_bwd: temperature %g (1e-6 to 1e6)", temperature);
   LpBwd k;
   k.v = uh_row_view(view), k.vo = uh_row_view(out_view);
   k.rows = view->outer * view->inner;

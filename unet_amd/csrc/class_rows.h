@@ -12,7 +12,7 @@
 //     with the true c, and nothing overflows;
 //   a row without a finite logit: m = 0, s = 0, and p = 0 everywhere;  a row with a NaN or +inf: s = NaN.
 //
-// Which kernel takes a row (class_path below): rows whose classes lie side by side are read by a group of lanes, 16 bytes
+// Which kernel takes a row (uh_class_path below): rows whose classes lie side by side are read by a group of lanes, 16 bytes
 // a load, and stay in registers between the maximum, the sums and the gradient; up to 64 classes, or classes that lie apart
 // (maps), a row is one thread's; anything else is one workgroup's, element by element.
 #pragma once
@@ -58,6 +58,10 @@ static inline int uh_check_view(const uh_class_view* v, const char* who) {
   UH_REQUIRE(v->so >= 0 && v->si >= 0 && v->sc >= 0, "%s: negative stride", who);
   return UH_OK;
 }
+
+// The range in which M = c m stays finite for |m| < 2^100 and what a maximum below -2^99 is clamped to is far from any exponent
+// that matters.
+static inline bool uh_temperature(float t) { return t >= 1e-6f && t <= 1e6f; }
 
 // ---- values -------------------------------------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ float ld(const T* p) { return (float)*p; }

@@ -719,7 +719,7 @@ static int distill_check(const char* who, const uh_class_view* v, const void* lo
   UH_REQUIRE(sl->value_dtype >= UH_F32 && sl->value_dtype <= UH_F16, "%s: slot dtype %d", who, sl->value_dtype);
   UH_REQUIRE(sl->index_bytes == 4 || sl->index_bytes == 8, "%s: slot indices of %d bytes", who, sl->index_bytes);
   UH_REQUIRE(logits && sl->value && sl->index, "%s: null pointer", who);
-  UH_REQUIRE(temperature > 0.f && temperature < INFINITY, "%s: temperature %g", who, temperature);
+  UH_REQUIRE(uh_temperature(temperature), "%s: temperature %g (1e-6 to 1e6)", who, temperature);
   return UH_OK;
 }
 
@@ -812,12 +812,14 @@ template <typename T, int MODE> static long long ds_launch(const DsArgs& a, cons
   }
   const dim3 grid((unsigned)cut.parts, (unsigned)(rows < 32768 ? rows : 32768), (unsigned)((rows + 32767) / 32768));
 #define UH_GO(NV) hipLaunchKernelGGL((ds_rows_kernel<T, NV, MODE>), grid, dim3(256), slot_lds(a.K), s, a, x, dx, q)
-  if (cut.len <= 256 * E) UH_GO(1);
-  else if (MODE == 1 || cut.len <= 256 * 4 * E) UH_GO(4);
-  else if constexpr (MODE != 1) {
-    if (cut.len <= 256 * 8 * E) UH_GO(8);
-    else UH_GO(16);
-  }
+  // parts of 32 bits are longer than 1024 classes; those of the loss alone longer than 32 KB only where 64 of 32 KB are not
+  // enough (more than 524288 classes of 32 bits)
+  if constexpr (MODE == 1) UH_GO(4);
+  else if (cut.len <= 256 * 4 * E) {
+    if constexpr (sizeof(T) == 2) { if (cut.len <= 256 * E) UH_GO(1); else UH_GO(4); }
+    else UH_GO(4);
+  } else if (cut.len <= 256 * 8 * E) UH_GO(8);
+  else if constexpr (MODE == 2 || sizeof(T) == 4) UH_GO(16);
 #undef UH_GO
   return MODE == 2 ? (long long)rows * cut.parts : rows;
 }
