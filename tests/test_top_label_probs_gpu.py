@@ -370,3 +370,14 @@ def test_logits_past_2_to_99(c):
 def test_widest_temperatures(shape, temperature):
     x = made(shape, torch.bfloat16, 44)
     check(x, labels_for(x, 1, 44), top=3, temperature=temperature, grads=temperature > 1)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape,top", [((1, 65, 64, 65), 5), ((2, 70, 50, 51), 64), ((3, 150, 41, 37), 4), ((5, 1001, 31, 29), 9), ((1, 80, 64, 64), 3),
+                                       ((1, 81, 17, 241), 0)])
+def test_many_rows_of_classes_that_lie_apart(shape, top, dtype):
+    """from 4097 rows on a thread walks its row"""
+    x = made(shape, dtype, 45)
+    x[0, ::3, 0] = -INF
+    x[0, :, 1] = -INF
+    check(x, labels_for(x, 1, 45), top=top, temperature=1.7)

@@ -426,3 +426,23 @@ def test_many_slots_of_short_rows(shape, k):
         check(x, *targets_for(x, k, 65, dim=-1), temperature=1.5, reduction="sum", dim=-1)
         padded = made(shape[:-1] + (shape[-1] + 3,), dtype, 66)[..., :shape[-1]]
         check(padded, *targets_for(padded, k, 66, dim=-1), temperature=0.7, dim=-1)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape,k", [((1, 65, 64, 65), 5), ((2, 70, 50, 51), 64), ((3, 150, 41, 37), 4), ((5, 1001, 31, 29), 9), ((1, 80, 64, 64), 3),
+                                     ((1, 81, 17, 241), 1)])
+def test_many_rows_of_classes_that_lie_apart(shape, k, dtype):
+    """from 4097 rows on a thread walks its row"""
+    x = made(shape, dtype, 67)
+    x[0, ::3, 0] = -INF
+    check(x.clamp(min=-1e4), *targets_for(x, k, 67), temperature=1.7, reduction="sum")
+    w = torch.rand((shape[0],) + shape[2:], generator=torch.Generator().manual_seed(68)).to(DEV)
+    w[0, 2] = 0.0
+    check(x.clamp(min=-1e4), *targets_for(x, k, 67), temperature=1.7, weight=w, grad_scale=3.0)
+
+
+@pytest.mark.parametrize("c", [36, 37, 38, 56, 57, 64])
+def test_short_rows_on_both_sides_of_28_kb(c):
+    for dtype in TYPES:
+        x = made((700, c), dtype, 69)
+        check(x, *targets_for(x, 4, 69), temperature=2.0, reduction="sum")

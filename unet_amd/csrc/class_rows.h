@@ -877,24 +877,33 @@ static inline unsigned uh_grid(long long blocks, long long most) { return (unsig
 enum { UH_GRID_WAVES = 256 * 32 };               // workgroups that loop over rows: 32 a CU
 
 // Rows of at most 64 classes are a thread's: a group of 16 lanes, four loads each, would leave most lanes empty (12 classes of
-// 16 bits: 2 of 16 at work).  STAGED needs one step from row to row, no more than 64 classes and a half further (LDS, and bytes
-// read between the rows), and a dense gradient.  With eight slots of a teacher or more the lanes have those to share, which a
-// thread walks alone, three times over: 16 lanes take such rows of 16 classes and more (166874 rows of 53 fp16 classes by threads
-// and by 16 lanes, 8 slots: 67 and 55 us, 22 slots: 138 and 90 us; 24 fp32 classes, 8 slots: 42 and 44 us; 20 classes of fp16,
-// 6 slots: 17 and 51 us).
+// 16 bits: 2 of 16 at work).  10^6 rows of 12 bf16 classes by threads and by 16 lanes: log probabilities 11.5 and 87 us, a
+// distillation loss of 3 slots 22 and 159 us; 300000 rows of 40: 10.6 and 27, 17.7 and 48 us.  STAGED needs one step from row to
+// row, no more than 64 classes and a half further (LDS, and bytes read between the rows), and a dense gradient.  16 lanes take
+// distillation's rows of 16 classes and more all the same
+//   with eight slots and more, which the lanes share and a thread walks alone, three times over (166874 rows of 53 fp16 classes,
+//   step, by threads and by 16 lanes: 8 slots 67 and 55 us, 22 slots 138 and 90 us; 24 fp32 classes, 8 slots: 42 and 44 us; 20
+//   fp16 classes, 6 slots: 17 and 51 us);
+//   where a thread's gradient, tile and table of the classes take more than 28 KB of LDS (300000 rows, 4 slots, step: fp32 32
+//   classes 55 and 72 us, 48 classes 83 and 75, 64 classes 156 and 83; bf16 48 classes 50 and 82, 64 classes 90 and 82).
+// Classes that lie apart are one address and a 32-bit offset a wave where that reaches (APART: 8 x 21 x 256 x 256 fp32, step: 27 us,
+// walked: 75).  Elsewhere a thread walks its row from 4097 rows on; below, 256 lanes take a row, in lines of which they use an
+// element (1000 fp32 classes, log probabilities, 256 lanes and one: 256 rows 5.3 and 59 us, 4096 rows 40 and 60, 16384 rows 158 and
+// 60; 100 classes: 1024 rows 4.1 and 9.2, 4096 rows 8.5 and 9.0, 16384 rows 21 and 9.1).
 enum ClassPath { PATH_GROUP, PATH_STAGED, PATH_APART, PATH_WALK, PATH_ANY };
 static inline ClassPath uh_class_path(const RowView& v, const RowView* vo, long long rows, int dtype, int slots = 0) {
   const int elem = uh_elem_bytes(dtype);
   const bool side_by_side = v.sc == 1 && (!vo || vo->sc == 1);
-  if (v.C <= 64 && !(side_by_side && v.C >= 16 && slots >= 8)) {
+  const bool shared = side_by_side && v.C >= 16 && (slots >= 8 || (slots && vo && v.C * 64 * (4 + 2 * elem) > 28672));
+  if (v.C <= 64 && !shared) {
     const bool staged = v.sc == 1 && v.inner == 1 && v.so >= v.C && v.so <= 96 &&
                         (!vo || (vo->sc == 1 && vo->inner == 1 && vo->so == v.C));
     if (staged) return PATH_STAGED;
     if (uh_apart(v, elem) && (!vo || uh_apart(*vo, elem))) return PATH_APART;
-    return rows >= 256 ? PATH_WALK : PATH_ANY;
+    return rows > 4096 ? PATH_WALK : PATH_ANY;
   }
   if (side_by_side) return PATH_GROUP;
-  return rows >= 256 ? PATH_WALK : PATH_ANY;
+  return rows > 4096 ? PATH_WALK : PATH_ANY;
 }
 
 // A row is cut when it is longer than the `most` bytes that a workgroup of 256 is to hold in registers (at most 64 KB), or when

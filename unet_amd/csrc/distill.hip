@@ -99,7 +99,8 @@ template <typename T, int G> __device__ __forceinline__ void group_fix(const DsA
   }
 }
 
-// MODE 0: loss, 1: gradient with statistics given, 2: both.  Four rows of 16 lanes a wave.
+// MODE 0: loss, 1: gradient with statistics given, 2: both.  Four rows of 16 lanes a wave: 100000 rows of 512 bf16 classes, 16
+// slots, step: 69 us, by 64 lanes 127 (of 300, 8 slots, loss: 26 and 83 us).
 template <typename T, int NV, int MODE>
 __global__ __launch_bounds__(64) void ds_quad_kernel(DsArgs a, const T* __restrict__ x, T* __restrict__ dx) {
   extern __shared__ __align__(16) char lds[];
@@ -248,7 +249,7 @@ struct SlotWave {
 };
 static inline size_t slot_lds(int K) { return (size_t)((K + 3) / 4 * 4) * 8; }
 
-// one wave a row
+// one wave a row, up to 8 KB (bf16, by 64 and by 256 lanes: step 20000 x 2000, 16 slots 48 and 64 us, loss 10000 x 4096 25 and 30 us)
 template <typename T, int NV, int MODE>
 __global__ __launch_bounds__(64) void ds_wave_kernel(DsArgs a, const T* __restrict__ x, T* __restrict__ dx) {
   extern __shared__ __align__(16) char lds[];
