@@ -120,8 +120,9 @@ __global__ __launch_bounds__(64) void lp_group_kernel(LpArgs a, const T* __restr
 // ---- longer rows: a workgroup of 256 takes a row, or one part of it ----------------------------------------------------------------
 // A part leaves its statistics and candidates for the alternatives: all it found, in any order, or the `top` largest where that
 // is more than `keep`.  low: order32 of a value that at least `top` of the part's elements reach (0: there are fewer).
-// A row of 32000 bf16 classes for training (4096 rows): read once, 59 us in one kernel (4.5 TB/s; the rest of the time is the
-// exponentials and multiply-adds, which the loads hide only in part); 1024 x 131072, top 64: 105 us; 2047 x 50021, top 8: 70 us.
+// The logits are read once; what bounds it is the exponentials and multiply-adds next to the loads, which hide them only in part
+// (a kernel that only reads reaches 6.4 to 7 TB/s here).  bf16: 4096 x 32000 58 us (4.5 TB/s) past the caches, 70 us where a
+// backward pass reads them again; 2047 x 50021, top 8: 66 us and 7 to join; 1024 x 131072, top 64: 87 us and 14 to join.
 struct LpPart {
   float m, s, t;
   uint32_t low;
@@ -232,7 +233,9 @@ __global__ __launch_bounds__(256) void lp_join_kernel(LpArgs a, const T* __restr
 }
 
 // ---- one thread per row ----------------------------------------------------------------------------------------------------------
-// up to 64 classes in registers (CREG), side by side through LDS (STAGED) or apart; LIST alternatives a sweep
+// up to 64 classes in registers (CREG), side by side through LDS (STAGED) or apart; LIST alternatives a sweep: instances of 2, 3,
+// 5 and 8, since what a place costs is paid for every class.  32 x 21 x 256 x 256 fp32, top 3: 51 us (176 MB read, 50 MB written,
+// 4.5 TB/s); 8 x 19 x 251 x 333 16.6 us, gradient 28 us.
 template <typename T, int CREG, bool STAGED, int LIST>
 __global__ __launch_bounds__(64) void lp_thread_kernel(LpArgs a, const T* __restrict__ x, bool wide) {
   extern __shared__ __align__(16) char lds[];
@@ -378,7 +381,7 @@ struct LpBwd {
   float inv_t, c2;
   const float *stats, *entropy, *g_lp, *g_ent;
 };
-// One pass: the row is read, its gradient written (4096 x 32000 bf16: 525 MB, 86 us, 6.1 TB/s, as fast as a copy).  The walk of
+// One pass: the row is read, its gradient written (4096 x 32000 bf16: 525 MB, 84 us, 6.2 TB/s, what a copy reaches).  The walk of
 // classes that lie apart: 8 x 150 x 128 x 128 bf16 25 us.
 // dx = e (b z + a) with e = 2^z, z = c x - M: the row's 1/s and ln s are folded into a and b
 struct LpCoef {
