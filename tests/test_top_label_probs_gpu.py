@@ -381,3 +381,17 @@ def test_many_rows_of_classes_that_lie_apart(shape, top, dtype):
     x[0, ::3, 0] = -INF
     x[0, :, 1] = -INF
     check(x, labels_for(x, 1, 45), top=top, temperature=1.7)
+
+
+def test_more_than_a_cache_holds():
+    """past 256 MB the rows of a training call are read past the caches: the same bits as those of fewer rows"""
+    x = made((550, 65536), torch.bfloat16, 46).repeat(4, 1)
+    y = labels_for(x, 1, 46)
+    results = []
+    for n in (2200, 1000):
+        leaf = x[:n].detach().requires_grad_(True)
+        r = label_log_probs(leaf, y[:n])
+        (dx,) = torch.autograd.grad([r.log_prob.sum() + r.entropy.sum()], leaf)
+        results.append((r.log_prob.detach(), r.entropy.detach(), dx))
+    for a, b in zip(*results):
+        assert torch.equal(a[:1000], b)

@@ -446,3 +446,16 @@ def test_short_rows_on_both_sides_of_28_kb(c):
     for dtype in TYPES:
         x = made((700, c), dtype, 69)
         check(x, *targets_for(x, 4, 69), temperature=2.0, reduction="sum")
+
+
+def test_more_than_a_cache_holds():
+    """past 256 MB the rows of a loss with a backward pass are read past the caches: the same bits as those of fewer rows"""
+    x = made((550, 65536), torch.bfloat16, 70).repeat(4, 1)
+    v, i = targets_for(x[:550], 5, 70)
+    v, i = v.repeat(4, 1), i.repeat(4, 1)
+    grads = []
+    for n in (2200, 1100):
+        leaf = x[:n].detach().requires_grad_(True)
+        (dx,) = torch.autograd.grad(topk_distill(leaf, v[:n], i[:n], reduction="sum"), leaf)
+        grads.append(dx)
+    assert torch.equal(grads[0][:1100], grads[1]) and torch.equal(grads[0][1100:], grads[1])

@@ -15,6 +15,7 @@ struct LpArgs {
   float *log_prob, *entropy, *top_lp;
   int* top_idx;
   float* stats;
+  bool once;                      // uh_read_once
 
   __device__ __forceinline__ long long label(long long r) const { return labels ? load_int(labels, label_bytes, r) : -1; }
   __device__ __forceinline__ bool ignored(long long l) const { return labels && l == ignore; }
@@ -148,8 +149,7 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(LpArgs a, const T* __restr
   const int n = min(part_len, a.v.C - c0);
   RowRegs<T, 256, NV> reg;
   const T* row = x + a.v.base(r);
-  // rows that no backward pass will read again go past the caches
-  if (!a.stats) reg.template load<true>(row, c0, n, lane);
+  if (a.once) reg.template load<true>(row, c0, n, lane);
   else reg.load(row, c0, n, lane);
   float vmax[TOP ? NV : 1];
   float lm;
@@ -635,6 +635,7 @@ extern "C" int uh_label_log_probs(const uh_class_view* view, const void* logits,
   a.labels = labels, a.label_bytes = label_bytes, a.ignore = ignore_index;
   a.top = top, a.inv_t = 1.f / temperature, a.c2 = (float)(1.4426950408889634 / (double)temperature);
   a.log_prob = log_prob, a.entropy = entropy, a.top_lp = top_log_prob, a.top_idx = top_index, a.stats = stats;
+  a.once = uh_read_once(a.v, a.rows, view->dtype, stats);
   if (view->dtype == UH_F32) lp_launch<float>(a, (const float*)logits, view->dtype, workspace, (hipStream_t)s);
   else if (view->dtype == UH_BF16) lp_launch<bf16>(a, (const bf16*)logits, view->dtype, workspace, (hipStream_t)s);
   else lp_launch<f16>(a, (const f16*)logits, view->dtype, workspace, (hipStream_t)s);

@@ -874,6 +874,12 @@ __device__ __forceinline__ RowStat walk_row_stat(const T* __restrict__ p, long l
 // ---- which kernel takes a call ---------------------------------------------------------------------------------------------
 static inline int uh_elem_bytes(int dtype) { return dtype == UH_F32 ? 4 : 2; }
 static inline unsigned uh_grid(long long blocks, long long most) { return (unsigned)(blocks < most ? blocks : most); }
+// Logits that nothing reads soon again go past the caches: those of calls that no backward pass follows, and those that the card's
+// last cache (256 MB) would not hold until it does (rows of 32000 bf16 classes with their gradient, through the caches and past
+// them: 2000 rows 81 and 86 us, 4096 rows 174 and 172, 8192 rows 335 and 319; distillation 80 and 84, 176 and 176, 339 and 329).
+static inline bool uh_read_once(const RowView& v, long long rows, int dtype, const float* stats) {
+  return !stats || rows * v.C * uh_elem_bytes(dtype) > 1ll << 28;
+}
 enum { UH_GRID_WAVES = 256 * 32 };               // workgroups that loop over rows: 32 a CU
 
 // Rows of at most 64 classes are a thread's: a group of 16 lanes, four loads each, would leave most lanes empty (12 classes of

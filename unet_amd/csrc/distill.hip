@@ -21,6 +21,7 @@ struct DsArgs {
   float grad_scale;               // scale * grad_scale, or scale where gout is given
   const float* gout;
   float* stats;                   // [rows][2]: m, s
+  bool once;                      // uh_read_once, for the loss alone (a step reads past the caches anyway)
   double* partial;
 
   __device__ __forceinline__ float weight_of(long long r) const { return weight ? weight[r] : 1.f; }
@@ -383,8 +384,7 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
   SlotWave q;
   const bool slots = first && (MODE != 0 || part == 0);
   if (slots) q.load(a, r, wl);
-  // rows that no backward pass will read again go past the caches
-  if (MODE == 2 || (MODE == 0 && !a.stats)) reg.template load<true>(row, c0, n, lane);
+  if (MODE == 2 || (MODE == 0 && a.once)) reg.template load<true>(row, c0, n, lane);
   else reg.load(row, c0, n, lane);
   if (slots) {
     // the loss alone is the first part's to work out; for a gradient every part has its classes' share of it
@@ -743,7 +743,7 @@ static DsArgs ds_args(const uh_class_view* view, const uh_class_view* out, const
   a.rows = view->outer * view->inner;
   a.value = s->value, a.index = s->index, a.K = s->slots, a.value_dtype = s->value_dtype, a.index_bytes = s->index_bytes;
   a.weight = weight, a.temperature = temperature, a.inv_t = 1.f / temperature, a.c2 = (float)(1.4426950408889634 / (double)temperature);
-  a.grad_scale = 0.f, a.gout = nullptr, a.stats = nullptr, a.partial = nullptr;
+  a.grad_scale = 0.f, a.gout = nullptr, a.stats = nullptr, a.partial = nullptr, a.once = false;
   return a;
 }
 
@@ -853,6 +853,7 @@ extern "C" int uh_topk_distill(const uh_class_view* view, const void* logits, co
              "topk_distill: null pointer or workspace of %zu bytes", workspace_bytes);
   DsArgs a = ds_args(view, view, slots, weight, temperature);
   a.stats = stats, a.partial = (double*)workspace;
+  a.once = uh_read_once(a.v, a.rows, view->dtype, stats);
   const DsPlan p = ds_plan(a.v, nullptr, a.rows, view->dtype, a.K, false);
   const long long n = ds_dispatch<0>(a, view->dtype, logits, nullptr, p, workspace, (hipStream_t)s);
   hipLaunchKernelGGL(ds_finish_kernel, dim3(1), dim3(1024), 0, (hipStream_t)s, n, (const double*)workspace, scale, loss);
