@@ -17,7 +17,12 @@ struct DsArgs {
   const void *value, *index;
   int K, value_dtype, index_bytes;
   const float* weight;
-  float temperature, inv_t, c2;
+  float temperature, c2;
+  // A row's loss without T^2 is a difference of logits over T, which may overflow where the loss itself does not (a class masked
+  // with the type's lowest value, T < 1).  So it is taken in units of 1/unit, a power of two between T/32 and T/16, which costs
+  // no bit: unit_t = unit / T, per_unit = 1 / unit.
+  float unit, unit_t;
+  double per_unit;
   float grad_scale;               // scale * grad_scale, or scale where gout is given
   const float* gout;
   float* stats;                   // [rows][2]: m, s
@@ -38,12 +43,14 @@ struct DsArgs {
     cls = i < 0 ? -1 : i >= v.C ? v.C : (int)i;
     if (cls < 0 && val == val) val = -INFINITY;
   }
+  // a row's loss of its sum_k t_k (ln t_k - ln p[i_k]) in units
+  __device__ __forceinline__ double row_loss(float w, float kl) const { return (double)w * temperature * temperature * kl * per_unit; }
   __device__ __forceinline__ float coef(float w) const { return (gout ? gout[0] * grad_scale : grad_scale) * w * temperature; }
 };
 
-// ln t_k - ln p of a slot, weighted by t_k: e is 2^(..) of the slot against the teacher's maximum vm, sv their sum
-__device__ __forceinline__ float slot_term(float t, float val, float vm, float ln_sv, float x, float m, float ln_s, float inv_t) {
-  return t > 0.f ? t * ((scaled(val, vm, inv_t) - ln_sv) - (scaled(x, m, inv_t) - ln_s)) : t == t ? 0.f : NAN;
+// t_k (ln t_k - ln p) of a slot, in units: vm is the teacher's maximum, sv the sum of its exponentials; the logarithms in units too
+__device__ __forceinline__ float slot_term(float t, float val, float vm, float ln_sv, float x, float m, float ln_s, float unit_t) {
+  return t > 0.f ? t * ((scaled(val, vm, unit_t) - ln_sv) - (scaled(x, m, unit_t) - ln_s)) : t == t ? 0.f : NAN;
 }
 
 // ---- a row by 16 lanes, or by any group with any strides: the slots in LDS -------------------------------------------------------
@@ -71,19 +78,19 @@ template <int G> __device__ __forceinline__ Teacher group_teacher(const DsArgs& 
     const float val = t_of[k];
     t_of[k] = ex2(ref.z(val)) * inv;
   }
-  return Teacher{m, ref.ln_s(m, sv), bad != 0.f || !(sv >= 0.f) ? NAN : sv == 0.f ? 0.f : 1.f};
+  return Teacher{m, ref.ln_s(m, sv) * a.unit, bad != 0.f || !(sv >= 0.f) ? NAN : sv == 0.f ? 0.f : 1.f};
 }
-// sum_k t_k (ln t_k - ln p[i_k]); the lanes read the slots' values again (t has taken their place)
+// sum_k t_k (ln t_k - ln p[i_k]), in units; the lanes read the slots' values again (t has taken their place)
 template <typename T, int G> __device__ __forceinline__ float group_kl(const DsArgs& a, long long r, const T* __restrict__ row, int lane,
                                                                        const Teacher& q, const RowStat& s, const float* t_of, const int* c_of,
                                                                        typename Red<G>::Buf& red) {
-  const float ln_s = s.s == 0.f ? 0.f : RowRef(s.m, a.c2).ln_s(s.m, s.s);      // no class left: ln p = -inf
+  const float ln_s = s.s == 0.f ? 0.f : RowRef(s.m, a.c2).ln_s(s.m, s.s) * a.unit;      // no class left: ln p = -inf
   float part = 0.f;
   if (!(q.sum == q.sum)) part = NAN;
   else if (q.sum != 0.f)
     for (int k = lane; k < a.K; k += G) {
       const float t = t_of[k];
-      if (t != 0.f) part += slot_term(t, a.value_of(a.v.entry(r, k, a.K)), q.vm, q.ln_sv, ld(row + c_of[k] * a.v.sc), s.m, ln_s, a.inv_t);
+      if (t != 0.f) part += slot_term(t, a.value_of(a.v.entry(r, k, a.K)), q.vm, q.ln_sv, ld(row + c_of[k] * a.v.sc), s.m, ln_s, a.unit_t);
     }
   return Red<G>::sum_(part, red);
 }
@@ -132,7 +139,7 @@ __global__ __launch_bounds__(64) void ds_quad_kernel(DsArgs a, const T* __restri
       s.s = group_sum<16>(s.s);
       const float kl = group_kl<T, 16>(a, r, row, lane, q, s, t_of, c_of, red);
       if (lane == 0 && there) {
-        if (!off && q.sum != 0.f) total += (double)w * a.temperature * a.temperature * kl;
+        if (!off && q.sum != 0.f) total += a.row_loss(w, kl);
         if (a.stats) { a.stats[2 * r] = off ? 0.f : s.m; a.stats[2 * r + 1] = off ? 0.f : s.s; }
       }
     }
@@ -205,7 +212,7 @@ struct SlotWave {
     const float inv = wrong ? NAN : sv == 0.f ? 0.f : rcp(sv);
 #pragma unroll
     for (int q = 0; q < 4; ++q) t[q] *= inv;
-    ln_sv = ref.ln_s(vm, sv);
+    ln_sv = ref.ln_s(vm, sv) * a.unit;
     sum = wrong || !(sv >= 0.f) ? NAN : sv == 0.f ? 0.f : 1.f;
     if (!classes) return;
     const int K4 = (a.K + 3) / 4;
@@ -228,15 +235,15 @@ struct SlotWave {
           mine[q] += ((c4.x == cls[q] ? t4.x : 0.f) + (c4.y == cls[q] ? t4.y : 0.f)) + ((c4.z == cls[q] ? t4.z : 0.f) + (c4.w == cls[q] ? t4.w : 0.f));
     }
   }
-  // sum_k t_k (ln t_k - ln p[i_k]) over the classes between c0 and c0 + n, in all lanes
+  // sum_k t_k (ln t_k - ln p[i_k]) in units, over the classes between c0 and c0 + n, in all lanes
   __device__ __forceinline__ float kl(const DsArgs& a, const RowStat& s, int c0, int n) const {
-    const float ln_s = s.s == 0.f ? 0.f : RowRef(s.m, a.c2).ln_s(s.m, s.s);    // no class left: ln p = -inf
+    const float ln_s = s.s == 0.f ? 0.f : RowRef(s.m, a.c2).ln_s(s.m, s.s) * a.unit;    // no class left: ln p = -inf
     float part = 0.f;
     if (!(sum == sum)) part = NAN;
     else {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        if (q * 64 < a.K && t[q] != 0.f && inside(a, q, c0, n)) part += slot_term(t[q], val[q], vm, ln_sv, xk[q], s.m, ln_s, a.inv_t);
+        if (q * 64 < a.K && t[q] != 0.f && inside(a, q, c0, n)) part += slot_term(t[q], val[q], vm, ln_sv, xk[q], s.m, ln_s, a.unit_t);
     }
     return group_sum<64>(part);
   }
@@ -282,7 +289,7 @@ __global__ __launch_bounds__(64) void ds_wave_kernel(DsArgs a, const T* __restri
       reg.template lane_sums<false>(RowRef(s.m, a.c2), C, s.s, s.t);
       s.s = group_sum<64>(s.s);
       const float kl = q.kl(a, s, 0, C);
-      if (q.sum != 0.f) total += (double)w * a.temperature * a.temperature * kl;
+      if (q.sum != 0.f) total += a.row_loss(w, kl);
       if (lane == 0 && a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
     }
     if constexpr (MODE != 0) {
@@ -445,7 +452,7 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
   if (MODE != 1 && first) {
     const float kl = MODE == 0 ? q.kl(a, s, 0, a.v.C) : q.kl(a, s, c0, n);
     if (wl == 0) {
-      a.partial[MODE == 2 ? r * p.parts + part : r] = sum_t != 0.f ? (double)w * a.temperature * a.temperature * kl : 0.0;
+      a.partial[MODE == 2 ? r * p.parts + part : r] = sum_t != 0.f ? a.row_loss(w, kl) : 0.0;
       if (MODE == 0 && a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
     }
   }
@@ -496,7 +503,7 @@ template <int KS> struct ThreadTeacher {
     }
     vm = best;
     inv = bad ? NAN : sv == 0.f ? 0.f : rcp(sv);
-    ln_sv = w != 0.f ? ref.ln_s(vm, sv) : 0.f;
+    ln_sv = w != 0.f ? ref.ln_s(vm, sv) * a.unit : 0.f;
     sum = bad || !(sv >= 0.f) ? NAN : sv == 0.f ? 0.f : 1.f;
   }
   __device__ __forceinline__ float t(float val) const { return ex2(ref.z(val)) * inv; }
@@ -505,11 +512,11 @@ template <int KS> struct ThreadTeacher {
 template <int KS, typename F> __device__ __forceinline__ float thread_kl(const DsArgs& a, long long r, const ThreadTeacher<KS>& q, const RowStat& s,
                                                                          F at) {
   if (!(q.sum == q.sum)) return NAN;
-  const float ln_s = s.s == 0.f ? 0.f : RowRef(s.m, a.c2).ln_s(s.m, s.s);      // no class left: ln p = -inf
+  const float ln_s = s.s == 0.f ? 0.f : RowRef(s.m, a.c2).ln_s(s.m, s.s) * a.unit;      // no class left: ln p = -inf
   float kl = 0.f;
   q.each(a, r, [&](float val, int cls) {
     const float t = q.t(val);
-    if (t != 0.f) kl += slot_term(t, val, q.vm, q.ln_sv, ld(at(cls)), s.m, ln_s, a.inv_t);
+    if (t != 0.f) kl += slot_term(t, val, q.vm, q.ln_sv, ld(at(cls)), s.m, ln_s, a.unit_t);
   });
   return kl;
 }
@@ -571,7 +578,7 @@ __global__ __launch_bounds__(64) void ds_thread_kernel(DsArgs a, const T* __rest
               if (c < n) tab[c * 64 + lane] = v[c];
             kl = thread_kl(a, r, q, s, [&](int c) { return tab + c * 64 + lane; });
           }
-          total += (double)w * a.temperature * a.temperature * kl;
+          total += a.row_loss(w, kl);
         }
         if (a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
       }
@@ -625,7 +632,7 @@ template <typename T, int MODE> __global__ __launch_bounds__(64) void ds_walk_ke
       else s = walk_row_stat(row, sc, C, a.c2, [](const float (&)[16], int) {});
     }
     if (MODE != 1) {
-      if (on) total += (double)w * a.temperature * a.temperature * thread_kl(a, r, q, s, [&](int c) { return row + c * sc; });
+      if (on) total += a.row_loss(w, thread_kl(a, r, q, s, [&](int c) { return row + c * sc; }));
       if (a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
     }
     if constexpr (MODE != 0) {
@@ -687,7 +694,7 @@ template <typename T, int MODE> __global__ __launch_bounds__(256) void ds_any_ke
     if (MODE != 1) {
       const float kl = group_kl<T, 256>(a, r, row, lane, q, s, t_of, c_of, red);
       if (lane == 0) {
-        if (on) total += (double)w * a.temperature * a.temperature * kl;
+        if (on) total += a.row_loss(w, kl);
         if (a.stats) { a.stats[2 * r] = s.m; a.stats[2 * r + 1] = s.s; }
       }
     }
@@ -742,7 +749,10 @@ static DsArgs ds_args(const uh_class_view* view, const uh_class_view* out, const
   a.v = uh_row_view(view), a.vo = uh_row_view(out);
   a.rows = view->outer * view->inner;
   a.value = s->value, a.index = s->index, a.K = s->slots, a.value_dtype = s->value_dtype, a.index_bytes = s->index_bytes;
-  a.weight = weight, a.temperature = temperature, a.inv_t = 1.f / temperature, a.c2 = (float)(1.4426950408889634 / (double)temperature);
+  int e;
+  frexpf(temperature, &e);                                 // 2^(e-1) <= T < 2^e
+  a.unit = ldexpf(1.f, e - 5), a.unit_t = 1.f / temperature * a.unit, a.per_unit = ldexp(1.0, 5 - e);
+  a.weight = weight, a.temperature = temperature, a.c2 = (float)(1.4426950408889634 / (double)temperature);
   a.grad_scale = 0.f, a.gout = nullptr, a.stats = nullptr, a.partial = nullptr, a.once = false;
   return a;
 }
