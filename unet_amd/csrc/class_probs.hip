@@ -27,7 +27,7 @@ struct LpArgs {
   }
   // by one thread: values of a row; x_label: its label's logit where the label is a class.  Returns ln s.
   __device__ __forceinline__ float write_row(long long r, long long l, float x_label, const RowStat& s) const {
-    const float ln_s = RowRef(s.m, c2).ln_s(s.m, s.s);
+    const float ln_s = AnyRef(s.m, c2).ln_s(s.m, s.s);
     // ln s and t share the rounding of M, so that the entropy takes the logarithm of s itself
     entropy[r] = s.s == 0.f ? 0.f : (lg2(s.s) - s.t * rcp(s.s)) * UH_LN2;
     if (labels)
@@ -79,10 +79,15 @@ __global__ __launch_bounds__(64) void lp_group_kernel(LpArgs a, const T* __restr
     if (s.m == -INFINITY) s.m = 0.f;
     reg.fresh();
     group_sums<T, G, NV>(reg, RowRef(s.m, a.c2), C, s, red);
+    if (__builtin_expect(__any(is_far(s.m, a.c2)), 0)) {
+      RowStat f = s;
+      group_sums<T, G, NV>(reg, FarRef(s.m, a.c2), C, f, red);
+      if (is_far(s.m, a.c2)) s = f;
+    }
     float ln_s = 0.f;
     if (!off) {
       if (lane == 0) ln_s = a.write_row(r, l, a.is_class(l) ? ld(row + l) : 0.f, s);
-      else if (LIST > 0 || TOP) ln_s = RowRef(s.m, a.c2).ln_s(s.m, s.s);
+      else if (LIST > 0 || TOP) ln_s = AnyRef(s.m, a.c2).ln_s(s.m, s.s);
     }
     if constexpr (LIST > 0) {
       TopList<LIST> list;
@@ -156,7 +161,7 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(LpArgs a, const T* __restr
   const RowStat s = arriving_stat<T, 256, NV, true, TOP ? NV : 0>(reg, a.c2, n, lm, vmax, red);
   float ln_s = 0.f;
   if (parts == 1) {
-    ln_s = RowRef(s.m, a.c2).ln_s(s.m, s.s);
+    ln_s = AnyRef(s.m, a.c2).ln_s(s.m, s.s);
     if (lane == 0) a.write_row(r, l, a.is_class(l) ? ld(row + l) : 0.f, s);
   }
   uint32_t low = 0;
@@ -214,7 +219,7 @@ __global__ __launch_bounds__(256) void lp_join_kernel(LpArgs a, const T* __restr
   }
   s = RowStat{__shfl(s.m, 0, 64), __shfl(s.s, 0, 64), __shfl(s.t, 0, 64)};
   low = __shfl(low, 0, 64);
-  const float ln_s = RowRef(s.m, a.c2).ln_s(s.m, s.s);
+  const float ln_s = AnyRef(s.m, a.c2).ln_s(s.m, s.s);
   if (threadIdx.x == 0) a.write_row(r, l, a.is_class(l) ? ld(x + a.v.base(r) + l) : 0.f, s);
   if (a.top == 0) return;
   const uint64_t cut = max((uint64_t)low << 32, (uint64_t)1);
@@ -403,7 +408,7 @@ struct LpCoef {
     label = l >= 0 && l < k.v.C && k.g_lp ? (int)l : -1;
     if (s == 0.f || off) a = b = own = 0.f, label = -1;
   }
-  __device__ __forceinline__ float of(const RowRef& ref, float x) const {
+  template <typename R> __device__ __forceinline__ float of(const R& ref, float x) const {
     const float z = ref.z(x);
     return ex2(z) * fmaf(b, fmaxf(z, UH_ZMIN), a);
   }
@@ -428,11 +433,11 @@ __global__ __launch_bounds__(G > 64 ? G : 64) void lp_bwd_group_kernel(LpBwd k, 
     }
     const T* row = x + k.v.base(r);
     reg.load(row, c0, n, lane);
-    const RowRef ref(q.m, k.c2);
-    reg.map_store(out, c0, n, lane, [&](float v) { return q.of(ref, v); });
+    with_ref(q.m, k.c2, [&](const auto& ref) { reg.map_store(out, c0, n, lane, [&](float v) { return q.of(ref, v); }); });
     // the label's class once more, by the lane that has just written it
     const int at = q.label - c0;
-    if (at >= 0 && at < n && (at / RowRegs<T, G, NV>::E) % G == lane) st(out + q.label, q.of(ref, ld(row + q.label)) + q.own);
+    if (at >= 0 && at < n && (at / RowRegs<T, G, NV>::E) % G == lane)
+      st(out + q.label, q.of(AnyRef(q.m, k.c2), ld(row + q.label)) + q.own);
   }
 }
 
@@ -452,21 +457,24 @@ template <typename T> __global__ __launch_bounds__(64) void lp_bwd_thread_kernel
     __syncthreads();
     if (lane < here) {
       const LpCoef q(k, r);
-      const RowRef ref(q.m, k.c2);
       const T* row = tile + lane * so;
       T* out = res + lane * C;
       if (q.off) {
         for (int c = 0; c < C; ++c) out[c] = (T)0.f;
-      } else if (wide) {                                   // C and so multiples of 16 bytes
-        for (int c = 0; c < C; c += E) {
-          T v[E];
-          *reinterpret_cast<U4*>(v) = *reinterpret_cast<const U4*>(row + c);
-#pragma unroll
-          for (int j = 0; j < E; ++j) v[j] = (T)(q.of(ref, (float)v[j]) + (c + j == q.label ? q.own : 0.f));
-          *reinterpret_cast<U4*>(out + c) = *reinterpret_cast<const U4*>(v);
-        }
       } else {
-        for (int c = 0; c < C; ++c) out[c] = (T)(q.of(ref, (float)row[c]) + (c == q.label ? q.own : 0.f));
+        with_ref(q.m, k.c2, [&](const auto& ref) {
+          if (wide) {                                      // C and so multiples of 16 bytes
+            for (int c = 0; c < C; c += E) {
+              T v[E];
+              *reinterpret_cast<U4*>(v) = *reinterpret_cast<const U4*>(row + c);
+#pragma unroll
+              for (int j = 0; j < E; ++j) v[j] = (T)(q.of(ref, (float)v[j]) + (c + j == q.label ? q.own : 0.f));
+              *reinterpret_cast<U4*>(out + c) = *reinterpret_cast<const U4*>(v);
+            }
+          } else {
+            for (int c = 0; c < C; ++c) out[c] = (T)(q.of(ref, (float)row[c]) + (c == q.label ? q.own : 0.f));
+          }
+        });
       }
     }
     __syncthreads();
@@ -483,16 +491,17 @@ template <typename T> __global__ __launch_bounds__(64) void lp_bwd_apart_kernel(
     const ApartRows at(k.v, b * 64, lane), to(k.vo, b * 64, lane);
     if (r >= k.rows) continue;
     const LpCoef q(k, r);
-    const RowRef ref(q.m, k.c2);
-    for (int c0 = 0; c0 < C; c0 += 16) {
-      float v[16];
+    with_ref(q.m, k.c2, [&](const auto& ref) {
+      for (int c0 = 0; c0 < C; c0 += 16) {
+        float v[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (c0 + j < C) v[j] = (float)*at.at(x, (c0 + j) * k.v.sc);
+        for (int j = 0; j < 16; ++j)
+          if (c0 + j < C) v[j] = (float)*at.at(x, (c0 + j) * k.v.sc);
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (c0 + j < C) *to.at(dx, (c0 + j) * k.vo.sc) = (T)(q.off ? 0.f : q.of(ref, v[j]) + (c0 + j == q.label ? q.own : 0.f));
-    }
+        for (int j = 0; j < 16; ++j)
+          if (c0 + j < C) *to.at(dx, (c0 + j) * k.vo.sc) = (T)(q.off ? 0.f : q.of(ref, v[j]) + (c0 + j == q.label ? q.own : 0.f));
+      }
+    });
   }
 }
 
@@ -501,7 +510,7 @@ template <typename T> __global__ __launch_bounds__(64) void lp_bwd_walk_kernel(L
   const long long r = (long long)blockIdx.x * 64 + threadIdx.x;
   if (r >= k.rows) return;
   const LpCoef q(k, r);
-  const RowRef ref(q.m, k.c2);
+  const AnyRef ref(q.m, k.c2);
   const T* row = x + k.v.base(r);
   T* out = dx + k.vo.base(r);
   const int C = k.v.C;
@@ -527,7 +536,7 @@ template <typename T> __global__ __launch_bounds__(64) void lp_bwd_walk_kernel(L
 template <typename T> __global__ __launch_bounds__(256) void lp_bwd_any_kernel(LpBwd k, const T* __restrict__ x, T* __restrict__ dx) {
   for (long long r = blockIdx.x; r < k.rows; r += gridDim.x) {
     const LpCoef q(k, r);
-    const RowRef ref(q.m, k.c2);
+    const AnyRef ref(q.m, k.c2);
     const T* row = x + k.v.base(r);
     T* out = dx + k.vo.base(r);
     for (int c = threadIdx.x; c < k.v.C; c += 256)

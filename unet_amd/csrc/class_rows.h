@@ -6,10 +6,10 @@
 //
 // Statistics of a row, fp32 whatever the logits' type: m = max x, and with c = log2(e) / T, M = c m rounded to fp32
 //     s = sum 2^(c x - M),   t = sum 2^(c x - M) (c x - M)          one fused multiply-add and one exponential each
-// The rounding of M is no error: it is a common factor of s that ln s = log(s) - (c m - M) ln 2 takes out again.
-//   |m| >= 2^100 (masks of the type's lowest value throughout, or fp32 logits of that size): c = 2^-20 instead, for which
-//     M is exact; neighbouring numbers of that size are 2^57 apart after it, so that p is 1/n for the n largest, as it is
-//     with the true c, and nothing overflows;
+// The rounding of M, r = c m - M, is a common factor 2^r of s that ln s = log(s) - r ln 2 takes out again.  It is at most 1/2 for
+// |M| < 2^24, where it costs less than the sums' own roundings, and grows with |M|: past 2^31 2^r itself would overflow or vanish.
+//   |M| >= 2^24 ("far": rows masked throughout with -1e9 or the type's lowest value, very small temperatures): 2^(c (x - m))
+//     instead, an instruction more an element, with s and t relative to m itself (r = 0);
 //   a row without a finite logit: m = 0, s = 0, and p = 0 everywhere;  a row with a NaN or +inf: s = NaN.
 //
 // Which kernel takes a row (uh_class_path below): rows whose classes lie side by side are read by a group of lanes, 16 bytes
@@ -59,8 +59,8 @@ static inline int uh_check_view(const uh_class_view* v, const char* who) {
   return UH_OK;
 }
 
-// The range in which M = c m stays finite for |m| < 2^100 and what a maximum below -2^99 is clamped to is far from any exponent
-// that matters.
+// The range in which c and 1/T are normal numbers with room to spare: products with a logit's difference may overflow, which
+// is an exponential of 0.
 static inline bool uh_temperature(float t) { return t >= 1e-6f && t <= 1e6f; }
 
 // ---- values -------------------------------------------------------------------------------------------------------------
@@ -75,13 +75,37 @@ __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x)
 __device__ __forceinline__ float lg2(float x) { return __builtin_amdgcn_logf(x); }
 __device__ __forceinline__ float rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 
-struct RowRef {           // the point and the scale a row's exponents are taken in
+// a maximum whose M is too large for its rounding to be taken out again (c2: log2(e) / T)
+__device__ __forceinline__ bool is_far(float m, float c2) { return fabsf(m * c2) >= 0x1p24f; }
+struct RowRef {           // the point and the scale a row's exponents are taken in, its maximum not far
   float c, M;
   __device__ __forceinline__ RowRef(float c_, float M_, int) : c(c_), M(M_) {}
-  __device__ __forceinline__ RowRef(float m, float c2) : c(fabsf(m) >= 0x1p100f ? 0x1p-20f : c2), M(m * c) {}
+  __device__ __forceinline__ RowRef(float m, float c2) : c(c2), M(m * c2) {}
   __device__ __forceinline__ float z(float x) const { return fmaf(x, c, -M); }
   __device__ __forceinline__ float ln_s(float m, float s) const { return (lg2(s) - fmaf(m, c, -M)) * UH_LN2; }
 };
+struct FarRef {           // the same for one that is
+  float c, m;
+  __device__ __forceinline__ FarRef(float m_, float c2) : c(c2), m(m_) {}
+  __device__ __forceinline__ float z(float x) const { return (x - m) * c; }
+};
+struct AnyRef {           // either, for a few values: the bits of the other two
+  float c, M, sub;
+  __device__ __forceinline__ AnyRef(float m, float c2) : c(c2), M(is_far(m, c2) ? 0.f : m * c2), sub(is_far(m, c2) ? m : 0.f) {}
+  __device__ __forceinline__ float z(float x) const { return fmaf(x - sub, c, -M); }
+  __device__ __forceinline__ float ln_s(float m, float s) const { return (lg2(s) - fmaf(m - sub, c, -M)) * UH_LN2; }
+};
+// f, a sweep over a row, with the reference that its maximum needs: two copies of the sweep, of which rows of ordinary logits never
+// pay for the second.  Lanes of one row agree.
+template <typename F> __device__ __forceinline__ void with_ref(float m, float c2, F f) {
+  if (__builtin_expect(is_far(m, c2), 0)) f(FarRef(m, c2));
+  else f(RowRef(m, c2));
+}
+// the same for the whole wave, whose rows may differ
+template <typename F> __device__ __forceinline__ void with_wave_ref(float m, float c2, F f) {
+  if (__builtin_expect(__any(is_far(m, c2)), 0)) f(AnyRef(m, c2));
+  else f(RowRef(m, c2));
+}
 struct RowStat { float m, s, t; };
 
 // (x - m) / T of a reported value; x - m may overflow where its quotient does not (a class masked with the type's lowest
@@ -91,14 +115,21 @@ __device__ __forceinline__ float scaled(float x, float m, float inv_t) {
   return d == -INFINITY ? x * inv_t - m * inv_t : d * inv_t;
 }
 
+// The exponent that takes sums relative to the point of the maximum m0 to that of m >= m0.
+__device__ __forceinline__ float ref_step(float m0, float m, float c2) {
+  const bool f0 = is_far(m0, c2), f = is_far(m, c2);
+  if (m0 == m) return 0.f;
+  return f ? (f0 ? (m0 - m) * c2 : -fmaf(m, c2, -(m0 * c2))) : (f0 ? fmaf(m0, c2, -(m * c2)) : m0 * c2 - m * c2);
+}
 // joins the statistics of two parts of a row; a part without a finite logit (s = 0) has no say in m
 __device__ __forceinline__ RowStat join(const RowStat& a, const RowStat& b, float c2) {
   const float ma = a.s == 0.f ? -INFINITY : a.m, mb = b.s == 0.f ? -INFINITY : b.m;
   float m = fmaxf(ma, mb);
   if (m == -INFINITY) m = 0.f;
-  const RowRef ref(m, c2), ra(a.m, c2), rb(b.m, c2);
-  const float da = a.s == 0.f ? 0.f : ra.c == ref.c ? ra.M - ref.M : (a.m - m) * c2;
-  const float db = b.s == 0.f ? 0.f : rb.c == ref.c ? rb.M - ref.M : (b.m - m) * c2;
+  float da = a.m * c2 - m * c2, db = b.m * c2 - m * c2;
+  if (__builtin_expect(__any(is_far(a.m, c2) || is_far(b.m, c2)), 0)) da = ref_step(a.m, m, c2), db = ref_step(b.m, m, c2);
+  if (a.s == 0.f) da = 0.f;
+  if (b.s == 0.f) db = 0.f;
   const float ea = ex2(da), eb = ex2(db);
   RowStat o;
   o.m = m;
@@ -253,7 +284,7 @@ template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Loose16
 
 struct Online {
   float top, M, s0, s1, t;
-  __device__ __forceinline__ explicit Online(float c2) : top(-INFINITY), M(-0x1p99f * c2), s0(0.f), s1(0.f), t(0.f) {}
+  __device__ __forceinline__ Online() : top(-INFINITY), M(-0x1p24f), s0(0.f), s1(0.f), t(0.f) {}
 };
 
 template <typename T> using LooseVec = __attribute__((ext_vector_type(4), aligned(sizeof(T)))) uint32_t;
@@ -356,7 +387,7 @@ template <typename T, int G, int NV> struct RowRegs {
   }
   // s and (ENT) t of a lane's elements, even and odd ones apart.  Without CLAMP a class of -inf makes t a NaN; the -inf that
   // fill the row's last vectors do not.
-  template <bool ENT, bool CLAMP = false> __device__ __forceinline__ void add_sums(const RowRef& ref, int n, float& s0, float& s1, float& t0, float& t1) const {
+  template <bool ENT, bool CLAMP = false, typename R> __device__ __forceinline__ void add_sums(const R& ref, int n, float& s0, float& s1, float& t0, float& t1) const {
     n = renew_uniform(n);
 #pragma unroll
     for (int r = 0; r < NV; ++r)
@@ -366,7 +397,7 @@ template <typename T, int G, int NV> struct RowRegs {
         __builtin_amdgcn_sched_barrier(0);
       }
   }
-  template <bool ENT, bool CLAMP> __device__ __forceinline__ void add_vector(int r, const RowRef& ref, float& s0, float& s1, float& t0, float& t1) const {
+  template <bool ENT, bool CLAMP, typename R> __device__ __forceinline__ void add_vector(int r, const R& ref, float& s0, float& s1, float& t0, float& t1) const {
 #pragma unroll
     for (int j = 0; j < E; j += 2) {
       const float z0 = ref.z(get(r, j)), z1 = ref.z(get(r, j + 1));
@@ -375,13 +406,14 @@ template <typename T, int G, int NV> struct RowRegs {
       if (ENT) t0 = fmaf(e0, CLAMP ? fmaxf(z0, UH_ZMIN) : z0, t0), t1 = fmaf(e1, CLAMP ? fmaxf(z1, UH_ZMIN) : z1, t1);
     }
   }
-  template <bool ENT, bool CLAMP = false> __device__ __forceinline__ void lane_sums(const RowRef& ref, int n, float& s, float& t) const {
+  template <bool ENT, bool CLAMP = false, typename R> __device__ __forceinline__ void lane_sums(const R& ref, int n, float& s, float& t) const {
     float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f;
     add_sums<ENT, CLAMP>(ref, n, s0, s1, t0, t1);
     s = s0 + s1, t = t0 + t1;
   }
-  // Largest element, s and (ENT) t of a lane in one sweep that takes the vectors as they arrive: against the running maximum,
-  // not below -2^99, whose M is returned; a vector that raises it rescales what is summed.  vmax as in lane_max.
+  // Largest element, s and (ENT) t of a lane in one sweep that takes the vectors as they arrive: against the running maximum's
+  // M, not below -2^24 (a row whose maximum is not far loses nothing by it), which is returned; a vector that raises it rescales
+  // what is summed.  vmax as in lane_max.
   template <bool ENT, int NM> __device__ __forceinline__ void online(float c2, int n, Online& o, float* vmax) const {
     n = renew_uniform(n);
 #pragma unroll
@@ -397,7 +429,7 @@ template <typename T, int G, int NV> struct RowRegs {
 #pragma unroll
     for (int j = 2; j < E; j += 2) v = max3(v, get(r, j), get(r, j + 1));
     o.top = fmaxf(o.top, v);
-    const float M = fmaxf(o.top, -0x1p99f) * c2, d = o.M - M, f = ex2(d);
+    const float M = fmaxf(o.top * c2, -0x1p24f), d = o.M - M, f = ex2(d);
     if (ENT) o.t = f * fmaf(o.s0 + o.s1, d, o.t);
     o.s0 *= f, o.s1 *= f;
     o.M = M;
@@ -446,14 +478,10 @@ template <typename T, int G, int NV> struct RowRegs {
   }
 };
 
-// A maximum against which the running sums of `online` are of no use: all logits, or the largest, of a size that only the other
-// scale of RowRef takes.
-__device__ __forceinline__ bool beyond_online(float m) { return fabsf(m) >= 0x1p99f && m != -INFINITY; }
-
 // s and t of a row in registers, given its maximum.  The clamp of its exponents, one instruction of nine an element, is only for
 // classes of -inf (0 times -inf): rows that hold one are found by their NaN and summed again with it.
-template <typename T, int G, int NV>
-__device__ __forceinline__ void group_sums(RowRegs<T, G, NV>& x, const RowRef& ref, int n, RowStat& s, typename Red<G>::Buf& red) {
+template <typename T, int G, int NV, typename R>
+__device__ __forceinline__ void group_sums(RowRegs<T, G, NV>& x, const R& ref, int n, RowStat& s, typename Red<G>::Buf& red) {
   x.template lane_sums<true>(ref, n, s.s, s.t);
   Red<G>::sum2(s.s, s.t, red);
   const bool again = s.t != s.t && s.s == s.s;
@@ -468,22 +496,23 @@ __device__ __forceinline__ void group_sums(RowRegs<T, G, NV>& x, const RowRef& r
 // arrive, instead of after the last of them, when nothing would be on its way.  lane_top: the lane's largest.
 template <typename T, int G, int NV, bool ENT, int NM>
 __device__ __forceinline__ RowStat arriving_stat(RowRegs<T, G, NV>& x, float c2, int n, float& lane_top, float* vmax, typename Red<G>::Buf& red) {
-  Online o(c2);
+  Online o;
   x.template online<ENT, NM>(c2, n, o, vmax);
   lane_top = o.top;
   x.fresh();                                                 // once, ahead of the branches: in them it would copy the row
   RowStat s;
   s.m = Red<G>::max_(o.top, red);
   if (s.m == -INFINITY) s.m = 0.f;
-  const RowRef ref(s.m, c2);
-  if (beyond_online(s.m)) {
-    if (ENT) group_sums<T, G, NV>(x, ref, n, s, red);
+  if (is_far(s.m, c2)) {                                     // what was summed is of no use
+    const FarRef far(s.m, c2);
+    if (ENT) group_sums<T, G, NV>(x, far, n, s, red);
     else {
-      x.template lane_sums<false>(ref, n, s.s, s.t);
+      x.template lane_sums<false>(far, n, s.s, s.t);
       s.s = Red<G>::sum_(s.s, red);
     }
     return s;
   }
+  const RowRef ref(s.m, c2);
   const float d = o.M - ref.M, f = ex2(d);
   s.s = (o.s0 + o.s1) * f;
   if (ENT) {
@@ -516,7 +545,7 @@ template <typename T, int G> __device__ RowStat strided_row_stat(const T* __rest
   for (int c = lane; c < C; c += G) m = fmaxf(m, ld(x + c * sc));
   m = Red<G>::max_(m, buf);
   if (m == -INFINITY) m = 0.f;
-  const RowRef ref(m, c2);
+  const AnyRef ref(m, c2);
   float s = 0.f, t = 0.f;
   for (int c = lane; c < C; c += G) {
     const float z = ref.z(ld(x + c * sc)), e = ex2(z);
@@ -827,26 +856,30 @@ template <typename T, int CREG> __device__ __forceinline__ void load_classes_wid
       for (int j = 0; j < E; ++j) x[c + j] = -INFINITY;
     }
 }
-template <int CREG, bool ENT> __device__ __forceinline__ RowStat thread_row_stat(const float (&x)[CREG], int C, float c2) {
+// FAR = false: the caller sums again what is_far
+template <int CREG, bool ENT, bool FAR = true> __device__ __forceinline__ RowStat thread_row_stat(const float (&x)[CREG], int C, float c2) {
   C = renew_uniform(C);
   float m = x[0];
 #pragma unroll
   for (int c = 1; c < CREG; c += 2)
     if (c < C) m = max3(m, x[c], c + 1 < CREG ? x[c + 1] : x[c]);
   if (m == -INFINITY) m = 0.f;
-  const RowRef ref(m, c2);
   float s = 0.f, t = 0.f;
   C = renew_uniform(C);
+  const auto sums = [&](const auto& ref) {
 #pragma unroll
-  for (int c = 0; c < CREG; ++c)
-    if (c < C) {
-      const float z = ref.z(x[c]), e = ex2(z);
-      s += e;
-      if (ENT) {
-        t = fmaf(e, fmaxf(z, UH_ZMIN), t);
-        asm volatile("" : "+v"(s), "+v"(t));                 // now: left to be summed later, the terms take two registers a class
+    for (int c = 0; c < CREG; ++c)
+      if (c < C) {
+        const float z = ref.z(x[c]), e = ex2(z);
+        s += e;
+        if (ENT) {
+          t = fmaf(e, fmaxf(z, UH_ZMIN), t);
+          asm volatile("" : "+v"(s), "+v"(t));               // now: left to be summed later, the terms take two registers a class
+        }
       }
-    }
+  };
+  if (FAR) with_ref(m, c2, sums);
+  else sums(RowRef(m, c2));
   return RowStat{m, s, t};
 }
 // the same of a row of any length that one thread walks, 16 classes at a time, the next 16 on their way; each(x, c0) sees them

@@ -69,22 +69,24 @@ template <int G> __device__ __forceinline__ Teacher group_teacher(const DsArgs& 
   }
   vm = Red<G>::max_(vm, red);
   const float m = vm == -INFINITY ? 0.f : vm;
-  const RowRef ref(m, a.c2);
-  float sv = 0.f;
-  for (int k = lane; k < a.K; k += G) sv += ex2(ref.z(t_of[k]));
-  Red<G>::sum2(sv, bad, red);
-  const float inv = bad != 0.f ? NAN : sv == 0.f ? 0.f : rcp(sv);
-  for (int k = lane; k < a.K; k += G) {
-    const float val = t_of[k];
-    t_of[k] = ex2(ref.z(val)) * inv;
-  }
-  return Teacher{m, ref.ln_s(m, sv) * a.unit, bad != 0.f || !(sv >= 0.f) ? NAN : sv == 0.f ? 0.f : 1.f};
+  float sv = 0.f, ln_sv;
+  with_wave_ref(m, a.c2, [&](const auto& ref) {
+    for (int k = lane; k < a.K; k += G) sv += ex2(ref.z(t_of[k]));
+    Red<G>::sum2(sv, bad, red);
+    const float inv = bad != 0.f ? NAN : sv == 0.f ? 0.f : rcp(sv);
+    for (int k = lane; k < a.K; k += G) {
+      const float val = t_of[k];
+      t_of[k] = ex2(ref.z(val)) * inv;
+    }
+    ln_sv = ref.ln_s(m, sv) * a.unit;
+  });
+  return Teacher{m, ln_sv, bad != 0.f || !(sv >= 0.f) ? NAN : sv == 0.f ? 0.f : 1.f};
 }
 // sum_k t_k (ln t_k - ln p[i_k]), in units; the lanes read the slots' values again (t has taken their place)
 template <typename T, int G> __device__ __forceinline__ float group_kl(const DsArgs& a, long long r, const T* __restrict__ row, int lane,
                                                                        const Teacher& q, const RowStat& s, const float* t_of, const int* c_of,
                                                                        typename Red<G>::Buf& red) {
-  const float ln_s = s.s == 0.f ? 0.f : RowRef(s.m, a.c2).ln_s(s.m, s.s) * a.unit;      // no class left: ln p = -inf
+  const float ln_s = s.s == 0.f ? 0.f : AnyRef(s.m, a.c2).ln_s(s.m, s.s) * a.unit;      // no class left: ln p = -inf
   float part = 0.f;
   if (!(q.sum == q.sum)) part = NAN;
   else if (q.sum != 0.f)
@@ -95,8 +97,8 @@ template <typename T, int G> __device__ __forceinline__ float group_kl(const DsA
   return Red<G>::sum_(part, red);
 }
 // classes the teacher names, written again after the dense part: p minus what all slots of that class hold
-template <typename T, int G> __device__ __forceinline__ void group_fix(const DsArgs& a, const T* __restrict__ row, T* __restrict__ out, int lane,
-                                                                       float sum_t, float coef, const RowRef& ref, float inv_s, const float* t_of,
+template <typename T, int G, typename R> __device__ __forceinline__ void group_fix(const DsArgs& a, const T* __restrict__ row, T* __restrict__ out, int lane,
+                                                                       float sum_t, float coef, const R& ref, float inv_s, const float* t_of,
                                                                        const int* c_of) {
   for (int k = lane; k < a.K; k += G) {
     const int c = c_of[k];
@@ -135,7 +137,7 @@ __global__ __launch_bounds__(64) void ds_quad_kernel(DsArgs a, const T* __restri
       s.m = group_max<16>(off ? -INFINITY : reg.lane_max(C));
       if (s.m == -INFINITY) s.m = 0.f;
       reg.fresh();
-      reg.template lane_sums<false>(RowRef(s.m, a.c2), C, s.s, s.t);
+      with_wave_ref(s.m, a.c2, [&](const auto& ref) { reg.template lane_sums<false>(ref, C, s.s, s.t); });
       s.s = group_sum<16>(s.s);
       const float kl = group_kl<T, 16>(a, r, row, lane, q, s, t_of, c_of, red);
       if (lane == 0 && there) {
@@ -146,13 +148,14 @@ __global__ __launch_bounds__(64) void ds_quad_kernel(DsArgs a, const T* __restri
     if constexpr (MODE != 0) {
       if (there) {
         T* out = dx + a.vo.base(r);
-        const RowRef ref(s.m, a.c2);
         const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * q.sum * inv_s;
         reg.fresh();
         if (off || q.sum == 0.f) reg.map_store(out, 0, C, lane, [](float) { return 0.f; });
         else {
-          reg.map_store(out, 0, C, lane, [&](float v) { return dense * ex2(ref.z(v)); });
-          group_fix<T, 16>(a, row, out, lane, q.sum, co, ref, inv_s, t_of, c_of);
+          with_wave_ref(s.m, a.c2, [&](const auto& ref) {
+            reg.map_store(out, 0, C, lane, [&](float v) { return dense * ex2(ref.z(v)); });
+            group_fix<T, 16>(a, row, out, lane, q.sum, co, ref, inv_s, t_of, c_of);
+          });
         }
       }
     }
@@ -201,7 +204,7 @@ struct SlotWave {
       }
     best = group_max<64>(best);
     vm = best == -INFINITY ? 0.f : best;
-    const RowRef ref(vm, a.c2);
+    const AnyRef ref(vm, a.c2);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       t[q] = q * 64 < a.K ? ex2(ref.z(val[q])) : 0.f;
@@ -237,7 +240,7 @@ struct SlotWave {
   }
   // sum_k t_k (ln t_k - ln p[i_k]) in units, over the classes between c0 and c0 + n, in all lanes
   __device__ __forceinline__ float kl(const DsArgs& a, const RowStat& s, int c0, int n) const {
-    const float ln_s = s.s == 0.f ? 0.f : RowRef(s.m, a.c2).ln_s(s.m, s.s) * a.unit;    // no class left: ln p = -inf
+    const float ln_s = s.s == 0.f ? 0.f : AnyRef(s.m, a.c2).ln_s(s.m, s.s) * a.unit;    // no class left: ln p = -inf
     float part = 0.f;
     if (!(sum == sum)) part = NAN;
     else {
@@ -248,7 +251,7 @@ struct SlotWave {
     return group_sum<64>(part);
   }
   // the classes the teacher names there, written again after the dense part
-  template <typename T> __device__ __forceinline__ void fix(const DsArgs& a, T* __restrict__ out, int c0, int n, float coef, const RowRef& ref,
+  template <typename T> __device__ __forceinline__ void fix(const DsArgs& a, T* __restrict__ out, int c0, int n, float coef, const AnyRef& ref,
                                                             float inv_s) const {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
@@ -286,7 +289,7 @@ __global__ __launch_bounds__(64) void ds_wave_kernel(DsArgs a, const T* __restri
       s.m = group_max<64>(reg.lane_max(C));
       if (s.m == -INFINITY) s.m = 0.f;
       reg.fresh();
-      reg.template lane_sums<false>(RowRef(s.m, a.c2), C, s.s, s.t);
+      with_ref(s.m, a.c2, [&](const auto& ref) { reg.template lane_sums<false>(ref, C, s.s, s.t); });
       s.s = group_sum<64>(s.s);
       const float kl = q.kl(a, s, 0, C);
       if (q.sum != 0.f) total += a.row_loss(w, kl);
@@ -294,13 +297,12 @@ __global__ __launch_bounds__(64) void ds_wave_kernel(DsArgs a, const T* __restri
     }
     if constexpr (MODE != 0) {
       T* out = dx + a.vo.base(r);
-      const RowRef ref(s.m, a.c2);
       const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * q.sum * inv_s;
       reg.fresh();
       if (q.sum == 0.f) reg.map_store(out, 0, C, lane, [](float) { return 0.f; });
       else {
-        reg.map_store(out, 0, C, lane, [&](float v) { return dense * ex2(ref.z(v)); });
-        q.fix(a, out, 0, C, co, ref, inv_s);
+        with_ref(s.m, a.c2, [&](const auto& ref) { reg.map_store(out, 0, C, lane, [&](float v) { return dense * ex2(ref.z(v)); }); });
+        q.fix(a, out, 0, C, co, AnyRef(s.m, a.c2), inv_s);
       }
     }
   }
@@ -341,23 +343,23 @@ template <typename T> __device__ __forceinline__ RowStat alone_part_stat(const T
   }
   m = group_max<64>(m);
   if (m == -INFINITY) m = 0.f;
-  const RowRef ref(m, c2);
+  const bool far = is_far(m, c2);
   float total = 0.f;
 #pragma unroll 1
   for (int w = 0; w < 4; ++w) {
-    Online o(c2);
+    Online o;
 #pragma unroll 1
     for (int first = 0; first < n; first += 256 * E) {
       v.load(p, c0 + first, n - first, lane + 64 * w);
-      if (beyond_online(m)) {
+      if (far) {
         float t0 = 0.f, t1 = 0.f;
-        v.template add_sums<false>(ref, n - first, o.s0, o.s1, t0, t1);
+        v.template add_sums<false>(FarRef(m, c2), n - first, o.s0, o.s1, t0, t1);
       } else {
         v.template online_vector<false>(0, c2, false, o);
       }
     }
     float s = o.s0 + o.s1;
-    if (!beyond_online(m)) s *= ex2(o.M - ref.M);
+    if (!far) s *= ex2(o.M - RowRef(m, c2).M);
     s = group_sum<64>(s);
     total = w == 0 ? s : total + s;
   }
@@ -438,15 +440,14 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
       s.m = joined[0], s.s = joined[1];
     }
   }
-  const RowRef ref(s.m, a.c2);
   const float sum_t = joined[2];
   if constexpr (MODE != 0) {
     const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * sum_t * inv_s;
     if (sum_t == 0.f) reg.map_store(out, c0, n, lane, [](float) { return 0.f; });
     else {
-      reg.map_store(out, c0, n, lane, [&](float v) { return dense * ex2(ref.z(v)); });
+      with_ref(s.m, a.c2, [&](const auto& ref) { reg.map_store(out, c0, n, lane, [&](float v) { return dense * ex2(ref.z(v)); }); });
       __syncthreads();                                     // another wave may have written the class
-      if (first) q.fix(a, out, c0, n, co, ref, inv_s);
+      if (first) q.fix(a, out, c0, n, co, AnyRef(s.m, a.c2), inv_s);
     }
   }
   if (MODE != 1 && first) {
@@ -461,9 +462,10 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
 // ---- one thread per row ----------------------------------------------------------------------------------------------------------
 // The teacher's softmax of a thread's own row.  KS > 0: at most KS slots, read once and kept; KS = 0: any number, read once for
 // the maximum, once for the sum and again for every use.
-template <int KS> struct ThreadTeacher {
+// R: RowRef, where the caller sees to the rows for which it will not do, or AnyRef.
+template <int KS, typename R> struct ThreadTeacher {
   float vm, ln_sv, inv, sum;
-  RowRef ref;
+  R ref;
   float val_[KS > 0 ? KS : 1];
   int cls_[KS > 0 ? KS : 1];
   template <typename F> __device__ __forceinline__ void each(const DsArgs& a, long long r, F f) const {
@@ -498,7 +500,7 @@ template <int KS> struct ThreadTeacher {
         best = fmaxf(best, val);
       });
       if (best == -INFINITY) best = 0.f;
-      ref = RowRef(best, a.c2);
+      ref = R(best, a.c2);
       each(a, r, [&](float val, int) { sv += ex2(ref.z(val)); });
     }
     vm = best;
@@ -509,13 +511,14 @@ template <int KS> struct ThreadTeacher {
   __device__ __forceinline__ float t(float val) const { return ex2(ref.z(val)) * inv; }
 };
 // at(c): where the student's class c lies
-template <int KS, typename F> __device__ __forceinline__ float thread_kl(const DsArgs& a, long long r, const ThreadTeacher<KS>& q, const RowStat& s,
-                                                                         F at) {
+template <int KS, typename R, typename F>
+__device__ __forceinline__ float thread_kl(const DsArgs& a, long long r, const ThreadTeacher<KS, R>& q, const RowStat& s, F at) {
   if (!(q.sum == q.sum)) return NAN;
-  const float ln_s = s.s == 0.f ? 0.f : RowRef(s.m, a.c2).ln_s(s.m, s.s) * a.unit;      // no class left: ln p = -inf
+  const float ln_s = s.s == 0.f ? 0.f : R(s.m, a.c2).ln_s(s.m, s.s) * a.unit;  // no class left: ln p = -inf
   float kl = 0.f;
   q.each(a, r, [&](float val, int cls) {
     const float t = q.t(val);
+    // (a free slot has t = 0: its exponent is -inf, or a NaN where a RowRef's M is -inf, and then the sum is one as well)
     if (t != 0.f) kl += slot_term(t, val, q.vm, q.ln_sv, ld(at(cls)), s.m, ln_s, a.unit_t);
   });
   return kl;
@@ -543,7 +546,7 @@ __global__ __launch_bounds__(64) void ds_thread_kernel(DsArgs a, const T* __rest
   for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
     const long long r = b * 64 + lane;
     const int here = (int)min(64ll, a.rows - b * 64);
-    ThreadTeacher<KS> q(a);
+    ThreadTeacher<KS, RowRef> q(a);
     float w = 0.f;
     if (lane < here) {
       w = a.weight_of(r);
@@ -561,11 +564,15 @@ __global__ __launch_bounds__(64) void ds_thread_kernel(DsArgs a, const T* __rest
       if (STAGED && wide) load_classes_wide<T, CREG>(v, tile + lane * so, C);
       else load_classes<T, CREG>(v, C, at);
       q.softmax(a, r, w);
-      const bool on = w != 0.f && q.sum != 0.f;
+      // a far maximum (class_rows.h) in either row: what the sweeps below make of it is worked out again, class by class and
+      // slot by slot, so that other rows pay a comparison
+      bool far = is_far(q.vm, a.c2);
+      const bool on = w != 0.f && (q.sum != 0.f || far);
       RowStat s{0.f, 0.f, 0.f};
       if (on) {
         if (MODE == 1) s.m = a.stats[2 * r], s.s = a.stats[2 * r + 1];
-        else s = thread_row_stat<CREG, false>(v, C, a.c2);
+        else s = thread_row_stat<CREG, false, false>(v, C, a.c2);
+        far |= is_far(s.m, a.c2);
       }
       if (MODE != 1) {
         if (on) {
@@ -577,6 +584,14 @@ __global__ __launch_bounds__(64) void ds_thread_kernel(DsArgs a, const T* __rest
             for (int c = 0; c < CREG; ++c)
               if (c < n) tab[c * 64 + lane] = v[c];
             kl = thread_kl(a, r, q, s, [&](int c) { return tab + c * 64 + lane; });
+          }
+          if (__builtin_expect(far, 0)) {
+            const AnyRef ref(s.m, a.c2);
+            s.s = 0.f;
+            for (int c = 0; c < C; ++c) s.s += ex2(ref.z(ld(at(c))));
+            ThreadTeacher<0, AnyRef> f(a);
+            f.softmax(a, r, w);
+            kl = thread_kl(a, r, f, s, at);
           }
           total += a.row_loss(w, kl);
         }
@@ -590,15 +605,25 @@ __global__ __launch_bounds__(64) void ds_thread_kernel(DsArgs a, const T* __rest
         } else {
           const RowRef ref(s.m, a.c2);
           const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * q.sum * inv_s;
+          const auto named = [&](const auto& teacher) {
 #pragma unroll 8
-          for (int c = 0; c < C; ++c) tab[c * 64 + lane] = 0.f;
-          q.each(a, r, [&](float val, int cls) {
-            if (cls >= 0 && cls < C) tab[cls * 64 + lane] -= q.t(val);
-          });
+            for (int c = 0; c < C; ++c) tab[c * 64 + lane] = 0.f;
+            teacher.each(a, r, [&](float val, int cls) {
+              if (cls >= 0 && cls < C) tab[cls * 64 + lane] -= teacher.t(val);
+            });
+          };
+          named(q);
           const int n = renew_uniform(C);
 #pragma unroll
           for (int c = 0; c < CREG; ++c)
             if (c < n) *to(c) = (T)fmaf(co, tab[c * 64 + lane], dense * ex2(ref.z(v[c])));
+          if (__builtin_expect(far, 0)) {
+            const AnyRef any(s.m, a.c2);
+            ThreadTeacher<0, AnyRef> f(a);
+            f.softmax(a, r, w);
+            named(f);
+            for (int c = 0; c < C; ++c) *to(c) = (T)fmaf(co, tab[c * 64 + lane], co * f.sum * inv_s * ex2(any.z(ld(at(c)))));
+          }
         }
       }
     }
@@ -623,7 +648,7 @@ template <typename T, int MODE> __global__ __launch_bounds__(64) void ds_walk_ke
     if (r >= a.rows) continue;
     const T* row = x + a.v.base(r);
     const float w = a.weight_of(r);
-    ThreadTeacher<0> q(a);
+    ThreadTeacher<0, AnyRef> q(a);
     q.softmax(a, r, w);
     const bool on = w != 0.f && q.sum != 0.f;
     RowStat s{0.f, 0.f, 0.f};
@@ -637,7 +662,7 @@ template <typename T, int MODE> __global__ __launch_bounds__(64) void ds_walk_ke
     }
     if constexpr (MODE != 0) {
       T* out = dx + a.vo.base(r);
-      const RowRef ref(s.m, a.c2);
+      const AnyRef ref(s.m, a.c2);
       const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * q.sum * inv_s;
       constexpr int N = 16;
       T next[N];
@@ -700,7 +725,7 @@ template <typename T, int MODE> __global__ __launch_bounds__(256) void ds_any_ke
     }
     if constexpr (MODE != 0) {
       T* out = dx + a.vo.base(r);
-      const RowRef ref(s.m, a.c2);
+      const AnyRef ref(s.m, a.c2);
       const float inv_s = s.s == 0.f ? 0.f : rcp(s.s), co = a.coef(w), dense = co * q.sum * inv_s;
       for (int c = lane; c < C; c += 256) st(out + c * a.vo.sc, on ? dense * ex2(ref.z(ld(row + c * a.v.sc))) : 0.f);
       __syncthreads();
