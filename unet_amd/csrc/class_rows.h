@@ -287,7 +287,12 @@ struct Online {
   __device__ __forceinline__ Online() : top(-INFINITY), M(-0x1p24f), s0(0.f), s1(0.f), t(0.f) {}
 };
 
-template <typename T> using LooseVec = __attribute__((ext_vector_type(4), aligned(sizeof(T)))) uint32_t;
+// the same as a vector, which the non-temporal load takes; spelt out for each size, since an alignment that depends on a template's
+// argument is dropped without a word (and 16 bytes assumed)
+typedef uint32_t LooseVec2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t LooseVec4 __attribute__((ext_vector_type(4), aligned(4)));
+template <int BYTES> struct LooseVecOf { typedef LooseVec2 type; };
+template <> struct LooseVecOf<4> { typedef LooseVec4 type; };
 
 template <typename T, int G, int NV> struct RowRegs {
   static constexpr int E = 16 / sizeof(T);
@@ -306,8 +311,9 @@ template <typename T, int G, int NV> struct RowRegs {
     return e + E <= n ? e : n - E;
   }
   template <bool ONCE> __device__ __forceinline__ void fetch(int r, const char* p) {
-    const LooseVec<T>* q = reinterpret_cast<const LooseVec<T>*>(p);
-    const LooseVec<T> u = ONCE ? __builtin_nontemporal_load(q) : *q;
+    typedef typename LooseVecOf<sizeof(T)>::type Vec;
+    const Vec* q = reinterpret_cast<const Vec*>(p);
+    const Vec u = ONCE ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[r][i] = u[i];
   }
