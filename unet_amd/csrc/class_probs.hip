@@ -465,11 +465,11 @@ template <typename T> __global__ __launch_bounds__(64) void lp_bwd_thread_kernel
         with_ref(q.m, k.c2, [&](const auto& ref) {
           if (wide) {                                      // C and so multiples of 16 bytes
             for (int c = 0; c < C; c += E) {
-              T v[E];
-              *reinterpret_cast<U4*>(v) = *reinterpret_cast<const U4*>(row + c);
+              alignas(16) T v[E];
+              *reinterpret_cast<Vec16*>(v) = *reinterpret_cast<const Vec16*>(row + c);
 #pragma unroll
               for (int j = 0; j < E; ++j) v[j] = (T)(q.of(ref, (float)v[j]) + (c + j == q.label ? q.own : 0.f));
-              *reinterpret_cast<U4*>(out + c) = *reinterpret_cast<const U4*>(v);
+              *reinterpret_cast<Vec16*>(out + c) = *reinterpret_cast<const Vec16*>(v);
             }
           } else {
             for (int c = 0; c < C; ++c) out[c] = (T)(q.of(ref, (float)row[c]) + (c == q.label ? q.own : 0.f));

@@ -279,20 +279,28 @@ __device__ __forceinline__ int renew_uniform(int C) {
 }
 
 // ---- a row in the registers of a group of lanes ------------------------------------------------------------------------------
-// 16 bytes wherever an element may lie: rows of odd sizes start anywhere (the hardware takes element-aligned vectors)
-template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Loose16 { uint32_t w[4]; };
+// 16 bytes wherever an element may lie: rows of odd sizes start anywhere (the hardware takes element-aligned vectors).  A vector
+// type, whose accesses the compiler takes to meet those of any other type: a class is read and written again by itself through
+// float* and the like.  Spelt out for each size, since an alignment that depends on a template's argument is dropped without a word
+// (and 16 bytes assumed).
+typedef uint32_t LooseVec2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t LooseVec4 __attribute__((ext_vector_type(4), aligned(4)));
+template <int BYTES> struct LooseVecOf { typedef LooseVec2 type; };
+template <> struct LooseVecOf<4> { typedef LooseVec4 type; };
+template <typename T> using LooseVec = typename LooseVecOf<sizeof(T)>::type;
+typedef uint32_t Vec16 __attribute__((ext_vector_type(4)));          // on 16 bytes: LDS
+
+// Between stores of one lane and those of another lane of the same wave to the same places: they leave in the order of the program.
+__device__ __forceinline__ void wave_stores_in_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 struct Online {
   float top, M, s0, s1, t;
   __device__ __forceinline__ Online() : top(-INFINITY), M(-0x1p24f), s0(0.f), s1(0.f), t(0.f) {}
 };
-
-// the same as a vector, which the non-temporal load takes; spelt out for each size, since an alignment that depends on a template's
-// argument is dropped without a word (and 16 bytes assumed)
-typedef uint32_t LooseVec2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t LooseVec4 __attribute__((ext_vector_type(4), aligned(4)));
-template <int BYTES> struct LooseVecOf { typedef LooseVec2 type; };
-template <> struct LooseVecOf<4> { typedef LooseVec4 type; };
 
 template <typename T, int G, int NV> struct RowRegs {
   static constexpr int E = 16 / sizeof(T);
@@ -311,9 +319,8 @@ template <typename T, int G, int NV> struct RowRegs {
     return e + E <= n ? e : n - E;
   }
   template <bool ONCE> __device__ __forceinline__ void fetch(int r, const char* p) {
-    typedef typename LooseVecOf<sizeof(T)>::type Vec;
-    const Vec* q = reinterpret_cast<const Vec*>(p);
-    const Vec u = ONCE ? __builtin_nontemporal_load(q) : *q;
+    const LooseVec<T>* q = reinterpret_cast<const LooseVec<T>*>(p);
+    const LooseVec<T> u = ONCE ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[r][i] = u[i];
   }
@@ -470,17 +477,17 @@ template <typename T, int G, int NV> struct RowRegs {
     }
   }
   template <typename F> __device__ __forceinline__ void put(int r, char* p, F f) const {
-    Loose16<T> u;
+    LooseVec<T> u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (sizeof(T) == 4) u.w[i] = __float_as_uint(f(get(r, i)));
+      if constexpr (sizeof(T) == 4) u[i] = __float_as_uint(f(get(r, i)));
       else {
         typedef __attribute__((ext_vector_type(2))) T T2;
         const T2 v = {(T)f(get(r, 2 * i)), (T)f(get(r, 2 * i + 1))};
-        u.w[i] = __builtin_bit_cast(uint32_t, v);
+        u[i] = __builtin_bit_cast(uint32_t, v);
       }
     }
-    *reinterpret_cast<Loose16<T>*>(p) = u;
+    *reinterpret_cast<LooseVec<T>*>(p) = u;
   }
 };
 
@@ -796,14 +803,14 @@ template <typename T> __device__ __forceinline__ void copy_to_lds(T* __restrict_
   const int lane = threadIdx.x;
   int i = lane * E;
   for (; i + E <= n; i += 64 * E)
-    *reinterpret_cast<U4*>(dst + i) = __builtin_bit_cast(U4, *reinterpret_cast<const Loose16<T>*>(src + i));
+    *reinterpret_cast<Vec16*>(dst + i) = *reinterpret_cast<const LooseVec<T>*>(src + i);
   for (int e = n / E * E + lane; e < n; e += 64) dst[e] = src[e];
 }
 template <typename T> __device__ __forceinline__ void copy_from_lds(T* __restrict__ dst, const T* __restrict__ src, int n) {
   constexpr int E = 16 / sizeof(T);
   const int lane = threadIdx.x;
   for (int i = lane * E; i + E <= n; i += 64 * E)
-    *reinterpret_cast<Loose16<T>*>(dst + i) = __builtin_bit_cast(Loose16<T>, *reinterpret_cast<const U4*>(src + i));
+    *reinterpret_cast<LooseVec<T>*>(dst + i) = *reinterpret_cast<const Vec16*>(src + i);
   for (int e = n / E * E + lane; e < n; e += 64) dst[e] = src[e];
 }
 // 64 rows that lie apart: one address for the wave and an offset of 32 bits for the lane (uh_apart checks that it fits), so that
@@ -853,8 +860,8 @@ template <typename T, int CREG> __device__ __forceinline__ void load_classes_wid
 #pragma unroll
   for (int c = 0; c < CREG; c += E)
     if (c < C) {
-      T v[E];
-      *reinterpret_cast<U4*>(v) = *reinterpret_cast<const U4*>(p + c);
+      alignas(16) T v[E];
+      *reinterpret_cast<Vec16*>(v) = *reinterpret_cast<const Vec16*>(p + c);
 #pragma unroll
       for (int j = 0; j < E; ++j) x[c + j] = c + j < C ? (float)v[j] : -INFINITY;
     } else {

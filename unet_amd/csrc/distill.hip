@@ -154,6 +154,7 @@ __global__ __launch_bounds__(64) void ds_quad_kernel(DsArgs a, const T* __restri
         else {
           with_wave_ref(s.m, a.c2, [&](const auto& ref) {
             reg.map_store(out, 0, C, lane, [&](float v) { return dense * ex2(ref.z(v)); });
+            wave_stores_in_order();
             group_fix<T, 16>(a, row, out, lane, q.sum, co, ref, inv_s, t_of, c_of);
           });
         }
@@ -302,6 +303,7 @@ __global__ __launch_bounds__(64) void ds_wave_kernel(DsArgs a, const T* __restri
       if (q.sum == 0.f) reg.map_store(out, 0, C, lane, [](float) { return 0.f; });
       else {
         with_ref(s.m, a.c2, [&](const auto& ref) { reg.map_store(out, 0, C, lane, [&](float v) { return dense * ex2(ref.z(v)); }); });
+        wave_stores_in_order();
         q.fix(a, out, 0, C, co, AnyRef(s.m, a.c2), inv_s);
       }
     }
