@@ -3,6 +3,7 @@
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch._C import _cuda_getCurrentRawStream as raw_stream       # current_stream() without making a Stream object
 
 from . import _lib
@@ -123,6 +124,14 @@ def fp32_rows(g):
     if g.dtype is not torch.float32:
         g = g.float()
     return g if g.is_contiguous() else g.contiguous()
+
+
+def refuse_tangents(what, *tensors):
+    """The kernels would leave a forward-mode tangent behind without a word."""
+    if forward_ad._current_level >= 0:                # inside a dual_level: outside of one there are none
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what}: the forward-mode gradient is not built")
 
 
 def checked_temperature(temperature, what):

@@ -14,7 +14,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import SLOTS_MAX, lib
-from .class_rows import DTYPE_CODE, INT_BYTES, Rows, byref, checked_temperature, fp32_rows
+from .class_rows import DTYPE_CODE, INT_BYTES, Rows, byref, checked_temperature, fp32_rows, refuse_tangents
 from .label_probs import label_log_probs
 
 
@@ -91,7 +91,7 @@ def _scale(r, reduction, what):
 
 def topk_distill(logits, top_logits, top_index, temperature=1.0, weight=None, reduction="mean", dim=1):
     """The distillation loss of a student's `logits` against a teacher's slots, a 0-dim fp32 tensor, differentiable with
-    respect to the logits (once):
+    respect to the logits (once, in reverse mode: forward-mode tangents are refused):
 
         t = softmax over the slots of top_logits / T,   p = softmax over the classes of logits / T
         loss = mean (or sum) over the rows of  weight * T^2 * sum_k t_k (ln t_k - ln p[top_index_k])
@@ -108,6 +108,7 @@ def topk_distill(logits, top_logits, top_index, temperature=1.0, weight=None, re
     r = Rows(logits, dim, what)
     temperature = checked_temperature(temperature, what)
     t = _Targets(r, top_logits, top_index, weight, what)
+    refuse_tangents(what, logits, top_logits, weight)
     scale = _scale(r, reduction, what)
     r.bind(what)
     if r.rows == 0:

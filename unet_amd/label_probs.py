@@ -14,7 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ._lib import TOP_MAX, lib
-from .class_rows import INT_BYTES, Rows, byref, checked_temperature, fp32_rows
+from .class_rows import INT_BYTES, Rows, byref, checked_temperature, fp32_rows, refuse_tangents
 
 LabelLogProbs = namedtuple("LabelLogProbs", "log_prob entropy top_log_prob top_index")
 
@@ -95,10 +95,11 @@ def label_log_probs(logits, labels=None, top=0, temperature=1.0, dim=1, ignore_i
     (there is no check that would have to wait for the device).  A row that holds a NaN or +inf gives NaN and indices -1;
     a row of nothing but -inf gives log_prob -inf, entropy 0 and no alternatives.
 
-    log_prob and entropy are differentiable with respect to the logits (once); the alternatives are not.  The gradient has
-    the logits' type; rows that are ignored or nothing but -inf get zeros."""
+    log_prob and entropy are differentiable with respect to the logits (once, in reverse mode: logits with a forward-mode
+    tangent are refused); the alternatives are not.  The gradient has the logits' type; rows that are ignored or nothing but -inf get zeros."""
     what = "label_log_probs"
     r = Rows(logits, dim, what)
+    refuse_tangents(what, logits)
     temperature = checked_temperature(temperature, what)
     top = int(top)
     if not 0 <= top <= min(TOP_MAX, r.classes):
