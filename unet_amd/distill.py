@@ -151,7 +151,8 @@ def teacher_targets(logits, top, dim=1):
 class TopKDistillLoss(nn.Module):
     """topk_distill as a criterion: forward(logits, targets) with targets = (top_logits, top_index) or (top_logits,
     top_index, weight).  The trainers (DataParallelTrainer, LUNeXtTrainer) take value and gradient from one pass
-    (`value_and_grad`); anything else may call it like any differentiable loss."""
+    (`value_and_grad`); anything else may call it like any differentiable loss, and so do the trainers with a subclass, whose
+    forward may add terms of its own."""
 
     def __init__(self, temperature=1.0, reduction="mean", dim=1):
         super().__init__()

@@ -376,7 +376,7 @@ class DataParallelTrainer:
         # d(mean over ranks of loss)/dlogits: the 1/world of gradient averaging is folded into the seed
         if self._fused_bce and masks.shape == logits.shape:
             loss, dlogits = bce_with_logits(logits.detach(), masks, 1.0 / self.world)
-        elif isinstance(self.criterion, TopKDistillLoss):      # masks: a teacher's targets
+        elif type(self.criterion) is TopKDistillLoss:          # masks: a teacher's targets (a subclass has a forward of its own)
             loss, dlogits = self.criterion.value_and_grad(logits.detach(), masks, 1.0 / self.world)
         else:
             loss = self.criterion(logits, masks)
@@ -470,7 +470,7 @@ class LUNeXtTrainer:
     all-reduced once per step (14 MB: one collective) and 1/world is folded into the loss gradient.
 
     criterion: "cl_dice", "bce", a TopKDistillLoss (train_step's masks are then a teacher's targets) or a callable
-    (logits, masks) -> loss, differentiated by autograd at the logits."""
+    (logits, masks) -> loss, differentiated by autograd at the logits; a subclass of TopKDistillLoss is such a callable."""
 
     def __init__(self, model, lr=1e-3, criterion="bce", process_group=None, standalone=False):
         from .lunext import flat_param_order
@@ -495,7 +495,7 @@ class LUNeXtTrainer:
             return cldice_with_logits(masks, logits, grad_scale=scale, prepared=prepared)
         if c == "bce" and masks.shape == logits.shape:
             return bce_with_logits(logits, masks, scale)
-        if isinstance(c, TopKDistillLoss):                     # masks: a teacher's targets
+        if type(c) is TopKDistillLoss:                         # masks: a teacher's targets (a subclass has a forward of its own)
             return c.value_and_grad(logits, masks, scale)
         fn = nn.BCEWithLogitsLoss() if c == "bce" else c
         lg = logits.detach().requires_grad_(True)
