@@ -95,8 +95,8 @@ __device__ __forceinline__ void band_epilogue(const GemmArgs& p, const f32x4 (&a
                                               const uint32_t (&fw)[4], int wm, int wn, int l15, int g, float* red,
                                               const float* coef, const uint2 (&yraw)[4][4]) {
   // While a workgroup is here none of its waves issues MFMAs, and at K = 64 this is a quarter of a tile's life,
-  // so the arithmetic is laid out for the packed fp32 instructions: values are handled as PAIRS OF ROWS (e, e+1),
-  // which are adjacent registers of one accumulator, so no register moves are needed to form the operands.
+  // so values are handled as PAIRS OF ROWS (e, e+1), which are adjacent registers of one accumulator: no register moves
+  // are needed to form operands (or packed fp32 ones, which the build forbids).
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   const int ncol = wn * 64 + l15 * 4;
   const int n0 = nt * BN;
