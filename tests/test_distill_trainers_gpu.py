@@ -73,3 +73,15 @@ def test_heavy_network(criterion, scaled):
         cos = (a.flatten() @ b.flatten()) / (a.norm() * b.norm())
         assert cos > 0.999 and abs((a.norm() / b.norm()).item() - 1.0) < 1e-2, name
     assert torch.isfinite(trainer.train_step(images, targets, scaler=scaler))
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_a_ranks_share_of_the_gradient(reduction):
+    """one of two ranks seeds its backward pass with half of its own loss's gradient (a power of two: the same bits, halved)"""
+    _, targets = made(True)
+    trainer = LUNeXtTrainer(unet_amd.LUNeXt(3, CLASSES).to(DEV).train(), criterion=TopKDistillLoss(2.0, reduction), standalone=True)
+    logits = torch.randn(2, CLASSES, 32, 48, generator=torch.Generator().manual_seed(4)).to(DEV)
+    loss, whole = trainer._loss(logits, targets)
+    trainer.world = 2
+    again, half = trainer._loss(logits, targets)
+    assert torch.equal(loss, again) and torch.equal(whole, half * 2.0)

@@ -48,7 +48,8 @@ struct LpArgs {
 // ---- rows whose classes lie side by side: 16 or 64 lanes a row, the row in registers -------------------------------------------
 // LIST > 0 (G = 16): up to LIST alternatives from the lanes' own falling lists; TOP (G = 64): any number.
 // 16 lanes where four loads each hold the row and no more than 8 alternatives are asked for (100000 rows of bf16, 16 and 64 lanes: 300
-// classes 17 and 40 us, 512 classes with 8 alternatives 85 and 121 us); 64 lanes up to 8 KB, past that a workgroup (bf16, 64
+// classes 17 and 40 us, 512 classes with 1 / 4 / 8 alternatives 46 / 52 / 80 and 97 / 107 / 114 us; 16 lanes with lists of 4 and 8, 300
+// classes, top 4: 44.5 and 57.1 us); 64 lanes up to 8 KB, past that a workgroup (bf16, 64
 // and 256 lanes: 20000 x 2000 19 and 26 us, 10000 x 4096 with 20 alternatives 39 and 48 us).
 template <typename T, int G, int NV, int LIST, bool TOP>
 __global__ __launch_bounds__(64) void lp_group_kernel(LpArgs a, const T* __restrict__ x) {
@@ -134,6 +135,7 @@ struct LpPart {
   uint32_t low;
   int count, pad[3];
 };
+// (0 / 16 / 32 / 64 more than `top`: 1024 x 131072 bf16, top 64 106 / 100 / 97.6 / 97.7 us; 4 x 32000, top 20 15.4 / 14.6 / 14.6 / 14.6)
 static inline int lp_keep(int top) { return top ? top + 32 : 0; }
 
 template <typename T, int NV, bool TOP>
@@ -238,8 +240,11 @@ __global__ __launch_bounds__(256) void lp_join_kernel(LpArgs a, const T* __restr
 }
 
 // ---- one thread per row ----------------------------------------------------------------------------------------------------------
-// up to 64 classes in registers (CREG), side by side through LDS (STAGED) or apart; LIST alternatives a sweep: instances of 2, 3,
-// 5 and 8, since what a place costs is paid for every class.  32 x 21 x 256 x 256 fp32, top 3: 51 us (176 MB read, 50 MB written,
+// up to 64 classes in registers (CREG), side by side through LDS (STAGED) or apart.  In 16, 32 and 64 registers: 8 x 16 x 256 x 256
+// fp32 8.3, 9.0 and 10.3 us; 8 x 32 x 256 x 256 - , 13.0 and 14.9.  LIST alternatives a sweep: instances of 2, 3, 5 and 8, since
+// what a place costs is paid for every class, and those that do not fit for another walk.  8 x 21 x 256 x 256 fp32 with a list of 2 /
+// 3 / 5 / 8: top 2 13.5 / 14.1 / 15.7 / 18.2 us, top 3 24.5 / 14.8 / 16.6 / 19.1, top 4 25.5 / 26.9 / 17.5 / 19.8, top 5 37.9 / 27.5 /
+// 18.2 / 20.7, top 6 38.4 / 27.8 / 31.4 / 21.2, top 8 51 / 41 / 33 / 22.2, top 9 63 / 42 / 34 / 38.  32 x 21 x 256 x 256 fp32, top 3: 51 us (176 MB read, 50 MB written,
 // 4.5 TB/s); 8 x 19 x 251 x 333 16.6 us, gradient 28 us.
 template <typename T, int CREG, bool STAGED, int LIST>
 __global__ __launch_bounds__(64) void lp_thread_kernel(LpArgs a, const T* __restrict__ x, bool wide) {
@@ -304,7 +309,8 @@ __global__ __launch_bounds__(64) void lp_thread_kernel(LpArgs a, const T* __rest
 }
 
 // more classes, lying apart: the thread walks its row, once for the statistics and the first LIST alternatives, and again for
-// every LIST more
+// every LIST more.  8 x 150 x 128 x 128 bf16 with a list of 4 and of 8: top 4 26.6 and 38.0 us, top 5 81.8 and 38.1; without
+// alternatives 15.3.
 template <typename T, int LIST>
 __global__ __launch_bounds__(64) void lp_walk_kernel(LpArgs a, const T* __restrict__ x) {
   const long long r = (long long)blockIdx.x * 64 + threadIdx.x;

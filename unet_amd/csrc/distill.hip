@@ -463,7 +463,9 @@ __global__ __launch_bounds__(256) void ds_rows_kernel(DsArgs a, const T* __restr
 
 // ---- one thread per row ----------------------------------------------------------------------------------------------------------
 // The teacher's softmax of a thread's own row.  KS > 0: at most KS slots, read once and kept; KS = 0: any number, read once for
-// the maximum, once for the sum and again for every use.
+// the maximum, once for the sum and again for every use.  Kept in 4 places and read again, step, 8 x 21 x 256 x 256 fp32: 1 slot 29.3
+// and 31.3 us, 2 32.3 and 35.1, 4 36.2 and 42.8; 2^20 x 12 bf16: 4 slots 38.9 and 54.1.  Kept in 8 places (no such instance) and
+// read again: 5 slots 38.9 and 46.4 us, 8 slots 44.8 and 44.9.
 // R: RowRef, where the caller sees to the rows for which it will not do, or AnyRef.
 template <int KS, typename R> struct ThreadTeacher {
   float vm, ln_sv, inv, sum;
