@@ -153,3 +153,19 @@ def test_parts_that_nobody_waits_for(dtype, temperature, fills, monkeypatch):
     monkeypatch.setenv("UNET_AMD_DISTILL_SPINS", "0")
     for a, b in zip(run(), want):
         assert torch.equal(a.reshape(-1).view(torch.uint8), b.reshape(-1).view(torch.uint8))
+
+
+@pytest.mark.parametrize("layout,c,repeat", PATHS)
+@pytest.mark.parametrize("dtype,temperature,most", [(torch.float32, 0.7, -3e38), (torch.float32, 1e-3, -1e36), (torch.bfloat16, 1e-6, -1e33),
+                                                    (torch.float32, 1.0, -3e38), (torch.bfloat16, 4.0, -3e38)])
+def test_masked_labels_in_rows_past_the_largest_quotient(layout, c, repeat, dtype, temperature, most):
+    """ln p of a class of -inf is -inf, also where the row's maximum over T is past the largest number"""
+    x = torch.randn(20, c, generator=torch.Generator().manual_seed(9)).double()
+    x[:10] = most
+    x[:, 1::2] = -float("inf")
+    x = x.to(dtype).repeat(repeat, 1)
+    x = x.to(DEV) if layout == "rows" else x.t().contiguous().view(1, c, -1, 5).to(DEV)
+    labels = probs.labels_for(x, 1, 7)
+    labels.view(-1)[::3] = 1
+    probs.check(x, labels, top=min(c, 5), temperature=temperature, grads=False)
+    check_gradient(x, labels, temperature)

@@ -109,10 +109,10 @@ template <typename F> __device__ __forceinline__ void with_wave_ref(float m, flo
 struct RowStat { float m, s, t; };
 
 // (x - m) / T of a reported value; x - m may overflow where its quotient does not (a class masked with the type's lowest
-// value, T > 1)
+// value, T > 1).  Fused, since m / T may overflow as well: beside x = -inf that would be a NaN.
 __device__ __forceinline__ float scaled(float x, float m, float inv_t) {
   const float d = x - m;
-  return d == -INFINITY ? x * inv_t - m * inv_t : d * inv_t;
+  return d == -INFINITY ? fmaf(-m, inv_t, x * inv_t) : d * inv_t;
 }
 
 // The exponent that takes sums relative to the point of the maximum m0 to that of m >= m0.

@@ -102,7 +102,8 @@ def topk_distill(logits, top_logits, top_index, temperature=1.0, weight=None, re
     counts twice.  weight: fp32 per row or None.
 
     Rows of weight 0 and rows without a filled slot count as 0 whatever they hold, and get zero gradients; the mean divides
-    by the number of all rows.  A class index past the last one, or a NaN, makes the loss NaN.  Without any row the loss is
+    by the number of all rows.  A slot whose t_k is below 2^-126, the smallest normal fp32 number, counts as t_k = 0, also where
+    the student gives its class no probability.  A class index past the last one, or a NaN, makes the loss NaN.  Without any row the loss is
     0.  The loss is summed in a fixed order: equal inputs give equal bits."""
     what = "topk_distill"
     r = Rows(logits, dim, what)
